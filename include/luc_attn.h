@@ -364,6 +364,126 @@ int luc_sort_and_sample(luc_ctx* ctx, void* stream, int dtype, const void* logit
                         float top_p, int top_k, float rand_val, void* sort_buffer,
                         size_t sort_buffer_bytes, uint32_t* out_idx);
 
+/* ---- Serving over a paged cache held on the GPU, in 16 or 4 bits ----------
+ * A serving step with no host work between its launches: pages for the new
+ * rows (luc_block_extend), their norms, rotation and cache write
+ * (luc_qk_norm_rope_append or luc_kv4_append), their attention
+ * (luc_kv4_attention over a 4-bit cache).  Every call may be captured in a HIP
+ * graph. */
+
+/* Block tables, slots and positions of a batch's new rows, from lengths kept on
+ * the device -- the free list and prepare_for_step of KVCache
+ * (src/layers/kv_cache.rs:73-76, 106-122) for many sequences, as luc_blocks_*
+ * below does it on the host.  All arrays are device memory:
+ *   new_tokens [batch]  tokens that each sequence gets, >= 0
+ *   lens [batch]        tokens that it holds, in ceil(lens / 16) pages; grows
+ *   block_tables [batch][table_stride]
+ *   free_list [num_blocks]  page ids; its first state[0] entries are free and
+ *                       handed out from the end (a free list of num_blocks - 1,
+ *                       ..., 0 hands out 0, 1, 2, ... as luc_blocks does)
+ *   state [4]           {free pages, status, used by the launch, unused}; all
+ *                       but the first zero at first use
+ *   slots, positions [rows]  of the packed new rows (sequence 0's first):
+ *                       slot = page * 16 + position % 16, or -1 for a page
+ *                       outside [0, num_blocks); both -1 past the last new row
+ *   cu_seqlens [batch + 1], start_pos [batch]  the rows of each sequence and the
+ *                       position of its first, as luc_paged_prefill and
+ *                       luc_kv4_attention take them
+ * Pages go to sequences in order.  All or nothing: a call that cannot be met
+ * takes nothing, leaves lens, tables and free list as they are, gives every
+ * sequence no rows (cu_seqlens 0, slots and positions -1) and sets bits of the
+ * status, which stays until the caller clears it: 1 free pages are short, 2 a
+ * table row is, 4 a length, count or the state is out of range, 8 rows is too
+ * small.  batch <= 4096 (else LUC_E_UNSUPPORTED), table_stride <= 2^26.  Calls
+ * on one free list must not overlap (one stream, in order). */
+int luc_block_extend(luc_ctx* ctx, void* stream, int batch, const int32_t* new_tokens, int32_t* lens,
+                     int32_t* block_tables, int table_stride, int32_t* free_list, int32_t* state,
+                     int num_blocks, int rows, int64_t* slots, int32_t* positions, int32_t* cu_seqlens,
+                     int32_t* start_pos);
+
+/* Shrinks sequences to min(lens, keep) tokens and puts the pages behind those
+ * back on the free list (keep 0: all of them; keep >= lens: the sequence stays
+ * as it is), their table entries to 0.  The exact inverse of luc_block_extend:
+ * the last sequence's pages go back first, and its last page first of them, so
+ * a step that is undone leaves the free list as it was.  A negative keep, or
+ * lengths that the tables or the pool cannot hold, change nothing and set
+ * status bit 4. */
+int luc_block_truncate(luc_ctx* ctx, void* stream, int batch, const int32_t* keep, int32_t* lens,
+                       int32_t* block_tables, int table_stride, int32_t* free_list, int32_t* state,
+                       int num_blocks);
+
+/* Norms of q's and k's heads, RoPE and the cache write of num_tokens rows in one
+ * pass, by slot: row r of q, k and v at + r * row_stride elements ([heads]
+ * [head_dim] each; the engine's qkv rows give three views),
+ *   x' = x + bias;  with norms given, x' = x' / sqrt(mean(x'^2) + eps) * norm
+ * over each head of q and k (q_norm, k_norm [head_dim], both or neither); then
+ * the rotation of luc_rope at positions[r], in f32 with one rounding at the
+ * end.  q goes to q_out (which may be q), k to the slot and, unless k_out is
+ * NULL, to k_out (which may be k); v + v_bias to the slot.  Without norms: the
+ * bits of luc_rope_append.  Slots are positions in the pool, page * 16 + offset;
+ * one outside [0, num_blocks * 16) is never an address (the row's cache write is
+ * skipped, as for a padding row), and a position outside [0, max_pos), the rows
+ * of the tables, leaves the row's outputs and its slot untouched.  Slots of one
+ * call are distinct.  Every operand 16-byte aligned (slots 8), row strides
+ * multiples of 8. */
+int luc_qk_norm_rope_append(luc_ctx* ctx, void* stream, int dtype, const void* q, const void* k,
+                            const void* v, int64_t row_stride, const void* q_bias, const void* k_bias,
+                            const void* v_bias, const void* q_norm, const void* k_norm, float eps,
+                            const float* cos_table, const float* sin_table, int max_pos,
+                            const int32_t* positions, const int64_t* slots, int num_tokens, void* q_out,
+                            int64_t q_out_stride, void* k_out, int64_t k_out_stride, void* k_pool,
+                            void* v_pool, int num_blocks, int layer, int num_layers, int num_q_heads,
+                            int num_kv_heads, int head_dim, int block_size);
+
+/* The 4-bit cache.  Pools are [num_blocks][num_layers][Hkv] slabs of
+ * luc_kv4_page_bytes(head_dim) = 10 * head_dim bytes (16 tokens of one head; 32 *
+ * head_dim in 16 bits).  32 consecutive dimensions of a token's head share a step
+ * s and a minimum m in fp16 and are n * s + m, n in 0 .. 15:
+ *   K slab: n as [16 tokens][head_dim / 2 bytes], the even dimension in the low
+ *     half; then (s, m) as [16 tokens][head_dim / 32][2]
+ *   V slab: n as [2 halves of the page][head_dim / 4][8 tokens][2 bytes], four
+ *     dimensions of a token in two bytes, the first lowest; then
+ *     [2 halves][head_dim / 32][s, m][8 tokens]
+ * luc_kv4_append is luc_qk_norm_rope_append into such pools.  Of the values as
+ * they would go to a 16-bit pool, clamped to +-60000: m = fp16(min), s =
+ * fp16((max - m) / 15), n = rint((x - m) / s); a group with a NaN is all NaN.
+ * k_out and v_out, either NULL or not, get what the cache now holds, rounded to
+ * dtype. */
+size_t luc_kv4_page_bytes(int head_dim);
+int luc_kv4_append(luc_ctx* ctx, void* stream, int dtype, const void* q, const void* k, const void* v,
+                   int64_t row_stride, const void* q_bias, const void* k_bias, const void* v_bias,
+                   const void* q_norm, const void* k_norm, float eps, const float* cos_table,
+                   const float* sin_table, int max_pos, const int32_t* positions, const int64_t* slots,
+                   int num_tokens, void* q_out, int64_t q_out_stride, void* k_out, void* v_out,
+                   int64_t kv_out_stride, void* k_pool, void* v_pool, int num_blocks, int layer,
+                   int num_layers, int num_q_heads, int num_kv_heads, int head_dim, int block_size);
+
+/* Attention of a batch's rows over a 4-bit cache, whose entries for those rows
+ * are written (luc_kv4_append): rows cu_seqlens[b] .. cu_seqlens[b+1] - 1 of q and
+ * out are sequence b's, at positions start_pos[b] on of table row b, and row i of
+ * them attends to positions 0 .. start_pos[b] + i.  cu_seqlens NULL: one row a
+ * sequence (a decode step; total_rows = batch, start_pos the positions).
+ * total_rows, max_rows and max_ctx are host-side bounds: of cu_seqlens[batch], of
+ * a sequence's rows and of its start_pos plus rows.  Rows at and past
+ * cu_seqlens[batch] stay as they are.  A sequence beyond max_rows or max_ctx, or
+ * at a negative position, gets NaN outputs; so do rows whose context reaches a
+ * page outside [0, num_blocks).  What the cache holds behind a row's own
+ * position (NaN too) does not reach the row.  q 16-byte aligned with a row stride
+ * that is a multiple of 8; out 8-byte aligned and 4.  max_ctx <= 2^30.
+ * The workspace holds luc_kv4_workspace_size bytes (0: none needed), 256-byte
+ * aligned, zero-filled once before its first use; every launch leaves it ready
+ * for the next, whatever that one's sizes, if it is large enough for it.
+ * Launches that may run at the same time need separate workspaces. */
+size_t luc_kv4_workspace_size(int batch, int total_rows, int max_rows, int max_ctx, int num_q_heads,
+                              int num_kv_heads, int head_dim);
+int luc_kv4_attention(luc_ctx* ctx, void* stream, int dtype, void* out, int64_t out_row_stride,
+                      const void* q, int64_t q_row_stride, const void* k_pool, const void* v_pool,
+                      const int32_t* block_tables, int table_stride, int num_blocks,
+                      const int32_t* cu_seqlens, const int32_t* start_pos, int batch, int total_rows,
+                      int max_rows, int max_ctx, int layer, int num_layers, int num_q_heads,
+                      int num_kv_heads, int head_dim, int block_size, float sm_scale, void* workspace,
+                      size_t workspace_bytes);
+
 /* ---- Multi-sequence page allocator (host only: no GPU call, no ctx) ------
  * Generalises KVCache's free list and prepare_for_step
  * (src/layers/kv_cache.rs:73-76, 106-122) from one sequence to max_seqs rows

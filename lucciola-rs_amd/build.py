@@ -25,6 +25,7 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 ARCH = "gfx950"
 
 KERNELS = ["rope_append", "paged_decode", "paged_decode_w8", "paged_prefill", "model_ops", "prompt_gemm",
+           "block_map", "norm_append", "kv4_attention",
            "sampling", "probe_gather"]
 # code objects built from another object's source with extra flags
 KERNEL_SOURCES = {"paged_decode_w8": ("paged_decode", ["-DLUC_DECODE_WIDE"])}
@@ -81,7 +82,7 @@ def build_host(verbose=False):
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wextra",
           "-D__HIP_PLATFORM_AMD__", "-I", os.path.join(ROCM, "include"),
           "-I", os.path.join(ROOT, "include"), os.path.join(CSRC, "luc_attn.cpp"),
-          os.path.join(CSRC, "luc_blocks.cpp"), scratch,
+          os.path.join(CSRC, "luc_blocks.cpp"), os.path.join(CSRC, "luc_kv4.cpp"), scratch,
           "-L", os.path.join(ROCM, "lib"), "-lamdhip64", f"-Wl,-rpath,{ROCM}/lib",
           "-o", tmp], verbose)
     os.replace(tmp, out)

@@ -10,10 +10,8 @@
 // After luc_init the context is read-only, so one context may be used from
 // several threads, each with its own stream.  Nothing here allocates device
 // memory or synchronises.
-#include "luc_attn.h"
+#include "luc_internal.h"
 #include "kernels/decode_args.h"
-
-#include <hip/hip_runtime_api.h>
 
 #include <dlfcn.h>
 
@@ -23,34 +21,18 @@
 #include <cstdio>
 #include <cstring>
 #include <string>
-#include <unordered_map>
 #include <vector>
-
-struct luc_ctx {
-  int device = 0;
-  int num_cus = 0;
-  void* scratch = nullptr;  // this device's copy of the library scratch (luc_scratch.hip)
-  std::vector<hipModule_t> modules;
-  std::unordered_map<std::string, hipFunction_t> fns;
-};
-
-namespace luc_internal {
-int scratch_setup(int device, void** out);
-}
 
 namespace {
 
-thread_local std::string g_err;
+using luc_internal::aligned;
+using luc_internal::ceil_div;
+using luc_internal::check_device;
+using luc_internal::fail;
+using luc_internal::get_fn;
+using luc_internal::launch;
 
-int fail(int code, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof buf, fmt, ap);
-  va_end(ap);
-  g_err = buf;
-  return code;
-}
+thread_local std::string g_err;
 
 #define LUC_HIP(expr)                                                                  \
   do {                                                                                 \
@@ -61,7 +43,9 @@ int fail(int code, const char* fmt, ...) {
 constexpr const char* kCodeObjects[] = {"rope_append.hsaco",   "paged_decode.hsaco",
                                          "paged_decode_w8.hsaco", "paged_prefill.hsaco",
                                          "model_ops.hsaco",     "prompt_gemm.hsaco",
-                                         "sampling.hsaco",      "probe_gather.hsaco"};
+                                         "sampling.hsaco",      "probe_gather.hsaco",
+                                         "block_map.hsaco",     "norm_append.hsaco",
+                                         "kv4_attention.hsaco"};
 
 // Kernel-side constants (kept in step with csrc/kernels/paged_decode.hip):
 // four waves per workgroup, which share one split; tiles of 64 tokens
@@ -88,10 +72,6 @@ constexpr int kPlanTiles = 256 * 4 * 2;
 
 const char* dt_name(int dtype) { return dtype == LUC_F16 ? "f16" : "bf16"; }
 
-bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
-
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 std::string self_dir() {
   Dl_info info;
   if (dladdr(reinterpret_cast<void*>(&luc_init), &info) && info.dli_fname) {
@@ -100,22 +80,6 @@ std::string self_dir() {
     return s == std::string::npos ? std::string(".") : p.substr(0, s);
   }
   return ".";
-}
-
-int get_fn(const luc_ctx* ctx, const std::string& name, hipFunction_t* fn) {
-  auto it = ctx->fns.find(name);
-  if (it == ctx->fns.end()) return fail(LUC_E_LOAD, "kernel %s not loaded", name.c_str());
-  *fn = it->second;
-  return LUC_OK;
-}
-
-int check_device(const luc_ctx* ctx) {
-  int cur = -1;
-  LUC_HIP(hipGetDevice(&cur));
-  if (cur != ctx->device)
-    return fail(LUC_E_INVALID, "current device %d differs from the context's device %d", cur,
-                ctx->device);
-  return LUC_OK;
 }
 
 int check_common(const luc_ctx* ctx, int dtype, int head_dim) {
@@ -130,12 +94,6 @@ int check_heads(int hq, int hkv) {
   if (hq <= 0 || hkv <= 0) return fail(LUC_E_INVALID, "head counts must be positive");
   if (hq % hkv) return fail(LUC_E_INVALID, "num_q_heads %d not a multiple of num_kv_heads %d", hq, hkv);
   if (hq / hkv > 8) return fail(LUC_E_UNSUPPORTED, "group size %d > 8", hq / hkv);
-  return LUC_OK;
-}
-
-int launch(hipFunction_t fn, dim3 grid, dim3 block, void* stream, void** args) {
-  LUC_HIP(hipModuleLaunchKernel(fn, grid.x, grid.y, grid.z, block.x, block.y, block.z, 0,
-                                reinterpret_cast<hipStream_t>(stream), args, nullptr));
   return LUC_OK;
 }
 
@@ -584,6 +542,28 @@ int fail(int code, const char* fmt, ...) {
   g_err = buf;
   return code;
 }
+
+int get_fn(const luc_ctx* ctx, const std::string& name, hipFunction_t* fn) {
+  auto it = ctx->fns.find(name);
+  if (it == ctx->fns.end()) return fail(LUC_E_LOAD, "kernel %s not loaded", name.c_str());
+  *fn = it->second;
+  return LUC_OK;
+}
+
+int check_device(const luc_ctx* ctx) {
+  int cur = -1;
+  LUC_HIP(hipGetDevice(&cur));
+  if (cur != ctx->device)
+    return fail(LUC_E_INVALID, "current device %d differs from the context's device %d", cur,
+                ctx->device);
+  return LUC_OK;
+}
+
+int launch(hipFunction_t fn, dim3 grid, dim3 block, void* stream, void** args) {
+  LUC_HIP(hipModuleLaunchKernel(fn, grid.x, grid.y, grid.z, block.x, block.y, block.z, 0,
+                                reinterpret_cast<hipStream_t>(stream), args, nullptr));
+  return LUC_OK;
+}
 }  // namespace luc_internal
 
 extern "C" {
@@ -643,6 +623,7 @@ int luc_init(int device, const char* code_object_dir, luc_ctx** out_ctx) {
           names.push_back(n + "_t2w8");
         }
   }
+  for (const std::string& n : luc_internal::kv4_kernel_names()) names.push_back(n);
   for (const auto& n : names) {
     hipFunction_t fn = nullptr;
     for (hipModule_t m : ctx->modules)

@@ -70,6 +70,20 @@ SIGNATURES = {
     "luc_gather_floor": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _i32, _i32,
                                 _i32, _i32, _vp]),
     "luc_stream_read": (_i32, [_vp, _vp, _vp, _sz, _vp]),
+    "luc_block_extend": (_i32, [_vp, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _i32, _vp, _vp,
+                                _vp, _vp]),
+    "luc_block_truncate": (_i32, [_vp, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _i32]),
+    "luc_qk_norm_rope_append": (_i32, [_vp, _vp, _i32, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp,
+                                       _f32, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _i64, _vp, _i64,
+                                       _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "luc_kv4_page_bytes": (_sz, [_i32]),
+    "luc_kv4_append": (_i32, [_vp, _vp, _i32, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _f32,
+                              _vp, _vp, _i32, _vp, _vp, _i32, _vp, _i64, _vp, _vp, _i64, _vp, _vp,
+                              _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "luc_kv4_workspace_size": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "luc_kv4_attention": (_i32, [_vp, _vp, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _i32,
+                                 _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
+                                 _i32, _f32, _vp, _sz]),
     "luc_blocks_create": (_i32, [_i32, _i32, _i32, ctypes.POINTER(_vp)]),
     "luc_blocks_destroy": (None, [_vp]),
     "luc_blocks_reserve": (_i32, [_vp, _i32, _i32]),
@@ -362,6 +376,157 @@ class LucAttn:
         self._check(self.lib.luc_embedding(self.ctx, _stream(stream), dtype_code(table), _p(out),
                                            _p(table), _p(ids), ids.numel(), table.shape[0],
                                            table.shape[1]))
+
+    # ---- serving over a cache held on the GPU ----
+    @staticmethod
+    def _arrays(name, device, **arrays):
+        """Operands of the page maps: contiguous, on the device, of the dtype and at least
+        the elements that each is given with."""
+        for key, (t, dtype, least) in arrays.items():
+            if t.dtype != dtype or t.device != device or not t.is_contiguous() or t.numel() < least:
+                raise ValueError(f"{name}: {key} {tuple(t.shape)} {t.dtype} on {t.device}: want "
+                                 f"contiguous {dtype} of at least {least} elements on {device}")
+
+    def block_extend(self, new_tokens, lens, tables, free_list, state, slots, positions, cu_seqlens,
+                     start_pos, stream=None):
+        """luc_block_extend: pages, slots and positions for new_tokens[b] more tokens of each
+        sequence b.  tables int32 [B, pages]; free_list int32 [num_blocks]; state int32 [4];
+        slots int64 and positions int32 of one length, the most rows of the batch; the others
+        int32 [B], cu_seqlens [B + 1]."""
+        batch, stride = tables.shape
+        i32, rows = torch.int32, slots.numel()
+        self._arrays("block_extend", tables.device, new_tokens=(new_tokens, i32, batch),
+                     lens=(lens, i32, batch), tables=(tables, i32, 0), free_list=(free_list, i32, 1),
+                     state=(state, i32, 4), slots=(slots, torch.int64, 0),
+                     positions=(positions, i32, rows), cu_seqlens=(cu_seqlens, i32, batch + 1),
+                     start_pos=(start_pos, i32, batch))
+        self._check(self.lib.luc_block_extend(
+            self.ctx, _stream(stream), batch, _p(new_tokens), _p(lens), _p(tables), stride,
+            _p(free_list), _p(state), free_list.numel(), rows, _p(slots), _p(positions),
+            _p(cu_seqlens), _p(start_pos)))
+
+    def block_truncate(self, keep, lens, tables, free_list, state, stream=None):
+        """luc_block_truncate: sequence b back to at most keep[b] tokens, its pages behind those
+        to the free list."""
+        batch, stride = tables.shape
+        i32 = torch.int32
+        self._arrays("block_truncate", tables.device, keep=(keep, i32, batch),
+                     lens=(lens, i32, batch), tables=(tables, i32, 0), free_list=(free_list, i32, 1),
+                     state=(state, i32, 4))
+        self._check(self.lib.luc_block_truncate(
+            self.ctx, _stream(stream), batch, _p(keep), _p(lens), _p(tables), stride, _p(free_list),
+            _p(state), free_list.numel()))
+
+    @staticmethod
+    def _rows(name, t, heads, head_dim):
+        """Rows and row stride of a [rows, heads * head_dim] view (or [rows, heads, head_dim])."""
+        width = heads * head_dim
+        if t.dim() == 3 and t.shape[1:] == (heads, head_dim) and t.stride(1) == head_dim:
+            inner, shape = t.stride(2), width
+        else:
+            inner, shape = t.stride(-1), t.shape[-1] if t.dim() == 2 else -1
+        if shape != width or inner != 1:
+            raise ValueError(f"{name} {tuple(t.shape)} with strides {t.stride()}: want rows of {width} "
+                             "consecutive elements")
+        return t.shape[0], t.stride(0)
+
+    def _append(self, fn, q, k, v, cos, sin, positions, slots, k_pool, v_pool, num_blocks, layer,
+                num_layers, hq, hkv, head_dim, q_norm, k_norm, eps, biases, q_out, outs, block_size,
+                stream):
+        rows, stride = self._rows("q", q, hq, head_dim)
+        for name, t in (("k", k), ("v", v)):
+            if self._rows(name, t, hkv, head_dim) != (rows, stride) and rows:
+                raise ValueError(f"{name}'s rows and their stride differ from q's")
+        dtype = dtype_code(q)
+        if q_out is None:
+            q_out = q
+        o_rows, o_stride = self._rows("q_out", q_out, hq, head_dim)
+        kv_strides = [self._rows("k_out / v_out", t, hkv, head_dim) for t in outs if t is not None]
+        if o_rows != rows or any(s != (rows, kv_strides[0][1]) for s in kv_strides):
+            raise ValueError("outputs of other row counts (or strides, of k_out and v_out)")
+        norms = [t for t in (q_norm, k_norm) if t is not None]
+        if any(t.numel() != head_dim or not t.is_contiguous() for t in norms):
+            raise ValueError(f"head norms of {head_dim} elements are wanted")
+        for t, n in zip(biases, (hq, hkv, hkv)):
+            if t is not None and (t.numel() != n * head_dim or not t.is_contiguous()):
+                raise ValueError("a bias of other than its heads' elements")
+        if any(t.dtype != q.dtype for t in (k, v, q_out, *(t for t in (*outs, *norms, *biases) if t is not None))):
+            raise TypeError(f"operands of other types than q's {q.dtype}")
+        if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape or \
+                cos.dim() != 2 or cos.shape[1] != head_dim // 2 or not (cos.is_contiguous() and sin.is_contiguous()):
+            raise ValueError(f"rope tables {tuple(cos.shape)}: want fp32 [positions, {head_dim // 2}]")
+        self._arrays("append", q.device, positions=(positions, torch.int32, rows),
+                     slots=(slots, torch.int64, rows))
+        args = [self.ctx, _stream(stream), dtype, _p(q), _p(k), _p(v), stride, *map(_p, biases),
+                _p(q_norm), _p(k_norm), eps, _p(cos), _p(sin), cos.shape[0], _p(positions), _p(slots),
+                rows, _p(q_out), o_stride, *map(_p, outs), kv_strides[0][1] if kv_strides else 0,
+                _p(k_pool), _p(v_pool), num_blocks, layer, num_layers, hq, hkv, head_dim, block_size]
+        self._check(fn(*args))
+
+    def qk_norm_rope_append(self, q, k, v, cos, sin, positions, slots, k_pool, v_pool, layer, num_layers,
+                            hq, hkv, head_dim, q_norm=None, k_norm=None, eps=1e-6, q_bias=None,
+                            k_bias=None, v_bias=None, q_out=None, k_out=None, block_size=16,
+                            stream=None, num_blocks=None):
+        """luc_qk_norm_rope_append: bias, head norms, RoPE and the write to `slots` (int64, as
+        block_extend gives them) of the rows q [rows, hq * d], k and v [rows, hkv * d] (views with
+        one row stride, as those into a qkv tensor); q_out (default: q itself) gets q, k_out, if
+        given, k."""
+        if k_pool.dtype != q.dtype or v_pool.dtype != q.dtype:
+            raise TypeError(f"pools of other types than q's {q.dtype}")
+        nb = num_blocks if num_blocks is not None else pool_pages(k_pool, num_layers, hkv, head_dim)
+        self._append(self.lib.luc_qk_norm_rope_append, q, k, v, cos, sin, positions, slots, k_pool,
+                     v_pool, nb, layer, num_layers, hq, hkv, head_dim, q_norm, k_norm, eps,
+                     (q_bias, k_bias, v_bias), q_out, (k_out,), block_size, stream)
+
+    def kv4_pages(self, pool, num_layers, hkv, head_dim) -> int:
+        """Pages in a 4-bit pool: uint8 [pages, layers, kv heads, 10 * head_dim]."""
+        want = (num_layers, hkv, self.lib.luc_kv4_page_bytes(head_dim))
+        if pool.dtype != torch.uint8 or not pool.is_contiguous() or tuple(pool.shape[1:]) != want:
+            raise ValueError(f"4-bit pool {tuple(pool.shape)} {pool.dtype}: want contiguous uint8 "
+                             f"[pages, {', '.join(map(str, want))}]")
+        return int(pool.shape[0])
+
+    def kv4_append(self, q, k, v, cos, sin, positions, slots, k_pool, v_pool, layer, num_layers, hq, hkv,
+                   head_dim, q_norm=None, k_norm=None, eps=1e-6, q_bias=None, k_bias=None, v_bias=None,
+                   q_out=None, k_out=None, v_out=None, block_size=16, stream=None, num_blocks=None):
+        """luc_kv4_append: qk_norm_rope_append into 4-bit pools; k_out and v_out, if given, get
+        the values that the cache holds now."""
+        pages = min(self.kv4_pages(k_pool, num_layers, hkv, head_dim),
+                    self.kv4_pages(v_pool, num_layers, hkv, head_dim))
+        self._append(self.lib.luc_kv4_append, q, k, v, cos, sin, positions, slots, k_pool, v_pool,
+                     pages if num_blocks is None else num_blocks, layer, num_layers, hq, hkv, head_dim,
+                     q_norm, k_norm, eps, (q_bias, k_bias, v_bias), q_out, (k_out, v_out), block_size,
+                     stream)
+
+    def kv4_workspace(self, batch, total_rows, max_rows, max_ctx, hq, hkv, head_dim, device=None):
+        """A zero-filled workspace for kv4_attention calls of these sizes (None: none needed)."""
+        need = self.lib.luc_kv4_workspace_size(batch, total_rows, max_rows, max_ctx, hq, hkv, head_dim)
+        if need == 0:
+            return None
+        return torch.zeros(need // 4, dtype=torch.float32,
+                           device=device if device is not None else f"cuda:{self.device}")
+
+    def kv4_attention(self, out, q, k_pool, v_pool, tables, start_pos, batch, total_rows, max_rows,
+                      max_ctx, layer, num_layers, hq, hkv, head_dim, sm_scale, cu_seqlens=None,
+                      workspace=None, block_size=16, stream=None, num_blocks=None):
+        """luc_kv4_attention: out and q [rows, hq * d]; start_pos int32 [batch]; cu_seqlens int32
+        [batch + 1], or None for one row a sequence; workspace from kv4_workspace."""
+        rows, q_stride = self._rows("q", q, hq, head_dim)
+        o_rows, o_stride = self._rows("out", out, hq, head_dim)
+        if min(rows, o_rows) < total_rows or out.dtype != q.dtype:
+            raise ValueError(f"kv4_attention: q {tuple(q.shape)} {q.dtype}, out {tuple(out.shape)} {out.dtype} "
+                             f"for {total_rows} rows")
+        more = {} if cu_seqlens is None else {"cu_seqlens": (cu_seqlens, torch.int32, batch + 1)}
+        self._arrays("kv4_attention", q.device, tables=(tables, torch.int32, batch * tables.shape[-1]),
+                     start_pos=(start_pos, torch.int32, batch), **more)
+        pages = min(self.kv4_pages(k_pool, num_layers, hkv, head_dim),
+                    self.kv4_pages(v_pool, num_layers, hkv, head_dim))
+        ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+        self._check(self.lib.luc_kv4_attention(
+            self.ctx, _stream(stream), dtype_code(q), _p(out), o_stride, _p(q), q_stride, _p(k_pool),
+            _p(v_pool), _p(tables), tables.shape[-1], pages if num_blocks is None else num_blocks,
+            _p(cu_seqlens), _p(start_pos), batch, total_rows, max_rows, max_ctx, layer, num_layers, hq,
+            hkv, head_dim, block_size, sm_scale, _p(workspace), ws_bytes))
 
     def gather_floor(self, k_pool, v_pool, tables, positions, batch, max_ctx, layer, num_layers,
                      hkv, head_dim, sink, stream=None):

@@ -48,7 +48,8 @@ def build():
     _run(["g++", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wextra", *SAN,
           "-D__HIP_PLATFORM_AMD__",
           "-I", os.path.join(ROCM, "include"), "-I", os.path.join(ROOT, "include"),
-          os.path.join(CSRC, "luc_attn.cpp"), os.path.join(CSRC, "luc_blocks.cpp"), scratch,
+          os.path.join(CSRC, "luc_attn.cpp"), os.path.join(CSRC, "luc_blocks.cpp"),
+          os.path.join(CSRC, "luc_kv4.cpp"), scratch,
           "-L", os.path.join(ROCM, "lib"), "-lamdhip64", f"-Wl,-rpath,{ROCM}/lib",
           "-o", os.path.join(OUT, "liblucattn.so")])
     _run(["gcc", "-std=c11", "-fPIC", "-shared", "-fopenmp", "-ffp-contract=off",
