@@ -47,10 +47,15 @@ struct Kv4AttnArgs {
   int32_t batch, total_rows, max_rows, max_ctx, layer, num_layers, hkv, group, num_blocks;
   int32_t tiles;         // column tiles (chunks) per (sequence, kv head)
   int32_t splits, split_tokens;
+  int32_t longest_first;
   float qk_scale_log2;
 };
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+// The running maximum moves when a score (in powers of two) passes it by this: weights are at most
+// 8, and 8 s below fp16's limit for every s of the format (8000 at most).
+constexpr float kKv4Lazy = 3.0f;
 
 __device__ inline f32x4_t mfma16(uint4 a, uint4 b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
@@ -62,7 +67,8 @@ __device__ inline uint32_t as_u(half2_t x) { return __builtin_bit_cast(uint32_t,
 
 // The four pairs (n i, n i + 4) of a dword's n, times s plus m, as packed fp16.
 __device__ inline void expand8(uint32_t w, half2_t s, half2_t m, uint32_t* o) {
-  constexpr uint32_t kBig = 0x64006400u;  // 1024.0 twice
+  uint32_t kBig = 0x64006400u;  // 1024.0 twice
+  asm("" : "+v"(kBig));         // in a VGPR: v_and_or_b32 takes one scalar operand, the mask
   const half2_t big = {(_Float16)1024.0f, (_Float16)1024.0f};
   const half2_t sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f}, less = {(_Float16)-64.0f, (_Float16)-64.0f};
   const uint32_t v = w >> 8;
@@ -80,6 +86,37 @@ __device__ inline void expand8(uint32_t w, half2_t s, half2_t m, uint32_t* o) {
 // infinities: an exponent of all ones is NaN).
 __device__ inline uint32_t kv4_nan(uint32_t s, uint32_t m) {
   return (((s & 0x7c007c00u) + 0x04000400u) | ((m & 0x7c007c00u) + 0x04000400u)) & 0x80008000u;
+}
+
+// s and m of V for the lane's tokens first .. first + 7, of half h of its dimensions, in a tile
+// at some column's edge.  Tokens that no column sees (from ctx on) hold anything: their s and m
+// become 0.  A NaN value that only some columns see must not reach the others through 0 * NaN: it
+// becomes 0 too, and nan_at, the first such position in group 2 h + g / 2, the one of the lane's
+// outputs, tells which columns get their NaN after the last tile.
+__device__ __attribute__((always_inline)) inline void kv4_mask_values(u32x4_t& vs, u32x4_t& vm, int first, int ctx, int g, int& nan_at) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t keep = (first + 2 * i < ctx ? 0xffffu : 0u) | (first + 2 * i + 1 < ctx ? 0xffff0000u : 0u);
+    vs[i] &= keep;
+    vm[i] &= keep;
+    any |= kv4_nan(vs[i], vm[i]);
+  }
+  if (!__any(any != 0)) return;
+  int at = 0x7fffffff;
+#pragma unroll
+  for (int i = 3; i >= 0; --i) {
+    const uint32_t nan = kv4_nan(vs[i], vm[i]);
+    if (nan & 0x80000000u) at = first + 2 * i + 1;
+    if (nan & 0x8000u) at = first + 2 * i;
+    const uint32_t keep = (nan & 0x8000u ? 0u : 0xffffu) | (nan & 0x80000000u ? 0u : 0xffff0000u);
+    vs[i] &= keep;
+    vm[i] &= keep;
+  }
+  // first of group 2 h + n / 8, from its lanes to those of group 2 h + g / 2
+  at = min(at, __shfl_xor(at, 16));
+  at = min(at, __shfl_xor(at, 32));
+  nan_at = min(nan_at, __shfl(at, 8 * (g >> 1)));
 }
 
 // What a lane loads of a 32-token tile.
@@ -252,46 +289,17 @@ template <int DT, int D, int F> struct Kv4Wave {
     }
     // ---- output
     if (edge) {
-      // Tokens that no column sees hold anything: their s and m become 0.  A NaN value that
-      // only some columns see must not reach the others through 0 * NaN: it becomes 0 too, and
-      // the columns that see it get their NaN in finish().
-      uint32_t any = 0;
+      u32x4_t vs[H], vm[H];
 #pragma unroll
       for (int h = 0; h < H; ++h) {
-        uint32_t sw[4] = {t.vs[h].x, t.vs[h].y, t.vs[h].z, t.vs[h].w};
-        uint32_t mw[4] = {t.vm[h].x, t.vm[h].y, t.vm[h].z, t.vm[h].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t keep = (first + 2 * i < ctx ? 0xffffu : 0u) | (first + 2 * i + 1 < ctx ? 0xffff0000u : 0u);
-          sw[i] &= keep;
-          mw[i] &= keep;
-          any |= kv4_nan(sw[i], mw[i]);
-        }
-        t.vs[h] = make_uint4(sw[0], sw[1], sw[2], sw[3]);
-        t.vm[h] = make_uint4(mw[0], mw[1], mw[2], mw[3]);
+        vs[h] = __builtin_bit_cast(u32x4_t, t.vs[h]);
+        vm[h] = __builtin_bit_cast(u32x4_t, t.vm[h]);
       }
-      if (__any(any != 0)) {
 #pragma unroll
-        for (int h = 0; h < H; ++h) {
-          uint32_t sw[4] = {t.vs[h].x, t.vs[h].y, t.vs[h].z, t.vs[h].w};
-          uint32_t mw[4] = {t.vm[h].x, t.vm[h].y, t.vm[h].z, t.vm[h].w};
-          int at = 0x7fffffff;
-#pragma unroll
-          for (int i = 3; i >= 0; --i) {
-            const uint32_t nan = kv4_nan(sw[i], mw[i]);
-            if (nan & 0x80000000u) at = first + 2 * i + 1;
-            if (nan & 0x8000u) at = first + 2 * i;
-            const uint32_t keep = (nan & 0x8000u ? 0u : 0xffffu) | (nan & 0x80000000u ? 0u : 0xffff0000u);
-            sw[i] &= keep;
-            mw[i] &= keep;
-          }
-          t.vs[h] = make_uint4(sw[0], sw[1], sw[2], sw[3]);
-          t.vm[h] = make_uint4(mw[0], mw[1], mw[2], mw[3]);
-          // first such token of group 2 h + n / 8; the lane's outputs are of group 2 h + g / 2
-          at = min(at, __shfl_xor(at, 16));
-          at = min(at, __shfl_xor(at, 32));
-          nan_at[h] = min(nan_at[h], __shfl(at, 8 * (g >> 1)));
-        }
+      for (int h = 0; h < H; ++h) {
+        kv4_mask_values(vs[h], vm[h], first, ctx, g, nan_at[h]);
+        t.vs[h] = __builtin_bit_cast(uint4, vs[h]);
+        t.vm[h] = __builtin_bit_cast(uint4, vm[h]);
       }
     }
 #pragma unroll
@@ -408,26 +416,471 @@ __device__ inline float ws_get(const float* p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-constexpr int kTokWaves = 4;
-constexpr int kTokMaxSplits = 64;
+__device__ inline int pick2(bool c, int a, int b) {
+  int r = c ? a : b;
+  asm("" : "+v"(r));
+  return r;
+}
 
-// ---- waves split tokens: one workgroup per (split, sequence, kv head, 16-column tile) ----
+// ---- stages: what a wave keeps in LDS of the tokens ahead ------------------------------
+//
+// A stage is 5 KB: the slabs of 32 (D = 128) or 64 (D = 64) tokens, in 320 chunks of 16 bytes,
+// five loads of 64 lanes straight into LDS.  A lane's source is free, its place in LDS is not, so
+// chunks are dealt such that the reads below are conflict-free:
+//   K n      [sub-tile][fragment][group][token of the fragment]
+//   V n      [sub-tile][group][octet][quad of the group]
+//   K (s, m) [sub-tile][token of the octet (pairs, D = 64)][octet]
+//   V s, V m [sub-tile][group][octet]
+template <int D> struct Kv4Stage {
+  static constexpr int SUB = D == 128 ? 1 : 2;  // 32-token sub-tiles
+  static constexpr int TOKENS = 32 * SUB;
+  static constexpr int PAGES = 2 * SUB;
+  static constexpr int LOADS = 5;
+  static constexpr int BYTES = 1024 * LOADS;
+
+  const char* src[3];  // of the lane, in page 0: K n, V n, scales
+
+  __device__ __attribute__((always_inline)) inline void begin(const char* k_pool, const char* v_pool) {
+    const int l = threadIdx.x & 63;
+    const int n = l & 15;
+    // K: D = 128 fragment i, group l / 16; D = 64 sub-tile i, fragment l / 32, group (l / 16) % 2
+    const int tok = 8 * (n >> 2) + (n & 3) + (D == 128 ? 0 : 4 * (l >> 5));
+    src[0] = k_pool + Kv4<D>::k_row(tok & 15) + 16 * (D == 128 ? l >> 4 : (l >> 4) & 1);
+    // V: D = 128 groups 2 i and 2 i + 1; D = 64 sub-tile i
+    src[1] = v_pool + Kv4<D>::v_quad(l & 8, 8 * (l >> 5) + (l & 7));
+    if (l < 32) {
+      const int o = l & 3;
+      src[2] = k_pool + Kv4<D>::k_scale(D == 128 ? (8 * o + (l >> 2)) & 15 : 8 * (o & 1) + 2 * ((l >> 2) & 3), 0);
+    } else {
+      const int x = l & 15;
+      src[2] = v_pool + Kv4<D>::v_scale(x & 1, D == 128 ? x >> 2 : (x >> 2) & 1) + (l < 48 ? 0 : 16);
+    }
+  }
+  // The loads of a stage.  p0 ..: its pages (alike in all lanes; scalars, since an array indexed
+  // by lane would go through memory).
+  __device__ __attribute__((always_inline)) inline void issue(char* lds, int p0, int p1, int p2, int p3, uint32_t page_stride) const {
+    // the second page of two by a bit of the lane, as begin() deals tokens and octets
+    const int l = threadIdx.x & 63;
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      const bool odd = l & (v ? 16 : 8);
+      const char* const a = src[v] + (uint64_t)(uint32_t)pick2(odd, p1, p0) * page_stride;
+      to_lds(a, lds + 2048 * v);
+      // four rows of K on; 16 quads of V on
+      to_lds(D == 128 ? a + 256 : src[v] + (uint64_t)(uint32_t)pick2(odd, p3, p2) * page_stride, lds + 2048 * v + 1024);
+    }
+    int id = pick2(l & 2, p1, p0);
+    if constexpr (PAGES == 4) id = pick2(l < 32 ? l & 16 : l & 8, pick2(l & 2, p3, p2), id);
+    to_lds(src[2] + (uint64_t)(uint32_t)id * page_stride, lds + 4096);
+  }
+  __device__ static inline void to_lds(const char* a, char* lds) {
+    __builtin_amdgcn_global_load_lds(a, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+  }
+};
+
+// LDS reads of a sub-tile with their wait: the compiler would wait for every load into LDS
+// that is under way before a read that it can see.
+template <int D> struct Kv4Reads;
+template <> struct Kv4Reads<128> {
+  typedef uint32_t pair __attribute__((ext_vector_type(2)));
+  pair kw[4];       // K n: fragment a groups 0 1, 2 3, fragment b
+  uint32_t am[2];   // (s, m) of the fragments' tokens for the m term
+  u32x4_t sm[4];    // (s, m) of the lane's 4 tokens, a dword a group
+  u32x4_t v[4], vm;  // a group each: the lane's quads of it; m of group n
+  pair vs[4];        // s of the lane's 4 tokens
+  __device__ __attribute__((always_inline)) inline void read_k(uint32_t kw_at, uint32_t sm_at, uint32_t am_at, int) {
+    asm volatile(
+        "ds_read2st64_b32 %0, %10 offset1:1\n\tds_read2st64_b32 %1, %10 offset0:2 offset1:3\n\t"
+        "ds_read2st64_b32 %2, %10 offset0:4 offset1:5\n\tds_read2st64_b32 %3, %10 offset0:6 offset1:7\n\t"
+        "ds_read_b32 %4, %12 offset:4096\n\tds_read_b32 %5, %12 offset:4352\n\t"
+        "ds_read_b128 %6, %11 offset:4096\n\tds_read_b128 %7, %11 offset:4160\n\t"
+        "ds_read_b128 %8, %11 offset:4224\n\tds_read_b128 %9, %11 offset:4288\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(kw[0]), "=&v"(kw[1]), "=&v"(kw[2]), "=&v"(kw[3]), "=&v"(am[0]), "=&v"(am[1]), "=&v"(sm[0]), "=&v"(sm[1]), "=&v"(sm[2]),
+          "=&v"(sm[3])
+        : "v"(kw_at), "v"(sm_at), "v"(am_at)
+        : "memory");
+  }
+  __device__ __attribute__((always_inline)) inline void read_v(uint32_t v_at, uint32_t vs_at, uint32_t vm_at, int) {
+    asm volatile(
+        "ds_read_b128 %0, %9 offset:2048\n\tds_read_b128 %1, %9 offset:2560\n\t"
+        "ds_read_b128 %2, %9 offset:3072\n\tds_read_b128 %3, %9 offset:3584\n\t"
+        "ds_read_b64 %4, %10 offset:4608\n\tds_read_b64 %5, %10 offset:4672\n\t"
+        "ds_read_b64 %6, %10 offset:4736\n\tds_read_b64 %7, %10 offset:4800\n\t"
+        "ds_read_b128 %8, %11 offset:4864\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(vs[0]), "=&v"(vs[1]), "=&v"(vs[2]), "=&v"(vs[3]), "=&v"(vm)
+        : "v"(v_at), "v"(vs_at), "v"(vm_at)
+        : "memory");
+  }
+  __device__ inline uint32_t k(int b, int j) const { return kw[2 * b + (j >> 1)][j & 1]; }
+  __device__ inline uint32_t scale(int i, int j) const { return sm[i][j]; }
+};
+template <> struct Kv4Reads<64> {
+  typedef uint32_t pair __attribute__((ext_vector_type(2)));
+  pair kw[2];
+  uint32_t am[2];
+  u32x4_t sm[2];    // two tokens each, two groups
+  u32x4_t v[2], vm;
+  pair vs[2];
+  __device__ __attribute__((always_inline)) inline void read_k(uint32_t kw_at, uint32_t sm_at, uint32_t am_at, int u) {
+    asm volatile(
+        "ds_read2st64_b32 %0, %6 offset1:1\n\tds_read2st64_b32 %1, %6 offset0:2 offset1:3\n\t"
+        "ds_read_b32 %2, %8 offset:4096\n\tds_read_b32 %3, %8 offset:4224\n\t"
+        "ds_read_b128 %4, %7 offset:4096\n\tds_read_b128 %5, %7 offset:4160\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(kw[0]), "=&v"(kw[1]), "=&v"(am[0]), "=&v"(am[1]), "=&v"(sm[0]), "=&v"(sm[1])
+        : "v"(kw_at + u * 1024), "v"(sm_at + u * 256), "v"(am_at + u * 256)
+        : "memory");
+  }
+  __device__ __attribute__((always_inline)) inline void read_v(uint32_t v_at, uint32_t vs_at, uint32_t vm_at, int u) {
+    asm volatile(
+        "ds_read_b128 %0, %5 offset:2048\n\tds_read_b128 %1, %5 offset:2560\n\t"
+        "ds_read_b64 %2, %6 offset:4608\n\tds_read_b64 %3, %6 offset:4672\n\t"
+        "ds_read_b128 %4, %7 offset:4864\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(v[0]), "=&v"(v[1]), "=&v"(vs[0]), "=&v"(vs[1]), "=&v"(vm)
+        : "v"(v_at + u * 1024), "v"(vs_at + u * 128), "v"(vm_at + u * 128)
+        : "memory");
+  }
+  __device__ inline uint32_t k(int b, int j) const { return kw[b][j]; }
+  __device__ inline uint32_t scale(int i, int j) const { return sm[i >> 1][2 * (i & 1) + j]; }
+};
+
+// One wave's 8 columns over stages.  Of a fragment's 16 columns the lower 8 take fragment a's tokens
+// and the upper 8, the same rows and heads again, fragment b's: q is zero in the others' places, so
+// both fragments' products add up in one accumulator, a lane has 4 tokens of one column, and
+// softmax costs half of what 16 columns would.  The two halves of a column are partial results
+// like those of two waves.
+template <int DT, int D> struct Kv4Row {
+  static constexpr int NG = D / 32;  // groups of 32 dimensions
+  static constexpr bool HILO = DT == kF16;  // weights in two fp16 parts: see step()
+
+  uint4 q[2][NG];  // [fragment]; group j's dimensions 8 g .. + 7 of it, pairs (i, i + 4), i odd divided by 16
+  uint32_t qsum;   // k = 8 g, 8 g + 1: the sum of group g's dimensions, high and low part
+  // O^T: [group][c], rows 4 g + i of it are dimensions 16 (g % 2) + 4 i + 2 (g / 2) + c of the group, in
+  // units of 2^-20; and the m term, whose rows are groups
+  f32x4_t acc[NG][2], acc_m;
+  float m, l, scale;
+  float bar;       // products above it move m
+  int limit;
+  int lane, n, g;
+  uint32_t mask[2];  // of the pairs of fragment a's and b's tokens in P: the lane's or 0
+  uint32_t kw_at, sm_at, am_at, v_at, vs_at, vm_at;  // LDS offsets of the lane's reads in a stage
+
+  __device__ __attribute__((always_inline)) inline void begin(const Kv4AttnArgs& A, int64_t row0, int kvh, int start, int ctx, int col0,
+                                                              int ncols) {
+    lane = threadIdx.x & 63;
+    n = lane & 15;
+    g = lane >> 4;
+    const int half = n >> 3;
+    kw_at = n * 16 + g * 4;
+    sm_at = g * 16 + half * (D == 128 ? 256 : 128);
+    am_at = D == 128 ? ((n & 3) * 4 + (n >> 2)) * 16 + g * 4
+                     : (((n & 3) >> 1) * 4 + (n >> 2)) * 16 + (n & 1) * 8 + (g & 1) * 4;
+    v_at = (g * 8 + (n & 7)) * 16;
+    vs_at = g * 16 + half * 8;
+    vm_at = ((n & (NG - 1)) * 4 + g) * 16;
+    mask[0] = half ? 0 : ~0u;
+    mask[1] = ~mask[0];
+    const int col = col0 + (n & 7);
+    const bool on = col < ncols;
+    const int r = on ? col / A.group : 0, hd = on ? col % A.group : 0;
+    limit = on ? start + r : ctx - 1;
+    const uint16_t* const src = A.q + (row0 + r) * A.q_stride + ((int64_t)kvh * A.group + hd) * D + 8 * g;
+    float x[NG][8];
+    float top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      const uint4 w = on ? *(const uint4*)(src + 32 * j) : make_uint4(0, 0, 0, 0);
+      const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[j][2 * e] = St<DT>::lo(ww[e]);
+        x[j][2 * e + 1] = St<DT>::hi(ww[e]);
+        top = fmaxf(top, fmaxf(fabsf(x[j][2 * e]), fabsf(x[j][2 * e + 1])));
+      }
+    }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    // a power of two takes the largest element into [2^14, 2^15) (infinities and NaN stay so)
+    const int e = min(max((int)(__float_as_uint(top) >> 23), 15), 253);
+    const float up = copysignf(__uint_as_float((uint32_t)(268 - e) << 23), A.qk_scale_log2);
+    // n is 2^-24 n in the products: 2^(e - 127) 2^-14 2^24.  The scale's sign goes to q, so that
+    // the largest product is the largest score.
+    scale = fabsf(A.qk_scale_log2) * 1024.0f * __uint_as_float((uint32_t)e << 23);
+    if (scale == 0.0f) scale = 1e-37f;  // (a masked product, -inf, times 0 is NaN)
+    float mine = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      uint32_t o[4];
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float f = i & 1 ? up * 0.0625f : up;
+        const half2_t p = {(_Float16)(x[j][i] * f), (_Float16)(x[j][i + 4] * f)};
+        o[i] = as_u(p);
+        sum += x[j][i] * up + x[j][i + 4] * up;
+      }
+#pragma unroll
+      for (int b = 0; b < 2; ++b) q[b][j] = make_uint4(o[0] & mask[b], o[1] & mask[b], o[2] & mask[b], o[3] & mask[b]);
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      mine = g == j ? sum : mine;
+    }
+    mine *= 0x1p-24f;
+    const _Float16 hi = (_Float16)mine;
+    const half2_t parts = {hi, (_Float16)(mine - (float)hi)};
+    qsum = as_u(parts);
+    m = -3.4028235e38f;
+    bar = -INFINITY;
+    l = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NG; ++j) acc[j][0] = acc[j][1] = (f32x4_t){0, 0, 0, 0};
+    acc_m = (f32x4_t){0, 0, 0, 0};
+  }
+
+  // Sub-tile u of the stage at LDS address lds: tokens tok0 .. tok0 + 31.
+  __device__ __attribute__((always_inline)) inline void step(uint32_t lds, int u, int tok0, int ctx, bool edge) {
+    Kv4Reads<D> R;
+    R.read_k(lds + kw_at, lds + sm_at, lds + am_at, u);
+    // ---- products with the tokens' K: sum over groups of s (n . q), and the m term by itself
+    f32x4_t x[2], c[NG];
+#pragma unroll
+    for (int j = 0; j < NG; ++j) c[j] = (f32x4_t){0, 0, 0, 0};
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        const uint32_t w = R.k(b, j), v = w >> 8;
+        // fp16 subnormals: n 2^-24, and 16 n 2^-24 for the odd ones
+        c[j] = mfma16(make_uint4(w & 0x000f000fu, w & 0x00f000f0u, v & 0x000f000fu, v & 0x00f000f0u), q[b][j], c[j]);
+      }
+      const uint32_t mm = R.am[b] >> 16 | (R.am[b] & 0xffff0000u);
+      x[b] = mfma16(make_uint4(D == 128 || g < 2 ? mm : 0, 0, 0, 0), make_uint4(qsum, 0, 0, 0), (f32x4_t){0, 0, 0, 0});
+    }
+    float s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[i] = mask[0] ? x[0][i] : x[1][i];  // (not a sum: m may be NaN in the other fragment)
+#pragma unroll
+      for (int j = 0; j < NG; ++j) s[i] = fmaf((float)as_h2(R.scale(i, j)).x, c[j][i], s[i]);
+    }
+    const int first = tok0 + 8 * g;  // the 8 tokens of the lane's V
+    const int own = first + (n >> 3) * 4;  // and the 4 of its column
+    if (edge) {
+      asm volatile("" ::: "memory");  // (stays a branch)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] = own + i <= limit ? s[i] : -INFINITY;
+    }
+    float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+    if (__any(top > bar)) {
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float mn = fmaxf(m, top * scale);
+      const float a = __builtin_amdgcn_exp2f(m - mn);
+      bar = fmaxf(bar, top + kKv4Lazy / scale);
+      m = mn;
+      l *= a;
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        acc[j][0] *= a;
+        acc[j][1] *= a;
+      }
+      acc_m *= a;
+    }
+    // fp16 rows get P in two parts, whose own rounding would show in their outputs; bf16 rows
+    // one, and l the sum of the same truncated weights
+    uint32_t ph[2], pl[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float y = __builtin_amdgcn_exp2f(fmaf(s[2 * i], scale, -m));
+      const float z = __builtin_amdgcn_exp2f(fmaf(s[2 * i + 1], scale, -m));
+      const half2_t h = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(y, z));
+      ph[i] = as_u(h);
+      if constexpr (HILO) {
+        pl[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y - (float)h.x, z - (float)h.y));
+        l += y + z;
+      } else {
+        l = __builtin_amdgcn_fdot2(h, (half2_t){(_Float16)1.0f, (_Float16)1.0f}, l, false);
+      }
+    }
+    uint32_t p[4] = {ph[0] & mask[0], ph[1] & mask[0], ph[0] & mask[1], ph[1] & mask[1]};
+    uint32_t p2[4];
+    if constexpr (HILO) {
+      p2[0] = pl[0] & mask[0]; p2[1] = pl[1] & mask[0]; p2[2] = pl[0] & mask[1]; p2[3] = pl[1] & mask[1];
+    }
+    // ---- output: the weights times s are the operand of each group's n, as fp16 subnormals, and the
+    // weights that of m
+    R.read_v(lds + v_at, lds + vs_at, lds + vm_at, u);
+    if (edge) {
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int t = own + 2 * i;
+        const uint32_t seen = (t <= limit ? 0xffffu : 0u) | (t + 1 <= limit ? 0xffff0000u : 0u);
+#pragma unroll
+        for (int j = 0; j < NG; ++j) R.vs[j][i] &= seen;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // of tokens that the column does not see nothing may come through, NaN neither: their s
+        // is 0; and m's operand is shared by all columns, so what is NaN (s is, too) or belongs
+        // to no token is 0 there
+        const int t = first + 2 * i;
+        const uint32_t live = (t < ctx ? 0xffffu : 0u) | (t + 1 < ctx ? 0xffff0000u : 0u);
+        const uint32_t nan = ((R.vm[i] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+        R.vm[i] &= live & ~((nan >> 15) * 0xffffu);
+      }
+    }
+    const uint32_t groups = n < NG ? ~0u : 0u;
+    const uint4 vm = make_uint4(R.vm[0] & groups, R.vm[1] & groups, R.vm[2] & groups, R.vm[3] & groups);
+    acc_m = mfma16(vm, make_uint4(p[0], p[1], p[2], p[3]), acc_m);
+    if constexpr (HILO) acc_m = mfma16(vm, make_uint4(p2[0], p2[1], p2[2], p2[3]), acc_m);
+    // lanes 8 .. 15 of a row have the same quads' upper two dimensions
+    const uint32_t shift = n & 8, turn = shift ? 4 : 28;
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      uint32_t w[4], w2[4], a0[4], a1[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const half2_t s2 = as_h2(R.vs[j][i & 1]);  // (one half of p is 0)
+        const half2_t ps = as_h2(p[i]) * s2;
+        w[i] = as_u(ps);
+        // what the product's rounding left out (n s is many times a value near 0), and the
+        // weights' second part
+        half2_t rest = __builtin_elementwise_fma(as_h2(p[i]), s2, -ps);
+        if constexpr (HILO) rest = __builtin_elementwise_fma(as_h2(p2[i]), s2, rest);
+        w2[i] = as_u(rest);
+        // 16 n 2^-24: the matrix unit aligns a subnormal's products by 2^-14, its nominal
+        // exponent, and n 2^-24 would lose 4 more bits (n s against m: near-zero values showed it)
+        a0[i] = __builtin_amdgcn_alignbit(R.v[j][i], R.v[j][i], turn) & 0x00f000f0u;
+        a1[i] = R.v[j][i] >> shift & 0x00f000f0u;
+      }
+      const uint4 b = make_uint4(w[0], w[1], w[2], w[3]);
+      const uint4 x0 = make_uint4(a0[0], a0[1], a0[2], a0[3]), x1 = make_uint4(a1[0], a1[1], a1[2], a1[3]);
+      acc[j][0] = mfma16(x0, b, acc[j][0]);
+      acc[j][1] = mfma16(x1, b, acc[j][1]);
+      const uint4 b2 = make_uint4(w2[0], w2[1], w2[2], w2[3]);
+      acc[j][0] = mfma16(x0, b2, acc[j][0]);
+      acc[j][1] = mfma16(x1, b2, acc[j][1]);
+    }
+  }
+
+  // After the last stage: l over the lanes of a column, NaN where it saw a page outside the pool
+  // (bad_at: the first one's position); o[4 j + i][c] its dimensions 32 j + 16 (g % 2) + 4 i +
+  // 2 (g / 2) + c.
+  __device__ __attribute__((always_inline)) inline void finish(int bad_at, float (&o)[4 * NG][2]) {
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (limit >= bad_at) l = __builtin_nanf("");
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      const float mt = __shfl(acc_m[j], n);  // row j: lanes 0 .. 15
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        o[4 * j + i][0] = fmaf(acc[j][0][i], 0x1p20f, mt);
+        o[4 * j + i][1] = fmaf(acc[j][1][i], 0x1p20f, mt);
+      }
+    }
+  }
+};
+
+// 16-byte agent-scope accesses of the workspace (sc1, as the scoped atomics above).
+__device__ inline __amdgpu_buffer_rsrc_t ws_rsrc(const float* p) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, 0x7fffffff, 0x00020000);
+}
+constexpr int kAuxSc1 = 16;
+__device__ inline float4 ws_get4(__amdgpu_buffer_rsrc_t r, int at) {  // at: floats
+  return __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(r, at * 4, 0, kAuxSc1));
+}
+__device__ inline void ws_put4(__amdgpu_buffer_rsrc_t r, int at, float4 x) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, x), r, at * 4, 0, kAuxSc1);
+}
+
+constexpr int kTokWaves = 4;
+constexpr int kTokCols = 8;   // columns of a workgroup
+constexpr int kTokRing = 2;  // stages of a wave
+constexpr int kTokMaxSplits = 256;
+
+// The work of workgroup blockIdx.x where there are more than fit the chip at once: full splits
+// first, then the sequences' last ones, longest first, so that the launch does not end on full splits
+// that started late (plain order deals a split of every sequence in turn).  At most 64 sequences, one a
+// lane; one tile a sequence.  False: no work.
+__device__ inline bool kv4_longest_first(const Kv4AttnArgs& A, Kv4Seq& S, int& split, int& b, int& kvh) {
+  const int lane = threadIdx.x & 63;
+  Kv4Seq own{};
+  if (lane < A.batch) own = kv4_seq(A, lane);
+  const int full = own.rows ? own.ctx / A.split_tokens : 0;
+  // (no context: the rows still get their NaN, from split 0)
+  const int rest = own.rows && (own.ctx == 0 || own.ctx % A.split_tokens) ? own.ctx % A.split_tokens : -1;
+  int end = full * A.hkv;
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) {
+    const int y = __shfl_up(end, k);
+    if (lane >= k) end += y;
+  }
+  int i = blockIdx.x;
+  const int all = __builtin_amdgcn_readlane(end, 63);
+  if (i < all) {
+    b = __builtin_ctzll(__ballot(i < end));
+    i -= __builtin_amdgcn_readlane(end - full * A.hkv, b);
+    split = i / A.hkv;
+  } else {
+    i -= all;
+    int rank = 0;
+    for (int k = 0; k < A.batch; ++k) {
+      const int r = __builtin_amdgcn_readlane(rest, k);
+      rank += r > rest || (r == rest && k < lane);
+    }
+    const uint64_t at = __ballot(rest >= 0 && rank == i / A.hkv);
+    if (!at) return false;
+    b = __builtin_ctzll(at);
+    split = __builtin_amdgcn_readlane(full, b);
+  }
+  kvh = i % A.hkv;
+  S.row0 = __builtin_amdgcn_readlane(own.row0, b);
+  S.rows = __builtin_amdgcn_readlane(own.rows, b);
+  S.start = __builtin_amdgcn_readlane(own.start, b);
+  S.ctx = __builtin_amdgcn_readlane(own.ctx, b);
+  return true;
+}
+
+// ---- waves split tokens: one workgroup per (split, sequence, kv head, 8-column tile) ----
 template <int DT, int D>
 __device__ void kv4_tokens_impl(const Kv4AttnArgs& A) {
-  constexpr int NW = kTokWaves;
+  constexpr int NW = kTokWaves, NT = 64 * NW, R = kTokRing;
+  using Stage = Kv4Stage<D>;
   constexpr int OS = D + 4;  // floats of a column's row in LDS
-  __shared__ float s_o[NW][16][OS];
-  __shared__ float s_m[NW][16], s_l[NW][16];
-  __shared__ float s_w[kTokMaxSplits][16];
+  constexpr int Q = D / 4;   // float4s of a column
+  __shared__ __attribute__((aligned(16))) char s_ring[NW][R][Stage::BYTES];
+  constexpr int TC = kTokCols;
+  __shared__ float s_m[NW][2 * TC], s_l[NW][2 * TC];
   __shared__ int s_last;
+  // the ring's memory after the last stage: the waves' o; then, in the merge of the splits, the sets' o
+  // and the splits' weights
+  float (*const s_o)[2 * TC][OS] = (float (*)[2 * TC][OS])s_ring;
+  float4* const s_x = (float4*)s_ring;
+  float (*const s_w)[TC] = (float (*)[TC])((char*)s_ring + NT * 16);
+  static_assert(NW * 2 * TC * OS * 4 <= (int)sizeof(s_ring) && NT * 16 + kTokMaxSplits * TC * 4 <= (int)sizeof(s_ring), "fits");
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int units = A.batch * A.hkv * A.tiles;
-  const int split = blockIdx.x / units, unit = blockIdx.x % units;
-  const int tile = unit % A.tiles, bh = unit / A.tiles;
-  const int b = bh / A.hkv, kvh = bh % A.hkv;
-  const Kv4Seq S = kv4_seq(A, b);
-  const int col0 = tile * 16, ncols = S.rows * A.group;
-  const int here = min(16, ncols - col0);
+  int split, tile, b, kvh;
+  Kv4Seq S;
+  if (A.longest_first) {
+    if (!kv4_longest_first(A, S, split, b, kvh)) return;
+    tile = 0;
+  } else {
+    const int units = A.batch * A.hkv * A.tiles;
+    split = blockIdx.x / units;
+    const int u = blockIdx.x % units;
+    tile = u % A.tiles;
+    b = u / A.tiles / A.hkv;
+    kvh = u / A.tiles % A.hkv;
+    S = kv4_seq(A, b);
+  }
+  const int unit = (b * A.hkv + kvh) * A.tiles + tile;
+  const int col0 = tile * TC, ncols = S.rows * A.group;
+  const int here = min(TC, ncols - col0);
   if (S.ctx == 0) {
     if (split == 0 && tile == 0) kv4_no_context<DT, D>(A, S, kvh);
     return;
@@ -440,52 +893,113 @@ __device__ void kv4_tokens_impl(const Kv4AttnArgs& A) {
   if (begin > last) return;
   const int end = min(last + 1, begin + A.split_tokens);
 
-  Kv4Wave<DT, D, 1> W;
-  W.begin(A, S.row0, kvh, S.start, S.ctx, col0, ncols);
+  // ---- the wave's stages: w, w + NW, ... of the split
+  const uint32_t page_stride = (uint32_t)(A.num_layers * A.hkv) * Kv4<D>::kSlab;
+  const int64_t base = ((int64_t)A.layer * A.hkv + kvh) * Kv4<D>::kSlab;
+  Stage st;
+  st.begin(A.k_pool + base, A.v_pool + base);
+  const int32_t* const table = A.tables + (int64_t)b * A.table_stride;
+  const int stages = (end - begin + Stage::TOKENS - 1) / Stage::TOKENS;
+  const int count = stages > w ? (stages - w + NW - 1) / NW : 0;
+  const int min_limit = S.start + col0 / A.group;
   int bad_at = 0x7fffffff;
-  kv4_walk<DT, D, 1>(A, W, A.tables + (int64_t)b * A.table_stride, kvh, begin / 32 + w, (end + 31) / 32, NW,
-                     S.ctx, S.start + col0 / A.group, bad_at);
-  const int n = W.n, g = W.g;
-  W.finish(bad_at);
-  if (g == 0) {
-    s_m[w][n] = W.m[0];
-    s_l[w][n] = W.l[0];
+  int pages[Stage::PAGES];  // of stage chunk + lane
+  auto load_pages = [&](int chunk) __attribute__((always_inline)) {
+    const int lane = threadIdx.x & 63;
+    const int64_t tok = begin + ((int64_t)(chunk + lane) * NW + w) * Stage::TOKENS;
+    int bad = 0x7fffffff;
+#pragma unroll
+    for (int i = Stage::PAGES - 1; i >= 0; --i) {
+      const int64_t at = tok + i * kPage;
+      pages[i] = at < end ? table[at / kPage] : 0;
+      // a page outside the pool is never an address: page 0 is read instead
+      if (pages[i] < 0 || pages[i] >= A.num_blocks) {
+        bad = (int)at;
+        pages[i] = 0;
+      }
+    }
+    if (__any(bad != 0x7fffffff)) {
+#pragma unroll
+      for (int k = 1; k < 64; k <<= 1) bad = min(bad, __shfl_xor(bad, k));
+      bad_at = min(bad_at, bad);
+    }
+  };
+  auto issue = [&](int i) __attribute__((always_inline)) {
+    const int p0 = __builtin_amdgcn_readlane(pages[0], i & 63), p1 = __builtin_amdgcn_readlane(pages[1], i & 63);
+    int p2 = 0, p3 = 0;
+    if constexpr (Stage::PAGES == 4) {
+      p2 = __builtin_amdgcn_readlane(pages[2], i & 63);
+      p3 = __builtin_amdgcn_readlane(pages[3], i & 63);
+    }
+    st.issue(s_ring[w][i % R], p0, p1, p2, p3, page_stride);
+  };
+  if (count) load_pages(0);
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (i < count) issue(i);
+  Kv4Row<DT, D> W;
+  W.begin(A, S.row0, kvh, S.start, S.ctx, col0, ncols);
+  for (int i = 0; i < count; ++i) {
+    const int newer = min(count - 1 - i, R - 1);
+    if (newer >= 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * Stage::LOADS) : "memory");
+    else if (newer == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(Stage::LOADS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const int tok0 = begin + (i * NW + w) * Stage::TOKENS;
+    const uint32_t lds = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)s_ring[w][i % R];
+#pragma unroll
+    for (int u = 0; u < Stage::SUB; ++u) {
+      const int t = tok0 + 32 * u;
+      if (t <= last) W.step(lds, u, t, S.ctx, t + 31 > min_limit);
+    }
+    const int nx = i + R;
+    if (nx < count) {
+      if ((nx & 63) == 0) load_pages(nx);
+      issue(nx);
+    }
   }
+  float o_wave[D / 8][2];
+  W.finish(bad_at, o_wave);
+  const int n = W.n, g = W.g;
+  if (g == 0) {
+    s_m[w][n] = W.m;
+    s_l[w][n] = W.l;
+  }
+  __syncthreads();  // every wave is done with its ring
 #pragma unroll
-  for (int h = 0; h < D / 64; ++h)
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      *(float4*)&s_o[w][n][64 * h + 16 * g + 4 * r] =
-          make_float4(W.acc[0][4 * h][r], W.acc[0][4 * h + 1][r], W.acc[0][4 * h + 2][r], W.acc[0][4 * h + 3][r]);
+  for (int k = 0; k < D / 8; ++k)
+    *(float2*)&s_o[w][n][32 * (k >> 2) + 16 * (g & 1) + 4 * (k & 3) + 2 * (g >> 1)] = make_float2(o_wave[k][0], o_wave[k][1]);
   __syncthreads();
+  auto store = [&](int col, int d, float4 o, float L) __attribute__((always_inline)) {
+    const int c = col0 + col;
+    uint16_t* const dst = A.out + (int64_t)(S.row0 + c / A.group) * A.out_stride + ((int64_t)kvh * A.group + c % A.group) * D + d;
+    const uint32_t a0 = St<DT>::store(o.x / L) | (uint32_t)St<DT>::store(o.y / L) << 16;
+    const uint32_t a1 = St<DT>::store(o.z / L) | (uint32_t)St<DT>::store(o.w / L) << 16;
+    *(uint2*)dst = make_uint2(a0, a1);
+  };
   // ---- the workgroup's columns
-  constexpr int Q = D / 4;  // float4s of a column
-  const int64_t part = (int64_t)unit * A.splits;
-  for (int i = threadIdx.x; i < here * Q; i += 64 * NW) {
+  const int64_t part = (int64_t)unit * A.splits * TC;  // (split, column) records
+  const __amdgpu_buffer_rsrc_t po = ws_rsrc(A.ws_o + part * D);
+  for (int i = threadIdx.x; i < here * Q; i += NT) {
     const int col = i / Q, d = i % Q * 4;
-    float M = s_m[0][col];
+    float M = fmaxf(s_m[0][col], s_m[0][col + TC]);
 #pragma unroll
-    for (int k = 1; k < NW; ++k) M = fmaxf(M, s_m[k][col]);
+    for (int k = 1; k < NW; ++k) M = fmaxf(M, fmaxf(s_m[k][col], s_m[k][col + TC]));
     float L = 0.0f;
     float4 o = make_float4(0, 0, 0, 0);
 #pragma unroll
-    for (int k = 0; k < NW; ++k) {
-      const float e = __builtin_amdgcn_exp2f(s_m[k][col] - M);
-      const float4 x = *(const float4*)&s_o[k][col][d];
-      L = fmaf(e, s_l[k][col], L);
+    for (int k = 0; k < 2 * NW; ++k) {
+      const int c = col + (k & 1) * TC;
+      const float e = __builtin_amdgcn_exp2f(s_m[k >> 1][c] - M);
+      const float4 x = *(const float4*)&s_o[k >> 1][c][d];
+      L = fmaf(e, s_l[k >> 1][c], L);
       o.x = fmaf(e, x.x, o.x); o.y = fmaf(e, x.y, o.y); o.z = fmaf(e, x.z, o.z); o.w = fmaf(e, x.w, o.w);
     }
     if (nsplit == 1) {
-      const int c = col0 + col;
-      uint16_t* const dst = A.out + (int64_t)(S.row0 + c / A.group) * A.out_stride + ((int64_t)kvh * A.group + c % A.group) * D + d;
-      const uint32_t a0 = St<DT>::store(o.x / L) | (uint32_t)St<DT>::store(o.y / L) << 16;
-      const uint32_t a1 = St<DT>::store(o.z / L) | (uint32_t)St<DT>::store(o.w / L) << 16;
-      *(uint2*)dst = make_uint2(a0, a1);
+      store(col, d, o, L);
     } else {
-      float* const po = A.ws_o + ((part + split) * 16 + col) * D + d;
-      ws_put(po, o.x); ws_put(po + 1, o.y); ws_put(po + 2, o.z); ws_put(po + 3, o.w);
+      ws_put4(po, (split * TC + col) * D + d, o);
       if (d == 0) {
-        float* const pm = A.ws_ml + ((part + split) * 16 + col) * 2;
+        float* const pm = A.ws_ml + (part + split * TC + col) * 2;
         ws_put(pm, M);
         ws_put(pm + 1, L);
       }
@@ -496,40 +1010,86 @@ __device__ void kv4_tokens_impl(const Kv4AttnArgs& A) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0)
-    s_last = __hip_atomic_fetch_add(A.ws_cnt + unit, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == nsplit - 1;
+    s_last = __hip_atomic_fetch_add(A.ws_cnt + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == nsplit - 1;
   __syncthreads();
   if (!s_last) return;
   if (threadIdx.x == 0) __hip_atomic_store(A.ws_cnt + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // weights 2^(m_s - M) and their sums (s_l's first row)
-  for (int col = threadIdx.x; col < here; col += 64 * NW) {
-    const float* const pm = A.ws_ml + (part * 16 + col) * 2;
-    float M = -INFINITY;
-    for (int s = 0; s < nsplit; ++s) M = fmaxf(M, ws_get(pm + (int64_t)s * 32));
-    float L = 0.0f;
-    for (int s = 0; s < nsplit; ++s) {
-      const float e = __builtin_amdgcn_exp2f(ws_get(pm + (int64_t)s * 32) - M);
-      L = fmaf(e, ws_get(pm + (int64_t)s * 32 + 1), L);
-      s_w[s][col] = e;
+  // (m, l): lane s of wave w has splits s, s + 64, ... of columns w, w + NW, ...; weights 2^(m_s - M)
+  // and l
+  constexpr int CW = TC / NW, SL = kTokMaxSplits / 64;
+  const int lane = threadIdx.x & 63;
+  float mv[CW][SL], lv[CW][SL];
+#pragma unroll
+  for (int c = 0; c < CW; ++c)
+#pragma unroll
+    for (int k = 0; k < SL; ++k) {
+      const int s = lane + 64 * k;
+      const bool on = s < nsplit && w + NW * c < here;
+      const float* const pm = A.ws_ml + (part + (on ? s * TC + w + NW * c : 0)) * 2;
+      mv[c][k] = on ? ws_get(pm) : -INFINITY;
+      lv[c][k] = on ? ws_get(pm + 1) : 0.0f;
     }
-    s_l[0][col] = L;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < here * Q; i += 64 * NW) {
-    const int col = i / Q, d = i % Q * 4;
-    const float* const po = A.ws_o + (part * 16 + col) * D + d;
+  // o: columns x Q float4s, the splits dealt to as many sets of threads as there are; NB loads
+  // of a thread under way (the rounds of loads are what a merge takes)
+  const int items = here * Q;
+  const int sets = max(NT / items, 1);
+  constexpr int NB = 16;
+  for (int i0 = 0; i0 < items; i0 += NT) {
+    const int item = sets > 1 ? threadIdx.x % items : i0 + threadIdx.x;
+    const int set = sets > 1 ? threadIdx.x / items : 0;
+    const bool on = item < items && set < sets;
+    const int col = on ? item / Q : 0, d = on ? item % Q * 4 : 0;
+    float4 x[NB];
+#pragma unroll
+    for (int k = 0; k < NB; ++k) x[k] = ws_get4(po, (min(set + k * sets, nsplit - 1) * TC + col) * D + d);
+    if (i0 == 0) {
+#pragma unroll
+      for (int c = 0; c < CW; ++c) {
+        float M = mv[c][0];
+#pragma unroll
+        for (int k = 1; k < SL; ++k) M = fmaxf(M, mv[c][k]);
+        M = wave_max(M);
+        float L = 0.0f, e[SL];
+#pragma unroll
+        for (int k = 0; k < SL; ++k) {
+          e[k] = __builtin_amdgcn_exp2f(mv[c][k] - M);
+          if (lane + 64 * k < nsplit) L = fmaf(e[k], lv[c][k], L);
+        }
+        L = wave_sum(L);
+        if (w + NW * c < here) {
+#pragma unroll
+          for (int k = 0; k < SL; ++k)
+            if (lane + 64 * k < nsplit) s_w[lane + 64 * k][w + NW * c] = e[k];
+          if (lane == 0) s_l[0][w + NW * c] = L;
+        }
+      }
+      __syncthreads();
+    }
     float4 o = make_float4(0, 0, 0, 0);
-    for (int s = 0; s < nsplit; ++s) {
-      const float e = s_w[s][col];
-      const float* const x = po + (int64_t)s * 16 * D;
-      o.x = fmaf(e, ws_get(x), o.x); o.y = fmaf(e, ws_get(x + 1), o.y);
-      o.z = fmaf(e, ws_get(x + 2), o.z); o.w = fmaf(e, ws_get(x + 3), o.w);
+    for (int s0 = set; s0 < nsplit; s0 += NB * sets) {
+      if (s0 != set) {
+#pragma unroll
+        for (int k = 0; k < NB; ++k) x[k] = ws_get4(po, (min(s0 + k * sets, nsplit - 1) * TC + col) * D + d);
+      }
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        const int s = s0 + k * sets;
+        if (s < nsplit) {
+          const float e = s_w[s][col];
+          o.x = fmaf(e, x[k].x, o.x); o.y = fmaf(e, x[k].y, o.y); o.z = fmaf(e, x[k].z, o.z); o.w = fmaf(e, x[k].w, o.w);
+        }
+      }
     }
-    const float L = s_l[0][col];
-    const int c = col0 + col;
-    uint16_t* const dst = A.out + (int64_t)(S.row0 + c / A.group) * A.out_stride + ((int64_t)kvh * A.group + c % A.group) * D + d;
-    const uint32_t a0 = St<DT>::store(o.x / L) | (uint32_t)St<DT>::store(o.y / L) << 16;
-    const uint32_t a1 = St<DT>::store(o.z / L) | (uint32_t)St<DT>::store(o.w / L) << 16;
-    *(uint2*)dst = make_uint2(a0, a1);
+    if (sets > 1) {  // (one round)
+      if (on && set) s_x[set * items + item] = o;
+      __syncthreads();
+      if (on && !set)
+        for (int k = 1; k < sets; ++k) {
+          const float4 y = s_x[k * items + item];
+          o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
+        }
+    }
+    if (on && !set) store(col, d, o, s_l[0][col]);
   }
 }
 

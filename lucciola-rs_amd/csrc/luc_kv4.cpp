@@ -140,13 +140,28 @@ struct Kv4AttnArgs {
   float* ws_ml;
   float* ws_o;
   int32_t batch, total_rows, max_rows, max_ctx, layer, num_layers, hkv, group, num_blocks;
-  int32_t tiles, splits, split_tokens;
+  int32_t tiles, splits, split_tokens, longest_first;
   float qk_scale_log2;
 };
 
 constexpr int kCUs = 256;
-constexpr int kTokCols = 16, kTokUnit = 128;  // columns of a workgroup; tokens of a round of its 4 waves
-constexpr int kTokMaxSplits = 64;             // kv4_attention.hip
+constexpr int kTokCols = 8;                   // columns of a workgroup
+constexpr int kTokMaxSplits = 256;            // kv4_attention.hip
+constexpr int kTokSlots = 2 * kCUs;           // resident workgroups
+// Split lengths of a tokens launch: what fills the chip once, but not shorter than is worth a merge
+// and not longer than lets mixed contexts end together.  us at fixed lengths, batch x context,
+// heads:
+//   8 x 32768, 12 and 2 of 128: 40.3 at 512, 25.6 at 1024 (the rule's) and 2048
+//   32 x 128..4096, 14 and 2 of 64: 13.9 at 256, 13.2 at 512 (the rule's), 13.7 at 1024
+//   64 x 1024..16384, 28 and 4 of 128: 104 at 1024, 87.6 at 2048 (the rule's), 90.9 at 4096;
+//     all of 8192: 74.8, 69.9 at 4096, 66.8 whole
+//   256 x 1000, 14 and 2 of 64: 24.1 at 256, 20.8 at 512, 15.4 whole (the rule's)
+//   1 x 32768, 14 and 2 of 64: 12.9 at 512 (the rule's), 13.1 at 1024
+//   4 x 4000, 28 and 4 of 128: 16.9 at 128, 13.3 at 256 and 512 (the rule's), 16.0 at 1024
+// More than one round of workgroups starts with the longest (64 x 1024..16384: 87.5, in plain order
+// 93.8).
+constexpr int kTokMinSplit = 512, kTokMaxSplit = 2048;
+constexpr int kTokRounds = 8;  // rounds of workgroups balance any contexts: longer splits beyond
 constexpr int64_t kMaxArrivals = 1 << 16;     // (sequence, kv head, column tile)
 constexpr int kMaxCtx = 1 << 30;
 
@@ -155,6 +170,7 @@ struct Kv4Plan {
   int tiles = 0;        // per (sequence, kv head)
   int splits = 1;
   int split_tokens = 0;
+  bool longest_first = false;
 };
 
 // Depends only on the arguments, so that the workspace size agrees with the launch.
@@ -166,8 +182,13 @@ Kv4Plan kv4_plan(int batch, int total_rows, int max_rows, int max_ctx, int hkv, 
   if (p.tokens) {
     p.tiles = (int)ceil_div(cols, kTokCols);
     const int64_t units = pairs * p.tiles;
-    const int64_t want = std::min<int64_t>(std::max<int64_t>(ceil_div(4 * kCUs, units), 1), kTokMaxSplits);
-    p.split_tokens = (int)(ceil_div(ceil_div(max_ctx, want), kTokUnit) * kTokUnit);
+    // a stage for each of 4 waves
+    const int round = head_dim == 64 ? 256 : 128;
+    const int64_t fill = units * max_ctx / kTokSlots;
+    int64_t st = std::min<int64_t>(std::max<int64_t>(fill, kTokMinSplit), kTokMaxSplit);
+    st = std::max({st, fill / kTokRounds, ceil_div(max_ctx, kTokMaxSplits)});
+    p.split_tokens = (int)(ceil_div(st, round) * round);
+    p.longest_first = p.tiles == 1 && batch <= 64 && units * ceil_div(max_ctx, p.split_tokens) > kTokSlots;
   } else {
     p.tiles = (int)ceil_div(cols, head_dim == 64 ? 256 : 128);
     const int64_t wgs = pairs * p.tiles;
@@ -318,12 +339,14 @@ int luc_kv4_attention(luc_ctx* ctx, void* stream, int dtype, void* out, int64_t 
   if (plan.tokens && plan.splits > 1 && units > kMaxArrivals)
     return fail(LUC_E_UNSUPPORTED, "split attention of %lld (sequence, kv head) units above %lld", (long long)units,
                 (long long)kMaxArrivals);
+  if ((int64_t)num_layers * num_kv_heads * 10 * head_dim > UINT32_MAX)
+    return fail(LUC_E_INVALID, "num_layers x num_kv_heads too large");
   if (units * plan.splits * 256 > UINT32_MAX) return fail(LUC_E_INVALID, "batch x kv heads x rows too large");
   if (int rc = check_device(ctx)) return rc;
   Kv4AttnArgs a{q, q_row_stride, out, out_row_stride, k_pool, v_pool, block_tables, table_stride, cu_seqlens,
                 start_pos, nullptr, nullptr, nullptr, batch, total_rows, max_rows, max_ctx, layer, num_layers,
                 num_kv_heads, group, num_blocks, plan.tiles, plan.splits, plan.split_tokens,
-                sm_scale * 1.4426950408889634f};
+                plan.longest_first, sm_scale * 1.4426950408889634f};
   if (need) {
     char* ws = static_cast<char*>(workspace);
     a.ws_cnt = reinterpret_cast<int32_t*>(ws);

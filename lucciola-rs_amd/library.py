@@ -155,7 +155,8 @@ def pool_pages(pool, num_layers, num_kv_heads, head_dim) -> int:
 
 def _stream(stream):
     if stream is None:
-        stream = torch.cuda.current_stream()
+        # torch.cuda.current_stream().cuda_stream, without the object (0.2 us of a call, not 1.5)
+        return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
     return stream.cuda_stream
 
 
@@ -378,14 +379,28 @@ class LucAttn:
                                            table.shape[1]))
 
     # ---- serving over a cache held on the GPU ----
+    # (plain checks without loops or keywords: a call of a small batch takes less on the GPU
+    # than its checks on the host otherwise would)
     @staticmethod
-    def _arrays(name, device, **arrays):
-        """Operands of the page maps: contiguous, on the device, of the dtype and at least
-        the elements that each is given with."""
-        for key, (t, dtype, least) in arrays.items():
-            if t.dtype != dtype or t.device != device or not t.is_contiguous() or t.numel() < least:
-                raise ValueError(f"{name}: {key} {tuple(t.shape)} {t.dtype} on {t.device}: want "
-                                 f"contiguous {dtype} of at least {least} elements on {device}")
+    def _array(name, t, dtype, dev, least):
+        """An operand read as a flat array: contiguous, of `dtype`, on device `dev`, of at least
+        `least` elements."""
+        if t.dtype is not dtype or t.get_device() != dev or t.numel() < least or not t.is_contiguous():
+            raise ValueError(f"{name} {tuple(t.shape)} {t.dtype} on {t.device}: want contiguous {dtype} of at "
+                             f"least {least} elements on the call's device")
+        return t.data_ptr()
+
+    @staticmethod
+    def _rows(name, t, width, head_dim, dtype, dev):
+        """(rows, row stride) of an operand [rows, width] or [rows, heads, head_dim] whose rows are
+        `width` consecutive elements."""
+        shape, strides = t.shape, t.stride()
+        if t.dtype is not dtype or t.get_device() != dev:
+            raise TypeError(f"{name} is {t.dtype} on {t.device}: want {dtype} on the call's device")
+        if len(shape) == 2 and shape[1] == width and strides[1] == 1 or \
+                len(shape) == 3 and shape[1] * shape[2] == width and strides[1:] == (head_dim, 1) and shape[2] == head_dim:
+            return shape[0], strides[0]
+        raise ValueError(f"{name} {tuple(shape)} with strides {strides}: want rows of {width} consecutive elements")
 
     def block_extend(self, new_tokens, lens, tables, free_list, state, slots, positions, cu_seqlens,
                      start_pos, stream=None):
@@ -394,74 +409,53 @@ class LucAttn:
         slots int64 and positions int32 of one length, the most rows of the batch; the others
         int32 [B], cu_seqlens [B + 1]."""
         batch, stride = tables.shape
-        i32, rows = torch.int32, slots.numel()
-        self._arrays("block_extend", tables.device, new_tokens=(new_tokens, i32, batch),
-                     lens=(lens, i32, batch), tables=(tables, i32, 0), free_list=(free_list, i32, 1),
-                     state=(state, i32, 4), slots=(slots, torch.int64, 0),
-                     positions=(positions, i32, rows), cu_seqlens=(cu_seqlens, i32, batch + 1),
-                     start_pos=(start_pos, i32, batch))
+        i32, rows, dev, arr = torch.int32, slots.numel(), tables.get_device(), self._array
+        blocks = free_list.numel()
         self._check(self.lib.luc_block_extend(
-            self.ctx, _stream(stream), batch, _p(new_tokens), _p(lens), _p(tables), stride,
-            _p(free_list), _p(state), free_list.numel(), rows, _p(slots), _p(positions),
-            _p(cu_seqlens), _p(start_pos)))
+            self.ctx, _stream(stream), batch, arr("new_tokens", new_tokens, i32, dev, batch),
+            arr("lens", lens, i32, dev, batch), arr("tables", tables, i32, dev, 0), stride,
+            arr("free_list", free_list, i32, dev, 0), arr("state", state, i32, dev, 4), blocks, rows,
+            arr("slots", slots, torch.int64, dev, 0), arr("positions", positions, i32, dev, rows),
+            arr("cu_seqlens", cu_seqlens, i32, dev, batch + 1), arr("start_pos", start_pos, i32, dev, batch)))
 
     def block_truncate(self, keep, lens, tables, free_list, state, stream=None):
         """luc_block_truncate: sequence b back to at most keep[b] tokens, its pages behind those
         to the free list."""
         batch, stride = tables.shape
-        i32 = torch.int32
-        self._arrays("block_truncate", tables.device, keep=(keep, i32, batch),
-                     lens=(lens, i32, batch), tables=(tables, i32, 0), free_list=(free_list, i32, 1),
-                     state=(state, i32, 4))
+        i32, dev, arr = torch.int32, tables.get_device(), self._array
         self._check(self.lib.luc_block_truncate(
-            self.ctx, _stream(stream), batch, _p(keep), _p(lens), _p(tables), stride, _p(free_list),
-            _p(state), free_list.numel()))
+            self.ctx, _stream(stream), batch, arr("keep", keep, i32, dev, batch),
+            arr("lens", lens, i32, dev, batch), arr("tables", tables, i32, dev, 0), stride,
+            arr("free_list", free_list, i32, dev, 0), arr("state", state, i32, dev, 4), free_list.numel()))
 
-    @staticmethod
-    def _rows(name, t, heads, head_dim):
-        """Rows and row stride of a [rows, heads * head_dim] view (or [rows, heads, head_dim])."""
-        width = heads * head_dim
-        if t.dim() == 3 and t.shape[1:] == (heads, head_dim) and t.stride(1) == head_dim:
-            inner, shape = t.stride(2), width
-        else:
-            inner, shape = t.stride(-1), t.shape[-1] if t.dim() == 2 else -1
-        if shape != width or inner != 1:
-            raise ValueError(f"{name} {tuple(t.shape)} with strides {t.stride()}: want rows of {width} "
-                             "consecutive elements")
-        return t.shape[0], t.stride(0)
-
-    def _append(self, fn, q, k, v, cos, sin, positions, slots, k_pool, v_pool, num_blocks, layer,
-                num_layers, hq, hkv, head_dim, q_norm, k_norm, eps, biases, q_out, outs, block_size,
-                stream):
-        rows, stride = self._rows("q", q, hq, head_dim)
-        for name, t in (("k", k), ("v", v)):
-            if self._rows(name, t, hkv, head_dim) != (rows, stride) and rows:
-                raise ValueError(f"{name}'s rows and their stride differ from q's")
-        dtype = dtype_code(q)
+    def _append_args(self, q, k, v, cos, sin, positions, slots, hq, hkv, head_dim, q_norm, k_norm, eps,
+                     q_bias, k_bias, v_bias, q_out, stream):
+        """The arguments that both appends share, from ctx to q_out_stride, and (rows, dtype, device)."""
+        dtype, dev, arr, f32 = q.dtype, q.get_device(), self._array, torch.float32
+        qw, kw = hq * head_dim, hkv * head_dim
+        rows, stride = own = self._rows("q", q, qw, head_dim, dtype, dev)
+        if rows and (self._rows("k", k, kw, head_dim, dtype, dev) != own or
+                     self._rows("v", v, kw, head_dim, dtype, dev) != own):
+            raise ValueError("k's or v's rows and their stride differ from q's")
+        o_stride = stride
         if q_out is None:
             q_out = q
-        o_rows, o_stride = self._rows("q_out", q_out, hq, head_dim)
-        kv_strides = [self._rows("k_out / v_out", t, hkv, head_dim) for t in outs if t is not None]
-        if o_rows != rows or any(s != (rows, kv_strides[0][1]) for s in kv_strides):
-            raise ValueError("outputs of other row counts (or strides, of k_out and v_out)")
-        norms = [t for t in (q_norm, k_norm) if t is not None]
-        if any(t.numel() != head_dim or not t.is_contiguous() for t in norms):
-            raise ValueError(f"head norms of {head_dim} elements are wanted")
-        for t, n in zip(biases, (hq, hkv, hkv)):
-            if t is not None and (t.numel() != n * head_dim or not t.is_contiguous()):
-                raise ValueError("a bias of other than its heads' elements")
-        if any(t.dtype != q.dtype for t in (k, v, q_out, *(t for t in (*outs, *norms, *biases) if t is not None))):
-            raise TypeError(f"operands of other types than q's {q.dtype}")
-        if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape or \
-                cos.dim() != 2 or cos.shape[1] != head_dim // 2 or not (cos.is_contiguous() and sin.is_contiguous()):
-            raise ValueError(f"rope tables {tuple(cos.shape)}: want fp32 [positions, {head_dim // 2}]")
-        self._arrays("append", q.device, positions=(positions, torch.int32, rows),
-                     slots=(slots, torch.int64, rows))
-        args = [self.ctx, _stream(stream), dtype, _p(q), _p(k), _p(v), stride, *map(_p, biases),
-                _p(q_norm), _p(k_norm), eps, _p(cos), _p(sin), cos.shape[0], _p(positions), _p(slots),
-                rows, _p(q_out), o_stride, *map(_p, outs), kv_strides[0][1] if kv_strides else 0,
-                _p(k_pool), _p(v_pool), num_blocks, layer, num_layers, hq, hkv, head_dim, block_size]
-        self._check(fn(*args))
+        else:
+            o_rows, o_stride = self._rows("q_out", q_out, qw, head_dim, dtype, dev)
+            if o_rows != rows:
+                raise ValueError(f"q_out has {o_rows} rows, q {rows}")
+        max_pos = cos.shape[0]
+        if cos.shape[-1] * 2 != head_dim or cos.shape != sin.shape:
+            raise ValueError(f"rope tables {tuple(cos.shape)}, {tuple(sin.shape)}: want [positions, {head_dim // 2}]")
+        return [self.ctx, _stream(stream), dtype_code(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), stride,
+                q_bias if q_bias is None else arr("q_bias", q_bias, dtype, dev, qw),
+                k_bias if k_bias is None else arr("k_bias", k_bias, dtype, dev, kw),
+                v_bias if v_bias is None else arr("v_bias", v_bias, dtype, dev, kw),
+                q_norm if q_norm is None else arr("q_norm", q_norm, dtype, dev, head_dim),
+                k_norm if k_norm is None else arr("k_norm", k_norm, dtype, dev, head_dim), eps,
+                arr("cos", cos, f32, dev, 0), arr("sin", sin, f32, dev, 0), max_pos,
+                arr("positions", positions, torch.int32, dev, rows), arr("slots", slots, torch.int64, dev, rows),
+                rows, q_out.data_ptr(), o_stride], rows, dtype, dev
 
     def qk_norm_rope_append(self, q, k, v, cos, sin, positions, slots, k_pool, v_pool, layer, num_layers,
                             hq, hkv, head_dim, q_norm=None, k_norm=None, eps=1e-6, q_bias=None,
@@ -471,32 +465,58 @@ class LucAttn:
         block_extend gives them) of the rows q [rows, hq * d], k and v [rows, hkv * d] (views with
         one row stride, as those into a qkv tensor); q_out (default: q itself) gets q, k_out, if
         given, k."""
-        if k_pool.dtype != q.dtype or v_pool.dtype != q.dtype:
-            raise TypeError(f"pools of other types than q's {q.dtype}")
-        nb = num_blocks if num_blocks is not None else pool_pages(k_pool, num_layers, hkv, head_dim)
-        self._append(self.lib.luc_qk_norm_rope_append, q, k, v, cos, sin, positions, slots, k_pool,
-                     v_pool, nb, layer, num_layers, hq, hkv, head_dim, q_norm, k_norm, eps,
-                     (q_bias, k_bias, v_bias), q_out, (k_out,), block_size, stream)
+        args, rows, dtype, dev = self._append_args(q, k, v, cos, sin, positions, slots, hq, hkv, head_dim,
+                                                   q_norm, k_norm, eps, q_bias, k_bias, v_bias, q_out, stream)
+        k_ptr, k_stride = None, 0
+        if k_out is not None:
+            k_ptr = k_out.data_ptr()
+            o_rows, k_stride = self._rows("k_out", k_out, hkv * head_dim, head_dim, dtype, dev)
+            if o_rows != rows:
+                raise ValueError(f"k_out has {o_rows} rows, q {rows}")
+        page = num_layers * hkv * 16 * head_dim
+        pages = min(k_pool.numel(), v_pool.numel()) // page if page > 0 else 0
+        if num_blocks is not None:
+            if num_blocks > pages:
+                raise ValueError(f"num_blocks {num_blocks}: the pools hold {pages} pages")
+            pages = num_blocks
+        self._check(self.lib.luc_qk_norm_rope_append(
+            *args, k_ptr, k_stride, self._array("k_pool", k_pool, dtype, dev, 0),
+            self._array("v_pool", v_pool, dtype, dev, 0), pages, layer, num_layers, hq, hkv, head_dim, block_size))
 
-    def kv4_pages(self, pool, num_layers, hkv, head_dim) -> int:
-        """Pages in a 4-bit pool: uint8 [pages, layers, kv heads, 10 * head_dim]."""
-        want = (num_layers, hkv, self.lib.luc_kv4_page_bytes(head_dim))
-        if pool.dtype != torch.uint8 or not pool.is_contiguous() or tuple(pool.shape[1:]) != want:
-            raise ValueError(f"4-bit pool {tuple(pool.shape)} {pool.dtype}: want contiguous uint8 "
-                             f"[pages, {', '.join(map(str, want))}]")
-        return int(pool.shape[0])
+    def _kv4_pools(self, k_pool, v_pool, num_layers, hkv, head_dim, num_blocks, dev):
+        """(k address, v address, pages) of 4-bit pools: uint8 [pages, layers, kv heads, 10 * head_dim]."""
+        shape = k_pool.shape
+        if len(shape) != 4 or shape[1:] != (num_layers, hkv, 10 * head_dim) or v_pool.shape != shape:
+            raise ValueError(f"4-bit pools {tuple(shape)}, {tuple(v_pool.shape)}: want [pages, {num_layers}, {hkv}, "
+                             f"{10 * head_dim}]")
+        pages = shape[0]
+        if num_blocks is not None:
+            if num_blocks > pages:
+                raise ValueError(f"num_blocks {num_blocks}: the pools hold {pages} pages")
+            pages = num_blocks
+        return (self._array("k_pool", k_pool, torch.uint8, dev, 0), self._array("v_pool", v_pool, torch.uint8, dev, 0),
+                pages)
 
     def kv4_append(self, q, k, v, cos, sin, positions, slots, k_pool, v_pool, layer, num_layers, hq, hkv,
                    head_dim, q_norm=None, k_norm=None, eps=1e-6, q_bias=None, k_bias=None, v_bias=None,
                    q_out=None, k_out=None, v_out=None, block_size=16, stream=None, num_blocks=None):
-        """luc_kv4_append: qk_norm_rope_append into 4-bit pools; k_out and v_out, if given, get
-        the values that the cache holds now."""
-        pages = min(self.kv4_pages(k_pool, num_layers, hkv, head_dim),
-                    self.kv4_pages(v_pool, num_layers, hkv, head_dim))
-        self._append(self.lib.luc_kv4_append, q, k, v, cos, sin, positions, slots, k_pool, v_pool,
-                     pages if num_blocks is None else num_blocks, layer, num_layers, hq, hkv, head_dim,
-                     q_norm, k_norm, eps, (q_bias, k_bias, v_bias), q_out, (k_out, v_out), block_size,
-                     stream)
+        """luc_kv4_append: qk_norm_rope_append into 4-bit pools (uint8 [pages, layers, kv heads,
+        10 * head_dim]); k_out and v_out (with one row stride), if given, get the values that the
+        cache holds now."""
+        args, rows, dtype, dev = self._append_args(q, k, v, cos, sin, positions, slots, hq, hkv, head_dim,
+                                                   q_norm, k_norm, eps, q_bias, k_bias, v_bias, q_out, stream)
+        kp, vp, pages = self._kv4_pools(k_pool, v_pool, num_layers, hkv, head_dim, num_blocks, dev)
+        o_stride, width = None, hkv * head_dim
+        for name, t in (("k_out", k_out), ("v_out", v_out)):
+            if t is not None:
+                o_rows, st = self._rows(name, t, width, head_dim, dtype, dev)
+                if o_rows != rows or o_stride not in (None, st):
+                    raise ValueError(f"{name}: {o_rows} rows of stride {st}; q has {rows} rows, k_out and v_out share "
+                                     "one stride")
+                o_stride = st
+        self._check(self.lib.luc_kv4_append(
+            *args, None if k_out is None else k_out.data_ptr(), None if v_out is None else v_out.data_ptr(),
+            o_stride or 0, kp, vp, pages, layer, num_layers, hq, hkv, head_dim, block_size))
 
     def kv4_workspace(self, batch, total_rows, max_rows, max_ctx, hq, hkv, head_dim, device=None):
         """A zero-filled workspace for kv4_attention calls of these sizes (None: none needed)."""
@@ -511,22 +531,21 @@ class LucAttn:
                       workspace=None, block_size=16, stream=None, num_blocks=None):
         """luc_kv4_attention: out and q [rows, hq * d]; start_pos int32 [batch]; cu_seqlens int32
         [batch + 1], or None for one row a sequence; workspace from kv4_workspace."""
-        rows, q_stride = self._rows("q", q, hq, head_dim)
-        o_rows, o_stride = self._rows("out", out, hq, head_dim)
-        if min(rows, o_rows) < total_rows or out.dtype != q.dtype:
-            raise ValueError(f"kv4_attention: q {tuple(q.shape)} {q.dtype}, out {tuple(out.shape)} {out.dtype} "
-                             f"for {total_rows} rows")
-        more = {} if cu_seqlens is None else {"cu_seqlens": (cu_seqlens, torch.int32, batch + 1)}
-        self._arrays("kv4_attention", q.device, tables=(tables, torch.int32, batch * tables.shape[-1]),
-                     start_pos=(start_pos, torch.int32, batch), **more)
-        pages = min(self.kv4_pages(k_pool, num_layers, hkv, head_dim),
-                    self.kv4_pages(v_pool, num_layers, hkv, head_dim))
-        ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+        dtype, dev, arr, i32 = q.dtype, q.get_device(), self._array, torch.int32
+        rows, q_stride = self._rows("q", q, hq * head_dim, head_dim, dtype, dev)
+        o_rows, o_stride = self._rows("out", out, hq * head_dim, head_dim, dtype, dev)
+        if rows < total_rows or o_rows < total_rows:
+            raise ValueError(f"q and out have {rows} and {o_rows} rows, fewer than total_rows {total_rows}")
+        kp, vp, pages = self._kv4_pools(k_pool, v_pool, num_layers, hkv, head_dim, num_blocks, dev)
+        stride = tables.shape[-1]
+        ws = None if workspace is None else arr("workspace", workspace, workspace.dtype, dev, 0)
         self._check(self.lib.luc_kv4_attention(
-            self.ctx, _stream(stream), dtype_code(q), _p(out), o_stride, _p(q), q_stride, _p(k_pool),
-            _p(v_pool), _p(tables), tables.shape[-1], pages if num_blocks is None else num_blocks,
-            _p(cu_seqlens), _p(start_pos), batch, total_rows, max_rows, max_ctx, layer, num_layers, hq,
-            hkv, head_dim, block_size, sm_scale, _p(workspace), ws_bytes))
+            self.ctx, _stream(stream), dtype_code(q), out.data_ptr(), o_stride, q.data_ptr(), q_stride, kp, vp,
+            arr("tables", tables, i32, dev, batch * stride), stride, pages,
+            cu_seqlens if cu_seqlens is None else arr("cu_seqlens", cu_seqlens, i32, dev, batch + 1),
+            arr("start_pos", start_pos, i32, dev, batch), batch, total_rows, max_rows, max_ctx, layer, num_layers,
+            hq, hkv, head_dim, block_size, sm_scale, ws,
+            0 if ws is None else workspace.numel() * workspace.element_size()))
 
     def gather_floor(self, k_pool, v_pool, tables, positions, batch, max_ctx, layer, num_layers,
                      hkv, head_dim, sink, stream=None):

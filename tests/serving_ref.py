@@ -143,7 +143,13 @@ def attention(q, k, v, start, scale):
     weight by that and its own truncation to fp16 (within 2^-11 of its mean, which the sum of
     the truncated weights shares).  The roundings are independent, so their sum over the
     tokens grows as the root of the squares; six times it is taken.  Weights below 2^-14 of the
-    largest lose up to 2^-24 each, and f32 sums of T terms up to T 2^-24 of the sum of their sizes."""
+    largest lose up to 2^-24 each, and f32 sums of T terms up to T 2^-24 of the sum of their sizes.
+
+    Where n and m are multiplied apart, n's weight is w s in two fp16 parts.  The second part (the
+    remainder of the first, below 2^-10 of it) is mostly subnormal, a multiple of 2^-24, and two
+    roundings to that take up to 2^-25 each: 2^-24 n <= 15 * 2^-24 a token, also where v = n s + m
+    itself is near 0.  The weights' largest is at least 1, so of the output this is p_max times
+    as much, T tokens at most, or six times sqrt(T / 3) where they are many."""
     n, hq, d = q.shape
     ctx, hkv = k.shape[:2]
     g = hq // hkv
@@ -166,7 +172,8 @@ def attention(q, k, v, start, scale):
         own = (p * p) @ vj ** 2 * half ** 2 / 3
         out[:, j] = o
         tol[:, j] = 6 * torch.sqrt((spread + own).clamp(min=0)) + \
-            ctx * 2.0 ** -24 * vj.abs().amax() + 2.0 ** -20 * (p @ vj.abs())
+            ctx * 2.0 ** -24 * vj.abs().amax() + 2.0 ** -20 * (p @ vj.abs()) + \
+            p.amax(-1, keepdim=True) * min(ctx, 6 * math.sqrt(ctx / 3)) * 15 * 2.0 ** -24
     return out, tol
 
 

@@ -142,45 +142,46 @@ def test_binding_refusals():
     """Shapes, types and strides that the binding checks before a call (tensors on the CPU)."""
     lib = object.__new__(library.LucAttn)
     lib.lib, lib.ctx, lib.device = library.load_cdll(), ctypes.c_void_p(), 0
+    stream = types.SimpleNamespace(cuda_stream=0)
     i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
     i64 = lambda *s: torch.zeros(s, dtype=torch.int64)  # noqa: E731
     ext = dict(new_tokens=i32(2), lens=i32(2), tables=i32(2, 4), free_list=i32(8), state=i32(4), slots=i64(5),
-               positions=i32(5), cu_seqlens=i32(3), start_pos=i32(2))
+               positions=i32(5), cu_seqlens=i32(3), start_pos=i32(2),
+               stream=stream)
     for k, v in dict(new_tokens=i64(2), lens=i32(1), tables=i64(2, 4), state=i32(3), slots=i32(5), positions=i32(4),
                      cu_seqlens=i32(2), start_pos=i32(1), free_list=i32(16)[::2]).items():
         with pytest.raises(ValueError):
             lib.block_extend(**(ext | {k: v}))
     with pytest.raises(ValueError):
-        lib.block_truncate(i32(1), i32(2), i32(2, 4), i32(8), i32(4))
+        lib.block_truncate(i32(1), i32(2), i32(2, 4), i32(8), i32(4), stream=stream)
     half = lambda *s: torch.zeros(s, dtype=torch.float16)  # noqa: E731
     qkv = half(3, 8 * 64)
     q, k, v = qkv[:, :256], qkv[:, 256:384], qkv[:, 384:]
     cos = torch.zeros(10, 32)
     pool4 = torch.zeros(2, 1, 2, 640, dtype=torch.uint8)
     base = dict(q=q, k=k, v=v, cos=cos, sin=cos, positions=i32(3), slots=i64(3), k_pool=pool4, v_pool=pool4, layer=0,
-                num_layers=1, hq=4, hkv=2, head_dim=64)
+                num_layers=1, hq=4, hkv=2, head_dim=64, stream=stream)
     for kw in (dict(q=q[:, :128]), dict(k=half(3, 128)), dict(v=v[:2]), dict(q_out=half(2, 256)), dict(cos=cos[:, :16]),
                dict(positions=i32(2)), dict(slots=i32(3)), dict(k_pool=pool4[..., :600]), dict(k_pool=half(2, 1, 2, 640)),
                dict(q_norm=half(32), k_norm=half(32)), dict(q_bias=half(128)), dict(k_out=half(3, 64)),
                dict(k_out=half(3, 128), v_out=half(3, 136)[:, :128])):
-        with pytest.raises(ValueError):
+        with pytest.raises((TypeError, ValueError)):
             lib.kv4_append(**(base | kw))
     for kw in (dict(k=k.bfloat16()), dict(q_out=torch.zeros(3, 256)), dict(v_bias=torch.zeros(128))):
         with pytest.raises((TypeError, ValueError)):
             lib.kv4_append(**(base | kw))
-    with pytest.raises(TypeError):
+    with pytest.raises((TypeError, ValueError)):
         lib.qk_norm_rope_append(**(base | dict(k_pool=torch.zeros(2, 1, 2, 16, 64), v_pool=half(2, 1, 2, 16, 64))))
-    stream = types.SimpleNamespace(cuda_stream=0)
     with pytest.raises(library.LucError, match="null context"):  # what is right reaches the library
-        lib.kv4_append(**base, stream=stream)
+        lib.kv4_append(**base)
     att = dict(out=half(3, 256), q=q, k_pool=pool4, v_pool=pool4, tables=i32(3, 2), start_pos=i32(3), batch=3,
-               total_rows=3, max_rows=1, max_ctx=32, layer=0, num_layers=1, hq=4, hkv=2, head_dim=64, sm_scale=0.125)
+               total_rows=3, max_rows=1, max_ctx=32, layer=0, num_layers=1, hq=4, hkv=2, head_dim=64, sm_scale=0.125, stream=stream)
     for kw in (dict(out=half(2, 256)), dict(out=torch.zeros(3, 256)), dict(q=half(3, 128)), dict(tables=i32(2, 2)),
                dict(start_pos=i32(2)), dict(cu_seqlens=i32(3)), dict(v_pool=pool4[:, :, :1]), dict(total_rows=4)):
-        with pytest.raises(ValueError):
+        with pytest.raises((TypeError, ValueError)):
             lib.kv4_attention(**(att | kw))
     with pytest.raises(library.LucError, match="null context"):
-        lib.kv4_attention(**att, stream=stream)
+        lib.kv4_attention(**att)
 
 
 def test_kernels_keep_their_values_in_registers():
