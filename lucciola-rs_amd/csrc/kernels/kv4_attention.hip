@@ -7,22 +7,18 @@
 // Columns.  The (row, head of the group) pairs of one sequence and kv head are the columns of
 // the products: S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_16x16x32_f16, 16 columns a fragment.
 // In the accumulators a lane has one column throughout (column lane % 16), so maxima, sums and
-// rescaling are lane-local up to the four lanes that share it, and the scores of a tile of
-// 32 tokens are already the operand of the second product: lane l holds rows 4 (l / 16) .. + 3 of two
-// 16-token fragments, whose tokens are dealt so that those 8 are tokens 8 (l / 16) .. + 7.
+// rescaling are lane-local up to the four lanes that share it, and the scores of 32 tokens are
+// already the operand of the second product: lane l holds four tokens of either 16-token fragment.
+// q is taken to fp16 after a power of two brings its largest element near one, exactly unless an
+// element is 2^-14 of that.  The running maximum moves only when a score passes it by some powers
+// of two, so most tiles rescale nothing.
 //
-// Operands.  A lane expands n to fp16 in registers: four n of a dword at a time fall in place of
-// the low bits of 1024.0 (or 16 n in those), one packed add or FMA makes them whole, one
-// packed FMA applies s and m: 13 VALU instructions for 8 values, no LDS.  K and V are rounded to fp16
-// there (2^-11 of the value at most, against a step of 1/15 of the group's range); q is taken to fp16 after
-// a power of two brings its largest element into [1, 2), exactly unless an element is 2^-14 of that.
-// P is fp16 in (0, 2^kLazyMax], and l sums the rounded P.
-//
-// Two work splits:
-//   tokens: 16 columns a workgroup; its 4 waves take 32-token tiles in turn and merge in LDS.
-//     Few columns a sequence (decode): every wave streams its own part of the cache.
-//   columns: 64 columns a wave, 4 waves, every wave walks all tiles of its context.  Prompts: an
-//     expanded tile serves 4 fragments.
+// Two kernels:
+//   tokens: 8 columns a workgroup; its 4 waves take stages of tokens in turn and merge in LDS.  Few
+//     columns a sequence (decode): every wave streams its own part of the cache, n goes to the
+//     matrix unit as it is, and s and m are applied to sums.
+//   columns: 128 (D = 64) or 256 columns a workgroup, every wave walks all tokens of its columns'
+//     contexts.  Prompts: an expanded tile of n s + m serves all of them.
 // Either may cut the context into splits over workgroups, whose partial (m, l, o) go to the
 // workspace; tokens: the last workgroup of a (sequence, kv head, column tile) to arrive
 // merges them; columns: a second launch does.
@@ -82,306 +78,23 @@ __device__ inline void expand8(uint32_t w, half2_t s, half2_t m, uint32_t* o) {
   o[3] = as_u(__builtin_elementwise_fma(n3, s, m));
 }
 
+// The four pairs as they are.
+__device__ inline void whole8(uint32_t w, uint32_t* o) {
+  uint32_t kBig = 0x64006400u;
+  asm("" : "+v"(kBig));
+  const half2_t big = {(_Float16)1024.0f, (_Float16)1024.0f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = as_u(as_h2((w >> (4 * i) & 0x000f000fu) | kBig) - big);
+}
+// NaN where one is.  (fmaxf, which passes over it, would first quiet every operand.)
+__device__ inline float max3(float a, float b, float c) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
+}
+
 // Of a pair of tokens' s and m, bit 15 or 31 where a token's is NaN (the format has no
 // infinities: an exponent of all ones is NaN).
 __device__ inline uint32_t kv4_nan(uint32_t s, uint32_t m) {
   return (((s & 0x7c007c00u) + 0x04000400u) | ((m & 0x7c007c00u) + 0x04000400u)) & 0x80008000u;
-}
-
-// s and m of V for the lane's tokens first .. first + 7, of half h of its dimensions, in a tile
-// at some column's edge.  Tokens that no column sees (from ctx on) hold anything: their s and m
-// become 0.  A NaN value that only some columns see must not reach the others through 0 * NaN: it
-// becomes 0 too, and nan_at, the first such position in group 2 h + g / 2, the one of the lane's
-// outputs, tells which columns get their NaN after the last tile.
-__device__ __attribute__((always_inline)) inline void kv4_mask_values(u32x4_t& vs, u32x4_t& vm, int first, int ctx, int g, int& nan_at) {
-  uint32_t any = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t keep = (first + 2 * i < ctx ? 0xffffu : 0u) | (first + 2 * i + 1 < ctx ? 0xffff0000u : 0u);
-    vs[i] &= keep;
-    vm[i] &= keep;
-    any |= kv4_nan(vs[i], vm[i]);
-  }
-  if (!__any(any != 0)) return;
-  int at = 0x7fffffff;
-#pragma unroll
-  for (int i = 3; i >= 0; --i) {
-    const uint32_t nan = kv4_nan(vs[i], vm[i]);
-    if (nan & 0x80000000u) at = first + 2 * i + 1;
-    if (nan & 0x8000u) at = first + 2 * i;
-    const uint32_t keep = (nan & 0x8000u ? 0u : 0xffffu) | (nan & 0x80000000u ? 0u : 0xffff0000u);
-    vs[i] &= keep;
-    vm[i] &= keep;
-  }
-  // first of group 2 h + n / 8, from its lanes to those of group 2 h + g / 2
-  at = min(at, __shfl_xor(at, 16));
-  at = min(at, __shfl_xor(at, 32));
-  nan_at = min(nan_at, __shfl(at, 8 * (g >> 1)));
-}
-
-// What a lane loads of a 32-token tile.
-template <int D> struct Kv4Tile {
-  static constexpr int KW = D / 32;  // dwords of K per token (16 or 32 dimensions)
-  static constexpr int H = D / 64;   // V quads per lane
-  uint32_t k[2][KW];                 // fragments a and b
-  uint32_t ksm[2];
-  uint4 v[H], vs[H], vm[H];
-};
-
-// One wave's walk over tiles for F fragments of 16 columns.
-template <int DT, int D, int F> struct Kv4Wave {
-  static constexpr int KS = D / 32;  // k steps of a score
-  static constexpr int NF = D / 16;  // output fragments: 4 a quad of V
-  static constexpr int H = D / 64;
-
-  uint4 q[F][KS];
-  f32x4_t acc[F][NF];
-  float m[F], l[F], scale[F];
-  int limit[F];  // last position that the lane's column sees
-  int nan_at[H];  // first NaN value (of a tile at an edge) in the group of the lane's outputs
-  int lane, n, g;
-
-  // Columns col0 + 16 f + n of a sequence with ncols of them whose first row is at `start`.
-  __device__ __attribute__((always_inline)) inline void begin(const Kv4AttnArgs& A, int64_t row0, int kvh, int start, int ctx, int col0,
-                               int ncols) {
-    lane = threadIdx.x & 63;
-    n = lane & 15;
-    g = lane >> 4;
-#pragma unroll
-    for (int h = 0; h < H; ++h) nan_at[h] = 0x7fffffff;
-#pragma unroll
-    for (int f = 0; f < F; ++f) {
-      const int col = col0 + 16 * f + n;
-      const bool on = col < ncols;
-      const int r = on ? col / A.group : 0, hd = on ? col % A.group : 0;
-      limit[f] = on ? start + r : ctx - 1;
-      const uint16_t* const src = A.q + (row0 + r) * A.q_stride + ((int64_t)kvh * A.group + hd) * D + g * (D / 4);
-      // the lane's D / 4 dimensions: those of its K loads
-      float x[D / 4];
-      float top = 0.0f;
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        const uint4 w = on ? *(const uint4*)(src + 8 * i) : make_uint4(0, 0, 0, 0);
-        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[8 * i + 2 * e] = St<DT>::lo(ww[e]);
-          x[8 * i + 2 * e + 1] = St<DT>::hi(ww[e]);
-          top = fmaxf(top, fmaxf(fabsf(x[8 * i + 2 * e]), fabsf(x[8 * i + 2 * e + 1])));
-        }
-      }
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      // 2^-e of the largest element (infinities and NaN stay what they are)
-      const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);
-      const float down = __uint_as_float((uint32_t)(254 - e) << 23);
-      scale[f] = A.qk_scale_log2 * __uint_as_float((uint32_t)e << 23);
-#pragma unroll
-      for (int j = 0; j < KS; ++j) {
-        uint32_t o[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const half2_t p = {(_Float16)(x[8 * j + i] * down), (_Float16)(x[8 * j + i + 4] * down)};
-          o[i] = as_u(p);
-        }
-        q[f][j] = make_uint4(o[0], o[1], o[2], o[3]);
-      }
-      m[f] = -3.4028235e38f;
-      l[f] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < NF; ++i) acc[f][i] = (f32x4_t){0, 0, 0, 0};
-    }
-  }
-
-  // Byte offsets of the lane's loads within slabs; page: which of the tile's two.
-  struct Offsets {
-    int k, ksm, v, vs;
-    bool kpage, vpage;
-  };
-  __device__ __attribute__((always_inline)) inline Offsets offsets() const {
-    // fragment a's row n is token 8 (n / 4) + n % 4 of the tile, b's 4 further
-    const int tok = 8 * (n >> 2) + (n & 3), t = tok & 15;
-    Offsets o;
-    o.kpage = tok >= 16;
-    o.k = Kv4<D>::k_row(t) + g * (D / 8);
-    o.ksm = Kv4<D>::k_scale(t, D == 128 ? g : g >> 1);
-    o.vpage = g >= 2;
-    o.v = Kv4<D>::v_quad(8 * (g & 1), n);
-    o.vs = Kv4<D>::v_scale(g & 1, n >> 3);
-    return o;
-  }
-  __device__ __attribute__((always_inline)) inline void load(Kv4Tile<D>& t, const Offsets& o, const char* kp, const char* vp, int64_t page_stride,
-                              int p0, int p1) const {
-    const char* const kb = kp + (o.kpage ? p1 : p0) * page_stride;
-    const char* const vb = vp + (o.vpage ? p1 : p0) * page_stride;
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      if constexpr (D == 128) {
-        const uint4 x = *(const uint4*)(kb + o.k + b * 4 * (D / 2));
-        t.k[b][0] = x.x; t.k[b][1] = x.y; t.k[b][2] = x.z; t.k[b][3] = x.w;
-      } else {
-        const uint2 x = *(const uint2*)(kb + o.k + b * 4 * (D / 2));
-        t.k[b][0] = x.x; t.k[b][1] = x.y;
-      }
-      t.ksm[b] = *(const uint32_t*)(kb + o.ksm + b * 4 * Kv4<D>::kGroups * 4);
-    }
-#pragma unroll
-    for (int h = 0; h < H; ++h) {
-      t.v[h] = *(const uint4*)(vb + o.v + h * 256);       // 16 quads on
-      t.vs[h] = *(const uint4*)(vb + o.vs + h * 64);      // two groups on
-      t.vm[h] = *(const uint4*)(vb + o.vs + h * 64 + 16);
-    }
-  }
-
-  // One tile of tokens tok0 .. tok0 + 31.  edge (alike in all lanes): some column's limit lies
-  // before its end.
-  __device__ __attribute__((always_inline)) inline void step(Kv4Tile<D>& t, int tok0, int ctx, bool edge) {
-    // ---- scores
-    uint4 ka[2][KS];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const half2_t sm = as_h2(t.ksm[b]);
-      const half2_t s = {sm.x, sm.x}, mm = {sm.y, sm.y};
-#pragma unroll
-      for (int j = 0; j < KS; ++j) {
-        uint32_t o[4];
-        expand8(t.k[b][j], s, mm, o);
-        ka[b][j] = make_uint4(o[0], o[1], o[2], o[3]);
-      }
-    }
-    const int first = tok0 + 8 * g;  // the lane's 8 tokens
-    uint4 p[F];
-#pragma unroll
-    for (int f = 0; f < F; ++f) {
-      float s[8];
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        f32x4_t c = {0, 0, 0, 0};
-#pragma unroll
-        for (int j = 0; j < KS; ++j) c = mfma16(ka[b][j], q[f][j], c);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[4 * b + i] = c[i] * scale[f];
-      }
-      if (edge) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s[i] = first + i <= limit[f] ? s[i] : -INFINITY;
-      }
-      float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-      if (__any(top > m[f] + kLazyMax)) {
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float mn = fmaxf(m[f], top);
-        const float a = __builtin_amdgcn_exp2f(m[f] - mn);
-        m[f] = mn;
-        l[f] *= a;
-#pragma unroll
-        for (int i = 0; i < NF; ++i) acc[f][i] *= a;
-      }
-      uint32_t o[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = __builtin_amdgcn_exp2f(s[2 * i] - m[f]), y = __builtin_amdgcn_exp2f(s[2 * i + 1] - m[f]);
-        const half2_t h = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(x, y));
-        o[i] = as_u(h);
-        l[f] = __builtin_amdgcn_fdot2(h, (half2_t){(_Float16)1.0f, (_Float16)1.0f}, l[f], false);
-      }
-      p[f] = make_uint4(o[0], o[1], o[2], o[3]);
-    }
-    // ---- output
-    if (edge) {
-      u32x4_t vs[H], vm[H];
-#pragma unroll
-      for (int h = 0; h < H; ++h) {
-        vs[h] = __builtin_bit_cast(u32x4_t, t.vs[h]);
-        vm[h] = __builtin_bit_cast(u32x4_t, t.vm[h]);
-      }
-#pragma unroll
-      for (int h = 0; h < H; ++h) {
-        kv4_mask_values(vs[h], vm[h], first, ctx, g, nan_at[h]);
-        t.vs[h] = __builtin_bit_cast(uint4, vs[h]);
-        t.vm[h] = __builtin_bit_cast(uint4, vm[h]);
-      }
-    }
-#pragma unroll
-    for (int h = 0; h < H; ++h) {
-      const uint32_t vw[4] = {t.v[h].x, t.v[h].y, t.v[h].z, t.v[h].w};
-      const uint32_t sw[4] = {t.vs[h].x, t.vs[h].y, t.vs[h].z, t.vs[h].w};
-      const uint32_t mw[4] = {t.vm[h].x, t.vm[h].y, t.vm[h].z, t.vm[h].w};
-      uint32_t o[4][4];  // [pair of tokens][dimension]
-#pragma unroll
-      for (int i = 0; i < 4; ++i) expand8(vw[i], as_h2(sw[i]), as_h2(mw[i]), o[i]);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const uint4 va = make_uint4(o[0][c], o[1][c], o[2][c], o[3][c]);
-#pragma unroll
-        for (int f = 0; f < F; ++f) acc[f][4 * h + c] = mfma16(va, p[f], acc[f][4 * h + c]);
-      }
-    }
-  }
-
-  // The sums of the columns after the last tile: l over the lanes of a column, NaN where the
-  // column saw a page outside the pool (bad_at: the first one's position) or a NaN value.
-  __device__ __attribute__((always_inline)) inline void finish(int bad_at) {
-#pragma unroll
-    for (int f = 0; f < F; ++f) {
-      l[f] += __shfl_xor(l[f], 16);
-      l[f] += __shfl_xor(l[f], 32);
-      if (limit[f] >= bad_at) l[f] = __builtin_nanf("");
-#pragma unroll
-      for (int h = 0; h < H; ++h)
-        if (limit[f] >= nan_at[h]) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) acc[f][4 * h + c] = (f32x4_t)__builtin_nanf("");
-        }
-    }
-  }
-};
-
-// Page numbers of the pair of pages of up to 64 tiles, one tile a lane.
-struct Kv4Pages {
-  int p0, p1;
-  // tile of lane i: base + i * step; tokens at and past ctx have none
-  __device__ __attribute__((always_inline)) inline void load(const int32_t* table, int tile0, int step, int ctx, int num_blocks, int& bad_at) {
-    const int lane = threadIdx.x & 63;
-    const int64_t tok = ((int64_t)tile0 + (int64_t)lane * step) * 32;
-    p0 = tok < ctx ? table[tok / kPage] : 0;
-    p1 = tok + kPage < ctx ? table[tok / kPage + 1] : 0;
-    // a page outside the pool is never an address: page 0 is read instead
-    int bad = 0x7fffffff;
-    if (p1 < 0 || p1 >= num_blocks) { bad = (int)tok + kPage; p1 = 0; }
-    if (p0 < 0 || p0 >= num_blocks) { bad = (int)tok; p0 = 0; }
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) bad = min(bad, __shfl_xor(bad, k));
-    bad_at = min(bad_at, bad);
-  }
-};
-
-// Tiles tile0, tile0 + step, ... < tile_end of the sequence, for one wave.
-template <int DT, int D, int F>
-__device__ __attribute__((always_inline)) inline void kv4_walk(const Kv4AttnArgs& A, Kv4Wave<DT, D, F>& W, const int32_t* table, int kvh, int tile0, int tile_end,
-                                int step, int ctx, int min_limit, int& bad_at) {
-  const int64_t page_stride = (int64_t)A.num_layers * A.hkv * Kv4<D>::kSlab;
-  const int64_t base = ((int64_t)A.layer * A.hkv + kvh) * Kv4<D>::kSlab;
-  const char* const kp = A.k_pool + base;
-  const char* const vp = A.v_pool + base;
-  const auto off = W.offsets();
-  for (int t0 = tile0; t0 < tile_end; t0 += 64 * step) {
-    Kv4Pages pages;
-    pages.load(table, t0, step, ctx, A.num_blocks, bad_at);
-    const int count = min(64, (tile_end - t0 + step - 1) / step);
-    auto at = [&](Kv4Tile<D>& t, int i) __attribute__((always_inline)) {
-      W.load(t, off, kp, vp, page_stride, __builtin_amdgcn_readlane(pages.p0, i),
-             __builtin_amdgcn_readlane(pages.p1, i));
-    };
-    Kv4Tile<D> cur, next;
-    at(cur, 0);
-    for (int i = 0; i < count; ++i) {
-      at(next, min(i + 1, count - 1));
-      const int tok0 = (t0 + i * step) * 32;
-      W.step(cur, tok0, ctx, tok0 + 31 > min_limit);
-      cur = next;
-    }
-  }
 }
 
 // A sequence's rows, the position of the first, and its context: 0 where that is longer, or the
@@ -1094,70 +807,479 @@ __device__ void kv4_tokens_impl(const Kv4AttnArgs& A) {
 }
 
 // ---- waves split columns: one workgroup per (chunk of columns, sequence, kv head, split) ----
-constexpr int kColWaves = 4;
+//
+// The waves expand a tile of 64 tokens together into LDS in operand order (a lane's 16 bytes
+// of every operand side by side: reads without conflicts), one tile ahead of the products and with
+// the loads of another under way; one barrier a tile.  A k step of a score is a group of 32
+// dimensions.
+//   bf16 rows: K and V are n s + m in fp16, one rounding of 2^-12, far below the output's 2^-9.
+//   fp16 rows (EXACT): that rounding of K and P's own would each add an error as large as the output's.
+//     K is n, and a group's products are scaled by s in 32 bits; the group's sum of q times m, q's sums
+//     in two fp16 parts, are a product of their own.  P is two fp16 parts.  V stays n s + m.
+template <int DT, int D> struct Kv4Tile {
+  static constexpr bool EXACT = DT == kF16;
+  static constexpr int KS = D / 32;   // k steps of a score
+  static constexpr int NF = D / 16;   // output fragments: 4 a quad of V
+  uint4 k[4][KS][64];                 // [fragment of 16 tokens][step][lane]
+  uint4 v[2][NF][64];                 // [half][fragment of dimensions][lane]
+  uint16_t ks[EXACT ? 4 : 1][16][KS]; // s by token and group
+  uint4 km[EXACT ? 4 : 1][16];        // m by token: the groups', repeated to 8
+};
 template <int D> struct Kv4Cols {
-  static constexpr int F = D == 64 ? 4 : 2;  // fragments of a wave
-  static constexpr int N = kColWaves * F * 16;
+  static constexpr int WAVES = D == 128 ? 8 : 4;
+  static constexpr int F = 2;  // fragments of a wave
+  static constexpr int N = WAVES * F * 16;
+};
+
+// What a wave loads of a tile and makes of it: of page w % 4, C dwords of K a lane, and V's quads n + 16 h
+// for HW halves h of the dimensions, four tokens a lane (two dwords).  One page: its address is scalar.
+template <int DT, int D> struct Kv4Expand {
+  static constexpr bool EXACT = DT == kF16;
+  static constexpr int KS = D / 32, C = D / 8 / Kv4Cols<D>::WAVES, HW = C / 2;
+  uint32_t k[C], ksm;
+  uint2 v[HW], vs[HW], vm[HW];
+  const char* kp;  // page 0
+  const char* vp;
+  int ko, kso, vo, vso;  // of the lane in a page
+  int n, g, page, part;  // part: of the lane's D / 32 dwords of K, or of V's halves
+
+  __device__ __attribute__((always_inline)) inline void begin(const char* k_pool, const char* v_pool, int wave) {
+    const int lane = threadIdx.x & 63;
+    n = lane & 15;
+    g = lane >> 4;
+    page = wave & 3;
+    part = wave >> 2;
+    kp = k_pool;
+    vp = v_pool;
+    ko = (int)Kv4<D>::k_row(n) + g * (D / 8) + part * C * 4;
+    kso = (int)Kv4<D>::k_scale(n, D == 128 ? g : g >> 1);
+    vo = (int)Kv4<D>::v_quad(8 * (g >> 1), n + 16 * HW * part) + 8 * (g & 1);
+    vso = (int)Kv4<D>::v_scale(g >> 1, (n >> 3) + 2 * HW * part) + 8 * (g & 1);
+  }
+  // p (alike in all lanes): the page.
+  __device__ __attribute__((always_inline)) inline void load(int p, uint32_t page_stride) {
+    const uint64_t at = (uint64_t)(uint32_t)p * page_stride;
+    const char* const ka = kp + at;
+    const char* const va = vp + at;
+    if constexpr (C == 4) {
+      const uint4 y = *(const uint4*)(ka + ko);
+      k[0] = y.x; k[1] = y.y; k[2] = y.z; k[3] = y.w;
+    } else {
+      const uint2 y = *(const uint2*)(ka + ko);
+      k[0] = y.x; k[1] = y.y;
+    }
+    ksm = *(const uint32_t*)(ka + kso);
+#pragma unroll
+    for (int h = 0; h < HW; ++h) {
+      v[h] = *(const uint2*)(va + vo + 256 * h);
+      vs[h] = *(const uint2*)(va + vso + 64 * h);
+      vm[h] = *(const uint2*)(va + vso + 64 * h + 16);
+    }
+  }
+  // What tokens from `end` on hold is unknown, and no column that is kept sees it: their s and m of
+  // V become 0.  So do NaN ones', since 0 * NaN would reach columns that do not see them: nan_at, by
+  // group, keeps the first position.
+  __device__ __attribute__((always_inline)) inline void store(Kv4Tile<DT, D>& T, int tok0, int end, int* nan_at) {
+    const int lane = threadIdx.x & 63;
+    const half2_t sm = as_h2(ksm);
+    const half2_t ks = {sm.x, sm.x}, km = {sm.y, sm.y};
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      uint32_t o[4];
+      if constexpr (EXACT) whole8(k[j], o); else expand8(k[j], ks, km, o);
+      // the lane's dword i of dimensions 8 (D / 32 g + i) and the next 7
+      const int i = D / 32 * g + part * C + j;
+      T.k[page][i >> 2][16 * (i & 3) + n] = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+    if constexpr (EXACT) {
+      const int group = D == 128 ? g : g >> 1;
+      if (part == 0 && (D == 128 || !(g & 1))) {
+        T.ks[page][n][group] = (uint16_t)ksm;
+        uint16_t* const to = (uint16_t*)&T.km[page][n] + group;
+#pragma unroll
+        for (int r = 0; r < 8; r += KS) to[r] = (uint16_t)(ksm >> 16);
+      }
+    }
+    const int first = tok0 + 16 * page + 4 * g;  // of the lane's four tokens
+    if (tok0 + 64 > end) {
+      const uint32_t lo = (first < end ? 0xffffu : 0u) | (first + 1 < end ? 0xffff0000u : 0u);
+      const uint32_t hi = (first + 2 < end ? 0xffffu : 0u) | (first + 3 < end ? 0xffff0000u : 0u);
+#pragma unroll
+      for (int h = 0; h < HW; ++h) {
+        vs[h].x &= lo; vs[h].y &= hi;
+        vm[h].x &= lo; vm[h].y &= hi;
+      }
+    }
+    // 0 times s and m: NaN where one is not finite (the format has no infinities)
+    half2_t any = {(_Float16)0.0f, (_Float16)0.0f};
+    const half2_t zero = any;
+#pragma unroll
+    for (int h = 0; h < HW; ++h) {
+      any = __builtin_elementwise_fma(as_h2(vs[h].x), zero, any);
+      any = __builtin_elementwise_fma(as_h2(vs[h].y), zero, any);
+      any = __builtin_elementwise_fma(as_h2(vm[h].x), zero, any);
+      any = __builtin_elementwise_fma(as_h2(vm[h].y), zero, any);
+    }
+    if (__any((as_u(any) & 0x7fff7fffu) != 0)) {
+#pragma unroll
+      for (int h = 0; h < HW; ++h) {
+        const uint32_t lo = kv4_nan(vs[h].x, vm[h].x), hi = kv4_nan(vs[h].y, vm[h].y);
+        const uint32_t keep_lo = (lo & 0x8000u ? 0u : 0xffffu) | (lo & 0x80000000u ? 0u : 0xffff0000u);
+        const uint32_t keep_hi = (hi & 0x8000u ? 0u : 0xffffu) | (hi & 0x80000000u ? 0u : 0xffff0000u);
+        vs[h].x &= keep_lo; vm[h].x &= keep_lo;
+        vs[h].y &= keep_hi; vm[h].y &= keep_hi;
+        if (lo | hi)
+          atomicMin(nan_at + (n >> 3) + 2 * (HW * part + h),
+                    first + (lo & 0x8000u ? 0 : lo ? 1 : hi & 0x8000u ? 2 : 3));
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < HW; ++h) {
+      uint32_t o[2][4];  // [pair of tokens][dimension]
+      expand8(v[h].x, as_h2(vs[h].x), as_h2(vm[h].x), o[0]);
+      expand8(v[h].y, as_h2(vs[h].y), as_h2(vm[h].y), o[1]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        ((uint2*)&T.v[page >> 1][4 * (HW * part + h) + c][lane])[page & 1] = make_uint2(o[0][c], o[1][c]);
+    }
+  }
+};
+
+// One wave's F fragments of 16 columns over tiles.
+template <int DT, int D> struct Kv4Chunk {
+  static constexpr bool EXACT = DT == kF16;
+  static constexpr int F = Kv4Cols<D>::F, KS = D / 32, NF = D / 16, H = D / 64;
+  uint4 q[F][KS], qsum[EXACT ? F : 1];
+  f32x4_t acc[F][NF], l[F];
+  float m[F], scale[F], bar[F];
+  int limit[F];  // last position that the lane's column sees
+  int lane, n, g;
+
+  // Columns col0 + 16 f + n of a sequence with ncols of them whose first row is at `start`.
+  __device__ __attribute__((always_inline)) inline void begin(const Kv4AttnArgs& A, int64_t row0, int kvh, int start, int ctx, int col0,
+                                                              int ncols) {
+    lane = threadIdx.x & 63;
+    n = lane & 15;
+    g = lane >> 4;
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+      const int col = col0 + 16 * f + n;
+      const bool on = col < ncols;
+      const int r = on ? col / A.group : 0, hd = on ? col % A.group : 0;
+      limit[f] = on ? start + r : ctx - 1;
+      const uint16_t* const src = A.q + (row0 + r) * A.q_stride + ((int64_t)kvh * A.group + hd) * D + 8 * g;
+      float x[KS][8];
+      float top = 0.0f;
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        const uint4 w = on ? *(const uint4*)(src + 32 * j) : make_uint4(0, 0, 0, 0);
+        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[j][2 * e] = St<DT>::lo(ww[e]);
+          x[j][2 * e + 1] = St<DT>::hi(ww[e]);
+          top = fmaxf(top, fmaxf(fabsf(x[j][2 * e]), fabsf(x[j][2 * e + 1])));
+        }
+      }
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      // a power of two takes the largest element into [1, 2) (infinities and NaN stay so), and the
+      // scale's sign goes to q, so that the largest product is the largest score
+      const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);
+      const float down = copysignf(__uint_as_float((uint32_t)(254 - e) << 23), A.qk_scale_log2);
+      scale[f] = fabsf(A.qk_scale_log2) * __uint_as_float((uint32_t)e << 23);
+      if (scale[f] == 0.0f) scale[f] = 1e-37f;  // (a masked product, -inf, times 0 is NaN)
+      uint32_t sums[KS];  // of q by group: two fp16 parts
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        uint32_t o[4];
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const half2_t p = {(_Float16)(x[j][i] * down), (_Float16)(x[j][i + 4] * down)};
+          o[i] = as_u(p);
+          sum += (float)p.x + (float)p.y;
+        }
+        q[f][j] = make_uint4(o[0], o[1], o[2], o[3]);
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        const _Float16 hi = (_Float16)sum;
+        sums[j] = as_u((half2_t){hi, (_Float16)(sum - (float)hi)});
+      }
+      if constexpr (EXACT) {
+        // k slots 0 .. KS - 1 of lanes 0 .. 15: first parts; KS .. 2 KS - 1: second parts
+        auto pair = [](uint32_t a, uint32_t b, bool second) __attribute__((always_inline)) {
+          return second ? (a >> 16) | (b & 0xffff0000u) : (a & 0xffffu) | b << 16;
+        };
+        if constexpr (KS == 4)
+          qsum[f] = make_uint4(pair(sums[0], sums[1], false), pair(sums[2], sums[3], false),
+                               pair(sums[0], sums[1], true), pair(sums[2], sums[3], true));
+        else
+          qsum[f] = make_uint4(pair(sums[0], sums[1], false), pair(sums[0], sums[1], true), 0, 0);
+        if (g != 0) qsum[f] = make_uint4(0, 0, 0, 0);
+      }
+      m[f] = -3.4028235e38f;
+      bar[f] = -INFINITY;
+      l[f] = (f32x4_t){0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < NF; ++i) acc[f][i] = (f32x4_t){0, 0, 0, 0};
+    }
+  }
+
+  // Half `half` of a tile: tokens tok0 .. tok0 + 31.  edge (alike in all lanes): some column's limit
+  // lies before its end.
+  __device__ __attribute__((always_inline)) inline void step(const Kv4Tile<DT, D>& T, int half, int tok0, bool edge) {
+    const f32x4_t zero = {0, 0, 0, 0};
+    float s[F][8];  // tokens 4 g .. 4 g + 3 of either page
+    // all of K's reads under way before the first product, all of V's before the softmax
+    uint4 kk[2][KS], km[2], ks[2][KS / 2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int j = 0; j < KS; ++j) kk[b][j] = T.k[2 * half + b][j][lane];
+      if constexpr (EXACT) {
+        km[b] = T.km[2 * half + b][n];
+#pragma unroll
+        for (int i = 0; i < KS / 2; ++i) ks[b][i] = ((const uint4*)T.ks[2 * half + b][4 * g])[i];  // 4 tokens' s
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      f32x4_t t[F];
+      if constexpr (EXACT) {
+        uint32_t sc[2 * KS];
+#pragma unroll
+        for (int i = 0; i < KS / 2; ++i) {
+          sc[4 * i] = ks[b][i].x; sc[4 * i + 1] = ks[b][i].y; sc[4 * i + 2] = ks[b][i].z; sc[4 * i + 3] = ks[b][i].w;
+        }
+#pragma unroll
+        for (int f = 0; f < F; ++f) t[f] = mfma16(km[b], qsum[f], zero);
+#pragma unroll
+        for (int j = 0; j < KS; ++j)
+#pragma unroll
+          for (int f = 0; f < F; ++f) {
+            const f32x4_t c = mfma16(kk[b][j], q[f][j], zero);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const half2_t sj = as_h2(sc[(i * KS + j) / 2]);
+              t[f][i] = fmaf(c[i], (float)(j & 1 ? sj.y : sj.x), t[f][i]);
+            }
+          }
+      } else {
+#pragma unroll
+        for (int j = 0; j < KS; ++j)
+#pragma unroll
+          for (int f = 0; f < F; ++f) t[f] = mfma16(kk[b][j], q[f][j], j == 0 ? zero : t[f]);
+      }
+#pragma unroll
+      for (int f = 0; f < F; ++f)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[f][4 * b + i] = t[f][i];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    uint4 vv[NF];
+#pragma unroll
+    for (int i = 0; i < NF; ++i) vv[i] = T.v[half][i][lane];
+    __builtin_amdgcn_sched_barrier(0);
+    if (edge) {
+#pragma unroll
+      for (int f = 0; f < F; ++f) {
+        const int room = limit[f] - tok0 - 4 * g;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[f][i] = 16 * (i >> 2) + (i & 3) <= room ? s[f][i] : -INFINITY;
+      }
+    }
+    float top[F];
+    bool over = false;
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+      top[f] = max3(max3(s[f][0], s[f][1], s[f][2]), max3(s[f][3], s[f][4], s[f][5]), max3(s[f][6], s[f][7], s[f][7]));
+      over |= top[f] > bar[f];
+    }
+    if (__any(over)) {
+#pragma unroll
+      for (int f = 0; f < F; ++f) {
+        float t = fmaxf(top[f], __shfl_xor(top[f], 16));
+        t = fmaxf(t, __shfl_xor(t, 32));
+        const float mn = fmaxf(m[f], t * scale[f]);
+        const float a = __builtin_amdgcn_exp2f(m[f] - mn);
+        bar[f] = fmaxf(bar[f], t + kLazyMax / scale[f]);
+        m[f] = mn;
+        l[f] *= a;
+#pragma unroll
+        for (int i = 0; i < NF; ++i) acc[f][i] *= a;
+      }
+    }
+    float less = -1.0f;
+    asm("" : "+s"(less));  // (times a fp16, plus an fp32: one instruction)
+    uint4 p[F], p2[EXACT ? F : 1];
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+      uint32_t o[4], o2[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[f][2 * i], scale[f], -m[f]));
+        const float y = __builtin_amdgcn_exp2f(fmaf(s[f][2 * i + 1], scale[f], -m[f]));
+        o[i] = as_u((half2_t){(_Float16)x, (_Float16)y});
+        if constexpr (EXACT) {
+          asm("" : "+v"(o[i]));  // (converted once, as a pair)
+          const half2_t h = as_h2(o[i]);
+          o2[i] = as_u((half2_t){(_Float16)fmaf((float)h.x, less, x), (_Float16)fmaf((float)h.y, less, y)});
+        }
+      }
+      p[f] = make_uint4(o[0], o[1], o[2], o[3]);
+      if constexpr (EXACT) p2[f] = make_uint4(o2[0], o2[1], o2[2], o2[3]);
+    }
+    const uint4 ones = make_uint4(0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u);
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+      l[f] = mfma16(ones, p[f], l[f]);
+      if constexpr (EXACT) l[f] = mfma16(ones, p2[f], l[f]);
+    }
+#pragma unroll
+    for (int i = 0; i < NF; ++i)
+#pragma unroll
+      for (int f = 0; f < F; ++f) {
+        acc[f][i] = mfma16(vv[i], p[f], acc[f][i]);
+        if constexpr (EXACT) acc[f][i] = mfma16(vv[i], p2[f], acc[f][i]);
+      }
+  }
+
+  // After the last tile: NaN where a column saw a page outside the pool
+  // (bad_at: the first one's position) or a NaN value (nan_at, by group; a lane's outputs of half h
+  // are of group 2 h + g / 2).
+  __device__ __attribute__((always_inline)) inline void finish(int bad_at, const int* nan_at) {
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+      if (limit[f] >= bad_at) l[f][0] = __builtin_nanf("");
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+        if (limit[f] >= nan_at[2 * h + (g >> 1)]) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) acc[f][4 * h + c] = (f32x4_t)__builtin_nanf("");
+        }
+    }
+  }
 };
 
 template <int DT, int D>
 __device__ void kv4_columns_impl(const Kv4AttnArgs& A) {
-  constexpr int F = Kv4Cols<D>::F;
+  using C = Kv4Cols<D>;
+  constexpr int F = C::F;
+  __shared__ Kv4Tile<DT, D> s_tile[2];
+  __shared__ int s_nan[D / 32 + 1];  // and the first position of a page outside the pool
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // the chunks that see the longest contexts first
+  // The chunks that see the longest contexts first, and split 0, which every chunk has, before the
+  // others; neighbours of a pair on different XCDs (block x runs on XCD x % 8).
   const int pairs = A.batch * A.hkv;
-  const int split = blockIdx.x % A.splits, rest = blockIdx.x / A.splits;
-  const int chunk = A.tiles - 1 - rest / pairs, bh = rest % pairs;
+  const int split = blockIdx.x / (pairs * A.tiles), rest = blockIdx.x % (pairs * A.tiles);
+  const int chunk = A.tiles - 1 - rest / pairs, bh = (rest + rest / pairs) % pairs;
   const int b = bh / A.hkv, kvh = bh % A.hkv;
   const Kv4Seq S = kv4_seq(A, b);
-  const int ncols = S.rows * A.group;
-  const int col0 = chunk * Kv4Cols<D>::N + w * (16 * F);
-  const int here = min(16 * F, ncols - col0);
-  const int hq = A.hkv * A.group;
   if (S.ctx == 0) {
     if (split == 0 && chunk == 0) kv4_no_context<DT, D>(A, S, kvh);
     return;
   }
-  if (here <= 0) return;  // (no barrier follows)
-  const int last = S.start + (col0 + here - 1) / A.group;
+  const int ncols = S.rows * A.group;
+  const int all0 = chunk * C::N, all = min(C::N, ncols - all0);  // the workgroup's columns
+  if (all <= 0) return;
+  const int all_last = S.start + (all0 + all - 1) / A.group;
   const int begin = split * A.split_tokens;  // (splits x split_tokens fits: luc_kv4.cpp)
-  if (begin > last) return;
-  const int end = A.splits == 1 ? last + 1 : min(last + 1, begin + A.split_tokens);
-  Kv4Wave<DT, D, F> W;
-  W.begin(A, S.row0, kvh, S.start, S.ctx, col0, ncols);
-  int bad_at = 0x7fffffff;
-  kv4_walk<DT, D, F>(A, W, A.tables + (int64_t)b * A.table_stride, kvh, begin / 32, (end + 31) / 32, 1, S.ctx,
-                     S.start + col0 / A.group, bad_at);
-  W.finish(bad_at);
+  if (begin > all_last) return;
+  const int end = A.splits == 1 ? all_last + 1 : min(all_last + 1, begin + A.split_tokens);
+  const int col0 = all0 + w * (16 * F);
+  const int here = min(16 * F, ncols - col0);  // the wave's, or none
+  const int last = here > 0 ? S.start + (col0 + here - 1) / A.group : -1;
+  const int min_limit = S.start + col0 / A.group;
+  if (threadIdx.x <= D / 32) s_nan[threadIdx.x] = 0x7fffffff;
+
+  const uint32_t page_stride = (uint32_t)(A.num_layers * A.hkv) * Kv4<D>::kSlab;
+  const int64_t base = ((int64_t)A.layer * A.hkv + kvh) * Kv4<D>::kSlab;
+  const int32_t* const table = A.tables + (int64_t)b * A.table_stride;
+  Kv4Expand<DT, D> E;
+  E.begin(A.k_pool + base, A.v_pool + base, w);
+  const int count = (end - begin + 63) / 64;  // tiles
+  int bad_at = 0x7fffffff;  // of the wave's pages
+  int pages = 0;            // the wave's of tile i + lane
+  auto load = [&](int i) __attribute__((always_inline)) {
+    if ((i & 63) == 0) {
+      const int64_t at = begin + (int64_t)(i + (threadIdx.x & 63)) * 64 + 16 * E.page;
+      pages = at < end ? table[at / kPage] : 0;
+      // a page outside the pool is never an address: page 0 is read instead
+      const bool bad = pages < 0 || pages >= A.num_blocks;
+      if (__any(bad)) {
+        int first = bad ? (int)at : 0x7fffffff;
+#pragma unroll
+        for (int k = 1; k < 64; k <<= 1) first = min(first, __shfl_xor(first, k));
+        if (bad_at == 0x7fffffff && (threadIdx.x & 63) == 0) atomicMin(s_nan + D / 32, first);
+        bad_at = min(bad_at, first);
+        pages = bad ? 0 : pages;
+      }
+    }
+    E.load(__builtin_amdgcn_readlane(pages, i & 63), page_stride);
+  };
+  __syncthreads();  // s_nan
+  load(0);
+  Kv4Chunk<DT, D> W;
+  W.begin(A, S.row0, kvh, S.start, S.ctx, min(col0, ncols - 1), ncols);
+  E.store(s_tile[0], begin, min(end, bad_at), s_nan);
+  if (count > 1) load(1);
+  __syncthreads();
+  for (int i = 0; i < count; ++i) {
+    const int tok0 = begin + 64 * i;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int t = tok0 + 32 * half;
+      if (t <= last) W.step(s_tile[i & 1], half, t, t + 31 > min_limit);
+    }
+    // (every wave is done with the other tile since the last barrier)
+    if (i + 1 < count) {
+      E.store(s_tile[(i + 1) & 1], tok0 + 64, min(end, bad_at), s_nan);
+      if (i + 2 < count) load(i + 2);
+      __syncthreads();
+    }
+  }
+  W.finish(s_nan[D / 32], s_nan);
+  // A lane holds 16 dimensions of a column.  By way of the wave's share of the tiles, which no wave
+  // reads any more, D / 4 lanes write a column side by side.
+  __syncthreads();
+  const int hq = A.hkv * A.group;
+  float4* const turn = (float4*)s_tile + w * (4 * D);  // [16 columns][D / 4], swizzled
+  static_assert(sizeof(s_tile) >= C::WAVES * 4 * D * sizeof(float4), "a share holds 16 columns");
 #pragma unroll
   for (int f = 0; f < F; ++f) {
-    const float l = W.l[f];
-    const int col = col0 + 16 * f + W.n;
-    if (col >= ncols) continue;
-    const int64_t row = S.row0 + col / A.group;
-    const int head = kvh * A.group + col % A.group;
-    if (A.splits == 1) {
-      uint16_t* const dst = A.out + row * A.out_stride + (int64_t)head * D + 16 * W.g;
-      const float inv = 1.0f / l;
+    const float inv = A.splits == 1 ? 1.0f / W.l[f][0] : 1.0f;
 #pragma unroll
-      for (int h = 0; h < D / 64; ++h)
+    for (int h = 0; h < D / 64; ++h)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const uint32_t a0 = St<DT>::store(W.acc[f][4 * h][r] * inv) | (uint32_t)St<DT>::store(W.acc[f][4 * h + 1][r] * inv) << 16;
-          const uint32_t a1 = St<DT>::store(W.acc[f][4 * h + 2][r] * inv) | (uint32_t)St<DT>::store(W.acc[f][4 * h + 3][r] * inv) << 16;
-          *(uint2*)(dst + 64 * h + 4 * r) = make_uint2(a0, a1);
-        }
-    } else {
-      const int64_t at = ((int64_t)split * A.total_rows + row) * hq + head;
-      if (W.g == 0) *(float2*)(A.ws_ml + at * 2) = make_float2(W.m[f], l);
-      float* const po = A.ws_o + at * D + 16 * W.g;
-#pragma unroll
-      for (int h = 0; h < D / 64; ++h)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          *(float4*)(po + 64 * h + 4 * r) = make_float4(W.acc[f][4 * h][r], W.acc[f][4 * h + 1][r], W.acc[f][4 * h + 2][r],
-                                                        W.acc[f][4 * h + 3][r]);
+      for (int r = 0; r < 4; ++r)
+        turn[W.n * (D / 4) + ((16 * h + 4 * W.g + r) ^ W.n)] =
+            make_float4(W.acc[f][4 * h][r] * inv, W.acc[f][4 * h + 1][r] * inv, W.acc[f][4 * h + 2][r] * inv,
+                        W.acc[f][4 * h + 3][r] * inv);
+    if (A.splits > 1 && W.g == 0 && col0 + 16 * f + W.n < ncols) {
+      const int col = col0 + 16 * f + W.n;
+      const int64_t at = ((int64_t)split * A.total_rows + S.row0 + col / A.group) * hq + kvh * A.group + col % A.group;
+      *(float2*)(A.ws_ml + at * 2) = make_float2(W.m[f], W.l[f][0]);
     }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      const int c = (64 / (D / 4)) * i + W.lane / (D / 4), part = W.lane % (D / 4);
+      const int col = col0 + 16 * f + c;
+      const float4 x = turn[c * (D / 4) + (part ^ c)];
+      if (col >= ncols) continue;
+      const int64_t row = S.row0 + col / A.group;
+      const int head = kvh * A.group + col % A.group;
+      if (A.splits == 1) {
+        const uint32_t a0 = St<DT>::store(x.x) | (uint32_t)St<DT>::store(x.y) << 16;
+        const uint32_t a1 = St<DT>::store(x.z) | (uint32_t)St<DT>::store(x.w) << 16;
+        *(uint2*)(A.out + row * A.out_stride + (int64_t)head * D + 4 * part) = make_uint2(a0, a1);
+      } else {
+        *(float4*)(A.ws_o + (((int64_t)split * A.total_rows + row) * hq + head) * D + 4 * part) = x;
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   }
 }
 
@@ -1184,16 +1306,31 @@ __device__ void kv4_merge_impl(const Kv4AttnArgs& A) {
   if (r < 0 || r >= S.rows || S.ctx == 0) return;  // no sequence's row, or written already
   const int nsplit = min(A.splits, (S.start + r) / A.split_tokens + 1);
   const int64_t step = (int64_t)A.total_rows * hq;
-  float M = -INFINITY;
-  for (int s = 0; s < nsplit; ++s) M = fmaxf(M, A.ws_ml[(item + s * step) * 2]);
-  float L = 0.0f;
+  float M = -3.4028235e38f, L = 0.0f;
   float4 o = make_float4(0, 0, 0, 0);
-  for (int s = 0; s < nsplit; ++s) {
-    const float2 ml = *(const float2*)(A.ws_ml + (item + s * step) * 2);
-    const float e = __builtin_amdgcn_exp2f(ml.x - M);
-    const float4 x = *(const float4*)(A.ws_o + (item + s * step) * D + d);
-    L = fmaf(e, ml.y, L);
-    o.x = fmaf(e, x.x, o.x); o.y = fmaf(e, x.y, o.y); o.z = fmaf(e, x.z, o.z); o.w = fmaf(e, x.w, o.w);
+  // eight splits' loads under way at once (those past the last read the last again, times 0)
+  for (int s0 = 0; s0 < nsplit; s0 += 8) {
+    float2 ml[8];
+    float4 x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t at = item + min(s0 + i, nsplit - 1) * step;
+      ml[i] = *(const float2*)(A.ws_ml + at * 2);
+      x[i] = *(const float4*)(A.ws_o + at * D + d);
+    }
+    float top = M;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, ml[i].x);
+    const float a = __builtin_amdgcn_exp2f(M - top);
+    M = top;
+    L *= a;
+    o.x *= a; o.y *= a; o.z *= a; o.w *= a;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float e = s0 + i < nsplit ? __builtin_amdgcn_exp2f(ml[i].x - M) : 0.0f;
+      L = fmaf(e, ml[i].y, L);
+      o.x = fmaf(e, x[i].x, o.x); o.y = fmaf(e, x[i].y, o.y); o.z = fmaf(e, x[i].z, o.z); o.w = fmaf(e, x[i].w, o.w);
+    }
   }
   const float inv = 1.0f / L;
   const uint32_t a0 = St<DT>::store(o.x * inv) | (uint32_t)St<DT>::store(o.y * inv) << 16;
@@ -1207,7 +1344,7 @@ __device__ void kv4_merge_impl(const Kv4AttnArgs& A) {
   extern "C" __global__ __launch_bounds__(256, 2) void luc_kv4_tokens_##DTN##_d##D(luc::Kv4AttnArgs a) {  \
     luc::kv4_tokens_impl<luc::DT, D>(a);                                                         \
   }                                                                                              \
-  extern "C" __global__ __launch_bounds__(256, 2) void luc_kv4_columns_##DTN##_d##D(luc::Kv4AttnArgs a) { \
+  extern "C" __global__ __launch_bounds__(64 * luc::Kv4Cols<D>::WAVES, D == 128 || luc::DT == luc::kF16 ? 2 : 3) void luc_kv4_columns_##DTN##_d##D(luc::Kv4AttnArgs a) { \
     luc::kv4_columns_impl<luc::DT, D>(a);                                                        \
   }                                                                                              \
   extern "C" __global__ __launch_bounds__(256) void luc_kv4_merge_##DTN##_d##D(luc::Kv4AttnArgs a) {      \

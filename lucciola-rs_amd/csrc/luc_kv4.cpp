@@ -162,6 +162,22 @@ constexpr int kTokSlots = 2 * kCUs;           // resident workgroups
 // 93.8).
 constexpr int kTokMinSplit = 512, kTokMaxSplit = 2048;
 constexpr int kTokRounds = 8;  // rounds of workgroups balance any contexts: longer splits beyond
+// Up to 16 columns go to the tokens kernel, which reads the cache once for each 8; up to 48 while its
+// tiles leave the chip room.  us, tokens and columns kernel, sequences x rows at 1000..2000 tokens:
+//   14 and 2 heads of 64: 1 x 6 of 8000 12.6, 18.2; 16 x 6 17.4, 18.2; 64 x 3 21.1, 19.6;
+//     64 x 6 (768 tiles) 26.6, 23.0; 256 x 3 of 100..200 (1536) 15.5, 11.0
+//   12 and 2 of 128: 1 x 8 of 8000 15.3, 22.5; 64 x 4 30.5, 38.2; 64 x 8 (768 tiles) 45.7, 41.4
+constexpr int kTokMostCols = 48;
+// Columns of a workgroup of the columns kernel (Kv4Cols).
+constexpr int kColsOf64 = 128, kColsOf128 = 256;
+// Its splits fill the chip (128: a workgroup a CU; 64: two) once, but are not shorter than pays for
+// their partials.  us:
+//   512 rows after 8000, 12 and 2 of 128: 44.3 at 832 and 45.0 at 896 (the rule's), 71 at 768, where a
+//     second round begins; 64 rows: 26.0 at 256 (the rule's), 29.8 at 512
+//   14 and 2 of 64, 512 rows after 8000: 45.2 at 576, 36.5 at 640, 36.7 at 960 (the rule's), 38.4 at
+//     1088; 128 rows: 21.7 at 256, 20.6 at 512 (the rule's), 27.7 at 1024
+//   4 x 1531..2048 rows, 14 and 2 of 64: 67 at 1024, 47.6 whole (the rule's)
+constexpr int kColsMinSplit64 = 512, kColsMinSplit128 = 256, kColsMaxSplits = 32;
 constexpr int64_t kMaxArrivals = 1 << 16;     // (sequence, kv head, column tile)
 constexpr int kMaxCtx = 1 << 30;
 
@@ -177,11 +193,11 @@ struct Kv4Plan {
 Kv4Plan kv4_plan(int batch, int total_rows, int max_rows, int max_ctx, int hkv, int group, int head_dim) {
   Kv4Plan p;
   const int64_t cols = (int64_t)std::min(max_rows, total_rows) * group;
-  p.tokens = cols <= 2 * kTokCols;
   const int64_t pairs = (int64_t)batch * hkv;
+  const int64_t units = pairs * ceil_div(cols, kTokCols);
+  p.tokens = units <= kMaxArrivals && (cols <= 2 * kTokCols || (cols <= kTokMostCols && units <= kTokSlots));
   if (p.tokens) {
     p.tiles = (int)ceil_div(cols, kTokCols);
-    const int64_t units = pairs * p.tiles;
     // a stage for each of 4 waves
     const int round = head_dim == 64 ? 256 : 128;
     const int64_t fill = units * max_ctx / kTokSlots;
@@ -190,10 +206,12 @@ Kv4Plan kv4_plan(int batch, int total_rows, int max_rows, int max_ctx, int hkv, 
     p.split_tokens = (int)(ceil_div(st, round) * round);
     p.longest_first = p.tiles == 1 && batch <= 64 && units * ceil_div(max_ctx, p.split_tokens) > kTokSlots;
   } else {
-    p.tiles = (int)ceil_div(cols, head_dim == 64 ? 256 : 128);
+    p.tiles = (int)ceil_div(cols, head_dim == 64 ? kColsOf64 : kColsOf128);
     const int64_t wgs = pairs * p.tiles;
-    const int64_t want = std::min<int64_t>(std::max<int64_t>(ceil_div(2 * kCUs, wgs), 1), 32);
-    p.split_tokens = (int)(std::max<int64_t>(ceil_div(ceil_div(max_ctx, want), 32), 16) * 32);
+    const int64_t want = std::min<int64_t>(std::max<int64_t>((head_dim == 64 ? 2 : 1) * kCUs / wgs, 1), kColsMaxSplits);
+    const int64_t least = head_dim == 64 ? kColsMinSplit64 : kColsMinSplit128;
+    // whole tiles of 64 tokens
+    p.split_tokens = (int)(ceil_div(std::max(ceil_div(max_ctx, want), least), 64) * 64);
   }
   p.splits = (int)ceil_div(max_ctx, p.split_tokens);
   return p;
@@ -359,7 +377,7 @@ int luc_kv4_attention(luc_ctx* ctx, void* stream, int dtype, void* out, int64_t 
   if (int rc = get_fn(ctx, (plan.tokens ? "luc_kv4_tokens_" : "luc_kv4_columns_") + suffix, &fn)) return rc;
   if (int rc = get_fn(ctx, "luc_kv4_merge_" + suffix, &merge)) return rc;
   void* args[] = {&a};
-  if (int rc = launch(fn, dim3((unsigned)(units * plan.splits)), dim3(256), stream, args)) return rc;
+  if (int rc = launch(fn, dim3((unsigned)(units * plan.splits)), dim3(!plan.tokens && head_dim == 128 ? 512 : 256), stream, args)) return rc;
   if (plan.tokens || plan.splits == 1) return LUC_OK;
   const int64_t items = (int64_t)total_rows * num_q_heads;
   return launch(merge, dim3((unsigned)ceil_div(items, 1024 / head_dim)), dim3(256), stream, args);
