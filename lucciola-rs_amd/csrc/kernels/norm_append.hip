@@ -18,6 +18,14 @@
 // Lanes.  A head takes D / 16 lanes; a lane has elements 8 c .. 8 c + 7 and the same plus
 // D / 2 (a rotation's partners), and four lanes a group of the low and one of the high half: sums and
 // extremes of a head are DPP steps inside 4 or 8 lanes, no LDS.
+//
+// Order.  All of q, row by row; then k, then v, head by head: a wave has one kind, so that only those
+// of k and v encode, and the rows of a page, which are mostly neighbours, write V's two bytes a token
+// side by side.  4100 rows of 14 + 2 x 2 heads of 64 into 4 bits: 7.8 us, 11.0 head by head of a row.
+//
+// What bounds it.  8191 rows of 28 + 2 x 4 heads of 128, 16 bits: 27 us for 151 MB, what a large copy
+// reaches; 32 rows of 14 + 2 x 2 of 64: 3.4 us, 64 rows of 28 + 2 x 4 of 128 into 4 bits 4.9 us, the
+// latency of a launch and of position -> row of the table -> slot.
 #include "kv4.h"
 
 namespace luc {
@@ -143,16 +151,22 @@ template <int DT, int D, bool POOL4>
 __device__ void norm_append_impl(const NormAppendArgs& A) {
 #pragma clang fp contract(off)
   constexpr int LANES = D / 16;
-  const int heads = A.hq + 2 * A.hkv;
-  const int64_t unit = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / LANES;
+  uint32_t unit = (blockIdx.x * blockDim.x + threadIdx.x) / LANES;  // (the grid's threads fit 32 bits)
   const int c = threadIdx.x % LANES;
-  const int row = (int)(unit / heads);
-  if (row >= A.rows) return;
-  const int h = (int)(unit % heads);
+  const uint32_t nq = (uint32_t)A.rows * A.hq, nk = (uint32_t)A.rows * A.hkv;
+  if (unit >= nq + 2 * nk) return;
+  const int kind = unit < nq ? 0 : unit < nq + nk ? 1 : 2;  // q, k, v
+  int row, hh;
+  if (kind == 0) {
+    row = unit / A.hq;
+    hh = unit % A.hq;
+  } else {
+    unit -= kind == 1 ? nq : nq + nk;
+    hh = unit / A.rows;
+    row = unit % A.rows;
+  }
   const int pos = A.positions[row];
   if (pos < 0 || pos >= A.max_pos) return;
-  const int kind = h < A.hq ? 0 : h < A.hq + A.hkv ? 1 : 2;  // q, k, v
-  const int hh = kind == 0 ? h : kind == 1 ? h - A.hq : h - A.hq - A.hkv;
   const uint16_t* src = pick(kind, A.q, A.k, A.v);
   const uint16_t* const bias = pick(kind, A.q_bias, A.k_bias, A.v_bias);
   src += row * A.row_stride + hh * D;
