@@ -7,7 +7,8 @@ gfx950 code objects it loads.  This package binds it for Python callers:
   (torch provides device memory and streams);
 * ``engine``  -- the reference engine's host-side API for this path
   (RopeCache, KVCache, apply_rope, apply_flash_decoding), written over the
-  binding, plus batched forms.
+  binding, plus batched forms, page tables held on the GPU (DeviceBlocks) and
+  a 4-bit cache over them (Kv4Cache).
 
 There is no fallback: if the library is missing or fails to load, every call
 raises.
@@ -16,6 +17,8 @@ from .library import LucAttn, LucError, lib_dir  # noqa: F401
 from .engine import (  # noqa: F401
     RopeCache,
     KVCache,
+    DeviceBlocks,
+    Kv4Cache,
     apply_rope,
     apply_flash_decoding,
     decode_step,

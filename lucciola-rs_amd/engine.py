@@ -9,7 +9,9 @@ Mirrors, with the same names, argument meaning and error behaviour:
 * ``apply_flash_decoding`` -- CudaFunctions::apply_flash_decoding,
                               src/kernels.rs:248-320
 
-and adds the batched forms the kernels are built for (``decode_step``).
+and adds the batched forms the kernels are built for (``decode_step``), page
+tables that live on the GPU (``DeviceBlocks``) and a 4-bit cache over them
+(``Kv4Cache``).
 Device memory comes from torch; every launch goes through liblucattn.so.
 """
 from __future__ import annotations
@@ -225,6 +227,135 @@ class PagedKVCache:
         self.block_tables.copy_(torch.from_numpy(self.blocks.table()))
 
 
+class DeviceBlocks:
+    """Lengths, block tables and free list of up to `max_seqs` sequences over one
+    pool of `num_blocks` pages, held on the GPU: BlockManager's counterpart for
+    loops with no host work between steps, captured ones among them
+    (luc_block_extend, luc_block_truncate).  A fresh one hands out pages 0, 1,
+    2, ... as BlockManager does.
+
+    After `extend`, `slots` and `positions` are the step's packed new rows,
+    `cu_seqlens` and `start_pos` each sequence's rows among them.  Neither call
+    waits for the GPU, so neither can raise for a step that could not be met;
+    such a step takes nothing and has no rows, and `check()` raises for it.
+    Calls must be in one stream's order."""
+
+    def __init__(self, num_blocks: int, max_seqs: int, max_blocks_per_seq: int, max_rows: int,
+                 device="cuda", lib=None):
+        if min(num_blocks, max_seqs, max_blocks_per_seq, max_rows) < 1:
+            raise ValueError(f"num_blocks {num_blocks}, max_seqs {max_seqs}, max_blocks_per_seq "
+                             f"{max_blocks_per_seq} and max_rows {max_rows} must be positive")
+        self.lib = _lib(lib)
+        self.num_blocks, self.max_seqs, self.max_rows = num_blocks, max_seqs, max_rows
+        kw = {"dtype": torch.int32, "device": device}
+        self.lens = torch.zeros(max_seqs, **kw)
+        self.block_tables = torch.zeros((max_seqs, max_blocks_per_seq), **kw)
+        self.free_list = torch.arange(num_blocks - 1, -1, -1, **kw)
+        self.state = torch.tensor([num_blocks, 0, 0, 0], **kw)
+        self.slots = torch.full((max_rows,), -1, dtype=torch.int64, device=device)
+        self.positions = torch.full((max_rows,), -1, **kw)
+        self.cu_seqlens = torch.zeros(max_seqs + 1, **kw)
+        self.start_pos = torch.zeros(max_seqs, **kw)
+
+    def extend(self, new_tokens, rows: int | None = None, stream=None) -> None:
+        """Pages, slots and positions for new_tokens (device int32 [max_seqs]) more
+        tokens of every sequence, `rows` (default max_rows) of them at most."""
+        rows = self.max_rows if rows is None else rows
+        if not 0 <= rows <= self.max_rows:
+            raise ValueError(f"rows {rows} outside [0, {self.max_rows}]")
+        self.lib.block_extend(new_tokens, self.lens, self.block_tables, self.free_list, self.state,
+                              self.slots[:rows], self.positions[:rows], self.cu_seqlens,
+                              self.start_pos, stream=stream)
+
+    def truncate(self, keep, stream=None) -> None:
+        """Every sequence back to at most keep (device int32 [max_seqs]) tokens, the pages
+        behind those to the free list; the exact inverse of `extend`."""
+        self.lib.block_truncate(keep, self.lens, self.block_tables, self.free_list, self.state,
+                                stream=stream)
+
+    def check(self) -> None:
+        """Waits for the current stream; raises LucError (and forgets the fault) if a step since
+        the last call could not be met."""
+        status = int(self.state[1].item())
+        if status == 0:
+            return
+        self.state[1].zero_()
+        what = [text for bit, text in ((1, "free pages are short"), (2, "a block table row is"),
+                                       (4, "a length, count or the state is out of range"),
+                                       (8, "there are more rows than the step allows")) if status & bit]
+        raise library.LucError(-6 if status == 1 else -1, "page maps: " + "; ".join(what))
+
+    @property
+    def num_free(self) -> int:
+        """Free pages (waits for the current stream)."""
+        return int(self.state[0].item())
+
+
+class Kv4Cache:
+    """A 4-bit paged cache of up to `max_seqs` sequences (pools of luc_kv4_append, 0.31 of the
+    bytes of 16 bits) and the DeviceBlocks behind it.  A step: `extend`, then `append` and
+    `attend` for every layer; all of it may be captured in a HIP graph, and so may `truncate`.
+    Calls must be in one stream's order."""
+
+    def __init__(self, num_layers, num_q_heads, num_kv_heads, head_dim, num_physical_blocks,
+                 max_seqs, max_position_embeddings, max_rows=None, device="cuda", lib=None):
+        self.lib = _lib(lib)
+        if head_dim not in (64, 128):
+            raise library.LucError(-2, f"Unsupported head dimension for attention kernel: {head_dim}")
+        self.num_layers, self.num_q_heads = num_layers, num_q_heads
+        self.num_kv_heads, self.head_dim = num_kv_heads, head_dim
+        self.block_size = BLOCK_SIZE
+        self.max_seq_len = max_position_embeddings
+        self.blocks = DeviceBlocks(num_physical_blocks, max_seqs, ceil_div(max_position_embeddings, BLOCK_SIZE),
+                                   max_rows or max_seqs, device, self.lib)
+        shape = (num_physical_blocks, num_layers, num_kv_heads, 10 * head_dim)
+        self.k_pool = torch.zeros(shape, dtype=torch.uint8, device=device)
+        self.v_pool = torch.zeros(shape, dtype=torch.uint8, device=device)
+        self._workspaces = []  # the largest last; a captured graph may hold an earlier one
+
+    def extend(self, new_tokens, rows=None, stream=None):
+        self.blocks.extend(new_tokens, rows, stream)
+
+    def truncate(self, keep, stream=None):
+        self.blocks.truncate(keep, stream)
+
+    def append(self, layer, q, k, v, rope, q_bias=None, k_bias=None, v_bias=None, q_norm=None, k_norm=None,
+               eps=1e-6, q_out=None, k_out=None, v_out=None, stream=None):
+        """Biases, head norms, RoPE and the cache write of the step's rows q [rows, Hq * d], k and v
+        [rows, Hkv * d] in `layer` (luc_kv4_append); q_out (default: q itself) gets q."""
+        b = self.blocks
+        self.lib.kv4_append(q, k, v, rope.cos, rope.sin, b.positions, b.slots, self.k_pool, self.v_pool, layer,
+                            self.num_layers, self.num_q_heads, self.num_kv_heads, self.head_dim, q_norm, k_norm,
+                            eps, q_bias, k_bias, v_bias, q_out, k_out, v_out, stream=stream)
+
+    def workspace(self, total_rows, max_rows, max_ctx, stream=None):
+        """The zero-filled workspace of `attend`, grown on demand (None: none needed).  Ask for it
+        before a capture that needs a larger one than there is."""
+        need = self.lib.lib.luc_kv4_workspace_size(self.blocks.max_seqs, total_rows, max_rows, max_ctx,
+                                                   self.num_q_heads, self.num_kv_heads, self.head_dim)
+        if need == 0:
+            return None
+        if not self._workspaces or self._workspaces[-1].numel() * 4 < need:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"Kv4Cache: a workspace of {need} bytes must be made before the capture")
+            with torch.cuda.stream(stream):  # (None: the current one) filled in the launch's order
+                self._workspaces.append(torch.zeros(need // 4, dtype=torch.float32, device=self.k_pool.device))
+        return self._workspaces[-1]
+
+    def attend(self, layer, out, q, max_ctx, max_rows=None, scale=None, stream=None):
+        """Attention of the step's rows (luc_kv4_attention): q and out [rows, Hq * d]; max_ctx and max_rows
+        (default: all of q's rows) bound a sequence's context, its new rows among it, and its new
+        rows; scale defaults to 1 / sqrt(d)."""
+        b = self.blocks
+        rows = q.shape[0]
+        max_rows = rows if max_rows is None else max_rows
+        self.lib.kv4_attention(out, q, self.k_pool, self.v_pool, b.block_tables, b.start_pos, b.max_seqs, rows,
+                               max_rows, max_ctx, layer, self.num_layers, self.num_q_heads, self.num_kv_heads,
+                               self.head_dim, sm_scale(self.head_dim) if scale is None else scale,
+                               cu_seqlens=b.cu_seqlens, workspace=self.workspace(rows, max_rows, max_ctx, stream),
+                               stream=stream)
+
+
 def apply_rope(rope, qkv, q_start_idx, k_start_idx, q_bias, k_bias, pos_ptr, head_dim,
                num_q_heads, num_k_heads, lib=None, stream=None):
     """q/k bias + RoPE in place on views of qkv (flat) at the position held in
@@ -288,6 +419,6 @@ def ceil_div(a, b):
     return -(-a // b)
 
 
-__all__ = ["RopeCache", "KVCache", "apply_rope", "apply_flash_decoding", "decode_step",
-           "decode_step_unfused",
+__all__ = ["RopeCache", "KVCache", "DeviceBlocks", "Kv4Cache", "apply_rope", "apply_flash_decoding",
+           "decode_step", "decode_step_unfused",
            "sm_scale", "BLOCK_SIZE"]

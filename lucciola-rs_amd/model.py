@@ -23,6 +23,8 @@ then h = rmsnorm(h, norm) (models.rs:755-761, 814-820), logits = h @ lm_head^T
 sampling by luc_argmax (models.rs:385-405).
 The q/k biases enter in the RoPE step and the v bias in the cache write, as in
 the reference (models.rs:505-534).
+With kv_bits=4 the cache is a Kv4Cache (0.31 of the bytes): att is then
+luc_kv4_append and luc_kv4_attention, of prompts and single tokens alike.
 
 Weights are bf16 in the reference's fused layout (models.rs:91-155):
 qkv_proj = [q; k; v] rows, qkv_bias likewise (zeros when the checkpoint has
@@ -38,7 +40,7 @@ import numpy as np
 import torch
 
 from . import library
-from .engine import KVCache, RopeCache, sm_scale
+from .engine import KVCache, Kv4Cache, RopeCache, ceil_div, sm_scale
 
 
 @dataclass(frozen=True)
@@ -143,11 +145,15 @@ class Qwen2Model:
     reference's [out, in] layout ("*_w"); those of a prompt are the MFMA products
     of luc_prompt_gemm and luc_prompt_mlp on the same weights, or, where
     prompt_kernels_win says so, hipBLASLt GEMMs on their transposes ("*_t": views,
-    or contiguous copies where hidden or intermediate is not a multiple of 64)."""
+    or contiguous copies where hidden or intermediate is not a multiple of 64).
+    kv_bits: 16, the reference's bf16 cache, or 4."""
 
     def __init__(self, cfg: Qwen2Config, weights: dict, num_blocks: int | None = None,
-                 max_positions: int | None = None, device="cuda", lib=None):
+                 max_positions: int | None = None, device="cuda", lib=None, kv_bits: int = 16):
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits {kv_bits} (4 or 16)")
         self.cfg = cfg
+        self.kv_bits = kv_bits
         self.lib = lib if lib is not None else library.default(torch.cuda.current_device())
         self.device = torch.device(device)
         d = cfg.head_dim
@@ -187,8 +193,14 @@ class Qwen2Model:
         self.rope = RopeCache(max_pos, d, cfg.rope_theta, cfg.rope_scaling_factor, device=self.device,
                               lib=self.lib)
         blocks = num_blocks or (max_pos + 15) // 16
-        self.kv = KVCache(cfg.num_hidden_layers, cfg.num_key_value_heads, d, blocks, max_pos,
-                          dtype=torch.bfloat16, device=self.device, lib=self.lib)
+        if kv_bits == 4:
+            self.kv = Kv4Cache(cfg.num_hidden_layers, cfg.num_attention_heads, cfg.num_key_value_heads, d,
+                               blocks, 1, max_pos, max_pos, self.device, self.lib)
+            self._count = torch.zeros(1, dtype=torch.int32, device=self.device)
+            self._one = torch.ones(1, dtype=torch.int32, device=self.device)
+        else:
+            self.kv = KVCache(cfg.num_hidden_layers, cfg.num_key_value_heads, d, blocks, max_pos,
+                              dtype=torch.bfloat16, device=self.device, lib=self.lib)
         self.pos = torch.zeros(1, dtype=torch.int32, device=self.device)
         self.hidden = torch.zeros(1, cfg.hidden_size, dtype=torch.bfloat16, device=self.device)
         self.idx = torch.zeros(1, dtype=torch.int32, device=self.device)
@@ -224,6 +236,30 @@ class Qwen2Model:
                                self.kv.block_table.view(1, -1), cu, start, S, cache_pos + S, li,
                                cfg.num_hidden_layers, cfg.num_attention_heads,
                                cfg.num_key_value_heads, cfg.head_dim, sm_scale(cfg.head_dim), att)
+        return att
+
+    def _extend4(self, cache_pos, rows):
+        """Pages, slots and positions of `rows` new tokens at cache_pos.. of the 4-bit cache, which
+        forgets what it held from there on."""
+        held = int(self.kv.blocks.lens.item())  # (replays of capture_decode's graph change it too)
+        if cache_pos > held:
+            raise ValueError(f"position {cache_pos} past the {held} tokens of the 4-bit cache")
+        if ceil_div(cache_pos + rows, self.kv.block_size) > self.kv.blocks.num_blocks:
+            raise RuntimeError("KVCache: Out of memory blocks")
+        if cache_pos < held:
+            self._count.fill_(cache_pos)
+            self.kv.truncate(self._count)
+        self._count.fill_(rows)
+        self.kv.extend(self._count, rows)
+
+    def _attention4(self, li, qkv, max_ctx):
+        cfg = self.cfg
+        L = self.layers[li]
+        H, kd = cfg.hidden_size, cfg.num_key_value_heads * cfg.head_dim
+        q, k, v = qkv[:, :H], qkv[:, H:H + kd], qkv[:, H + kd:]
+        self.kv.append(li, q, k, v, self.rope, L["q_bias"], L["k_bias"], L["v_bias"])
+        att = torch.empty(qkv.shape[0], H, dtype=torch.bfloat16, device=self.device)
+        self.kv.attend(li, att, q, max_ctx)
         return att
 
     def _layer(self, li, h, attention, out=None):
@@ -294,6 +330,10 @@ class Qwen2Model:
         ids = torch.tensor([int(i) for i in input_ids], dtype=torch.int32, device=self.device)
         h = torch.empty(S, cfg.hidden_size, dtype=torch.bfloat16, device=self.device)
         self.lib.embedding(h, self.embed, ids)
+        if self.kv_bits == 4:
+            self._extend4(cache_pos, S)
+            self._decoder(h, lambda li, qkv: self._attention4(li, qkv, cache_pos + S))
+            return
         # the pages of every position first, and of those before it that no step
         # has reserved (prepare_for_step appends one page a call, whatever the gap)
         reserved = len(self.kv.block_table_cpu) * self.kv.block_size
@@ -306,6 +346,12 @@ class Qwen2Model:
             cu = torch.tensor([0, S], dtype=torch.int32, device=self.device)
             start = torch.tensor([cache_pos], dtype=torch.int32, device=self.device)
             attention = lambda li, qkv: self._attention_prefill(li, qkv, cache_pos, cu, start)  # noqa: E731
+        self._decoder(h, attention)
+
+    def _decoder(self, h, attention):
+        """Every layer on the rows h; the last row's hidden state to self.hidden."""
+        cfg = self.cfg
+        S = h.shape[0]
         n = cfg.num_hidden_layers
         if S > 1 and prompt_kernels_win(cfg, S):
             self._prompt_layers(h, attention)
@@ -348,15 +394,24 @@ class Qwen2Model:
         its pages are taken now, the split-K workspace is sized for it, and the
         attention launches are bounded by it (the kernels read the actual
         position from self.pos).  Set self.idx and self.pos before the first
-        replay."""
+        replay.  With a 4-bit cache a replay itself takes the page that its token
+        opens, and goes back to self.pos first where the cache holds more tokens;
+        self.pos must not be past those."""
         cfg = self.cfg
         if max_ctx > self.max_positions:
             raise ValueError(f"max_ctx {max_ctx} exceeds {self.max_positions} positions")
-        for p in range(max_ctx):
-            self.kv.prepare_for_step(p)
-        ws = self.kv.workspace(cfg.num_attention_heads, max_ctx)
+        if self.kv_bits == 4:
+            if ceil_div(max_ctx, self.kv.block_size) > self.kv.blocks.num_blocks:
+                raise RuntimeError("KVCache: Out of memory blocks")
+            self.kv.workspace(1, 1, max_ctx)
+        else:
+            for p in range(max_ctx):
+                self.kv.prepare_for_step(p)
+            ws = self.kv.workspace(cfg.num_attention_heads, max_ctx)
 
         def attention(li, qkv):
+            if self.kv_bits == 4:
+                return self._attention4(li, qkv, max_ctx)
             L = self.layers[li]
             att = torch.empty(1, cfg.hidden_size, dtype=torch.bfloat16, device=self.device)
             self.lib.decode_step(qkv, L["q_bias"], L["k_bias"], L["v_bias"], self.rope.cos,
@@ -371,6 +426,9 @@ class Qwen2Model:
         with torch.cuda.graph(graph):
             h = torch.empty(1, cfg.hidden_size, dtype=torch.bfloat16, device=self.device)
             self.lib.embedding(h, self.embed, self.idx)
+            if self.kv_bits == 4:
+                self.kv.truncate(self.pos)
+                self.kv.extend(self._one, 1)
             for li in range(cfg.num_hidden_layers - 1):
                 h = self._layer(li, h, attention)
             self._layer(cfg.num_hidden_layers - 1, h, attention, out=self.hidden)

@@ -48,7 +48,7 @@ class Maps:
 def encode(x):
     """x float32 array [..., d] of 16-bit values: (n uint8 [..., d], s, m fp16 [..., d / 32])."""
     with np.errstate(invalid="ignore", over="ignore"):
-        g = np.clip(x.reshape(*x.shape[:-1], -1, GROUP).astype(np.float32), np.float32(-LIMIT), np.float32(LIMIT))
+        g = np.clip(x.reshape(*x.shape[:-1], x.shape[-1] // GROUP, GROUP).astype(np.float32), np.float32(-LIMIT), np.float32(LIMIT))
         nan = np.isnan(g).any(-1)
         m = g.min(-1).astype(np.float16)
         s = np.maximum((g.max(-1) - m.astype(np.float32)) / np.float32(15), np.float32(0)).astype(np.float16)
@@ -62,7 +62,7 @@ def encode(x):
 
 def values(n, s, m):
     """float64 values of n [..., d] with s, m [..., d / 32]."""
-    g = n.reshape(*n.shape[:-1], -1, GROUP).astype(np.float64)
+    g = n.reshape(*n.shape[:-1], n.shape[-1] // GROUP, GROUP).astype(np.float64)
     return (g * s.astype(np.float64)[..., None] + m.astype(np.float64)[..., None]).reshape(n.shape)
 
 
@@ -102,7 +102,7 @@ def pack_pool(x, is_v):
     else:
         sm = np.stack([s, m], -1)
     sm = np.ascontiguousarray(sm).view(np.uint8)
-    pool = np.concatenate([by.reshape(*lead, -1), sm.reshape(*lead, -1)], -1)
+    pool = np.concatenate([by.reshape(*lead, 8 * d), sm.reshape(*lead, 2 * d)], -1)
     return pool, values(n, s, m)
 
 

@@ -190,3 +190,39 @@ def test_kernels_keep_their_values_in_registers():
         assert kernels
         for kernel, spilled, scratch in kernels:
             assert (spilled, scratch) == (0, 0), kernel
+
+
+def test_engine_refusals():
+    """DeviceBlocks and Kv4Cache say what they were given wrongly before any launch."""
+    import torch
+    from lucciola_rs_amd.engine import DeviceBlocks, Kv4Cache
+    from lucciola_rs_amd.library import LucError
+
+    calls = []
+
+    class Lib:
+        def block_extend(self, *a, **kw):
+            calls.append(a)
+
+    for sizes in ((0, 1, 1, 1), (4, 0, 1, 1), (4, 1, 0, 1), (4, 1, 1, 0)):
+        with pytest.raises(ValueError, match="must be positive"):
+            DeviceBlocks(*sizes, device="cpu", lib=Lib())
+    blocks = DeviceBlocks(4, 2, 3, 10, device="cpu", lib=Lib())
+    assert blocks.free_list.tolist() == [3, 2, 1, 0] and blocks.num_free == 4
+    new = torch.zeros(2, dtype=torch.int32)
+    for rows in (-1, 11):
+        with pytest.raises(ValueError, match="outside"):
+            blocks.extend(new, rows=rows)
+    assert not calls
+    blocks.extend(new, rows=0)
+    blocks.extend(new)
+    assert [a[5].numel() for a in calls] == [0, 10]
+    blocks.check()
+    for status, code, text in ((1, -6, "pages"), (2, -1, "table row"), (5, -1, "out of range"), (8, -1, "rows")):
+        blocks.state[1] = status
+        with pytest.raises(LucError, match=text) as e:
+            blocks.check()
+        assert e.value.code == code
+        blocks.check()
+    with pytest.raises(LucError, match="head dimension"):
+        Kv4Cache(1, 4, 2, 96, 4, 1, 64, device="cpu", lib=Lib())
