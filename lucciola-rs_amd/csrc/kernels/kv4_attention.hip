@@ -949,6 +949,7 @@ template <int DT, int D> struct Kv4Expand {
 template <int DT, int D> struct Kv4Chunk {
   static constexpr bool EXACT = DT == kF16;
   static constexpr int F = Kv4Cols<D>::F, KS = D / 32, NF = D / 16, H = D / 64;
+  static constexpr bool AHEAD = !EXACT || D == 128;  // V is read before the softmax, where registers allow
   uint4 q[F][KS], qsum[EXACT ? F : 1];
   f32x4_t acc[F][NF], l[F];
   float m[F], scale[F], bar[F];
@@ -1077,11 +1078,15 @@ template <int DT, int D> struct Kv4Chunk {
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[f][4 * b + i] = t[f][i];
     }
-    __builtin_amdgcn_sched_barrier(0);
     uint4 vv[NF];
+    if constexpr (AHEAD) {
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < NF; ++i) vv[i] = T.v[half][i][lane];
-    __builtin_amdgcn_sched_barrier(0);
+      for (int i = 0; i < NF; ++i) vv[i] = T.v[half][i][lane];
+      __builtin_amdgcn_sched_barrier(0);
+    } else {
+      asm volatile("" ::: "memory");  // (no read of V moves up)
+    }
     if (edge) {
 #pragma unroll
       for (int f = 0; f < F; ++f) {
@@ -1136,6 +1141,10 @@ template <int DT, int D> struct Kv4Chunk {
     for (int f = 0; f < F; ++f) {
       l[f] = mfma16(ones, p[f], l[f]);
       if constexpr (EXACT) l[f] = mfma16(ones, p2[f], l[f]);
+    }
+    if constexpr (!AHEAD) {
+#pragma unroll
+      for (int i = 0; i < NF; ++i) vv[i] = T.v[half][i][lane];
     }
 #pragma unroll
     for (int i = 0; i < NF; ++i)
@@ -1344,7 +1353,7 @@ __device__ void kv4_merge_impl(const Kv4AttnArgs& A) {
   extern "C" __global__ __launch_bounds__(256, 2) void luc_kv4_tokens_##DTN##_d##D(luc::Kv4AttnArgs a) {  \
     luc::kv4_tokens_impl<luc::DT, D>(a);                                                         \
   }                                                                                              \
-  extern "C" __global__ __launch_bounds__(64 * luc::Kv4Cols<D>::WAVES, D == 128 || luc::DT == luc::kF16 ? 2 : 3) void luc_kv4_columns_##DTN##_d##D(luc::Kv4AttnArgs a) { \
+  extern "C" __global__ __launch_bounds__(64 * luc::Kv4Cols<D>::WAVES, D == 128 ? 2 : 3) void luc_kv4_columns_##DTN##_d##D(luc::Kv4AttnArgs a) { \
     luc::kv4_columns_impl<luc::DT, D>(a);                                                        \
   }                                                                                              \
   extern "C" __global__ __launch_bounds__(256) void luc_kv4_merge_##DTN##_d##D(luc::Kv4AttnArgs a) {      \
