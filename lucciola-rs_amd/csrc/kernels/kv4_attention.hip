@@ -560,6 +560,17 @@ __device__ inline bool kv4_longest_first(const Kv4AttnArgs& A, Kv4Seq& S, int& s
 }
 
 // ---- waves split tokens: one workgroup per (split, sequence, kv head, 8-column tile) ----
+//
+// What bounds it, us a launch:
+//   64 sequences of 1024..16384, 28 and 4 heads of 128: 87.4 for 383 MB, 4.4 TB/s of the 5.2 that a large copy
+//     reaches; the stream alone takes 74, the rest is products that do not hide behind it
+//   8 of 32768, 12 and 2 of 128: 26.2 for 81 MB: stream 14, products 5, the waves' merge 1.4, partials and
+//     their arrival 2.4, the merge of 32 splits 3.7
+//   32 of 128..4096, 14 and 2 of 64: 12.7 for 13 MB; one of 512: 6.7: the chain of lengths, pages, stages and
+//     arrivals, not bytes
+// Tried: equal runs of stages over all units (104..119 at the first; the prologue of every run), eight
+// waves a workgroup (24.8 at the second, slower elsewhere), a ring of three at less occupancy (103),
+// V in fp16 before the product (equal, less exact), K and V in rings of their own (100).
 template <int DT, int D>
 __device__ void kv4_tokens_impl(const Kv4AttnArgs& A) {
   constexpr int NW = kTokWaves, NT = 64 * NW, R = kTokRing;
@@ -811,7 +822,20 @@ __device__ void kv4_tokens_impl(const Kv4AttnArgs& A) {
 // The waves expand a tile of 64 tokens together into LDS in operand order (a lane's 16 bytes
 // of every operand side by side: reads without conflicts), one tile ahead of the products and with
 // the loads of another under way; one barrier a tile.  A k step of a score is a group of 32
-// dimensions.
+// dimensions.  A wave has 32 columns; all of K's and V's reads of 32 tokens are under way before the products and
+// the softmax that need them.
+//
+// What bounds it: issue.  A product of 16 x 16 x 32 keeps a SIMD's VALU from issuing for about 8 of its
+// 16 cycles, and 32 tokens of 16 columns take (128 dimensions, bf16) 17 products and some 60 VALU
+// instructions: the softmax's 34, the column's share of the expansion, masks and loop.
+//   16 prompts of 1531..2048, 14 and 2 heads of 64, bf16: 141 us, 650 TFLOP/s; fp16: 208 (28 products and 32
+//     more FMAs: EXACT); 12 and 2 of 128, bf16: 224 us, 700 TFLOP/s
+//   4 of them: 47.4, the longest columns' chain of 32 tiles at the end
+//   512 rows after 8000, 12 and 2 of 128: fp16 65.7 with 7.6 in the merge of ten splits; bf16 45
+// Tried at the last three (bf16, bf16, bf16): 16 waves of one fragment 71.6, -, 54.9; 4 waves of four
+// fragments at 64 dimensions 65; 8 waves of one fragment there 52.8; reads of LDS as they are
+// needed 48.3, 77, 47; a raised wave priority around the products no gain; expansion by every
+// wave for itself 105, -, 91 (fp16).
 //   bf16 rows: K and V are n s + m in fp16, one rounding of 2^-12, far below the output's 2^-9.
 //   fp16 rows (EXACT): that rounding of K and P's own would each add an error as large as the output's.
 //     K is n, and a group's products are scaled by s in 32 bits; the group's sum of q times m, q's sums
