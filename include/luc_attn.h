@@ -394,7 +394,8 @@ int luc_sort_and_sample(luc_ctx* ctx, void* stream, int dtype, const void* logit
  * sequence no rows (cu_seqlens 0, slots and positions -1) and sets bits of the
  * status, which stays until the caller clears it: 1 free pages are short, 2 a
  * table row is, 4 a length, count or the state is out of range, 8 rows is too
- * small.  batch <= 4096 (else LUC_E_UNSUPPORTED), table_stride <= 2^26.  Calls
+ * small.  batch <= 4096 (else LUC_E_UNSUPPORTED; 0 writes nothing),
+ * table_stride <= 2^26.  Calls
  * on one free list must not overlap (one stream, in order). */
 int luc_block_extend(luc_ctx* ctx, void* stream, int batch, const int32_t* new_tokens, int32_t* lens,
                      int32_t* block_tables, int table_stride, int32_t* free_list, int32_t* state,

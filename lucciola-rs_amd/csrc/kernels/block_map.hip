@@ -156,7 +156,7 @@ __device__ void extend_impl(const MapArgs& A) {
   // sums of rejected lengths mean nothing: only the lengths' own bits are told
   if (verdict & (kMapBadLength | kMapTableFull)) verdict &= kMapBadLength | kMapTableFull;
   if (verdict) {
-    for (int r = blockIdx.x * kMapThreads + t; r < A.rows; r += gridDim.x * kMapThreads) {
+    for (uint32_t r = blockIdx.x * kMapThreads + t; r < (uint32_t)A.rows; r += gridDim.x * kMapThreads) {
       A.slots[r] = -1;
       A.positions[r] = -1;
     }
@@ -194,8 +194,10 @@ __device__ void extend_impl(const MapArgs& A) {
     if (blockIdx.x == 0 && t == 0) A.cu_seqlens[0] = 0;
   }
   __syncthreads();
+  // (32 unsigned bits: the last step may pass 2^31)
   const int total = (int)S.all_a;
-  for (int r = blockIdx.x * kMapThreads + t; r < A.rows; r += gridDim.x * kMapThreads) {
+  for (uint32_t x = blockIdx.x * kMapThreads + t; x < (uint32_t)A.rows; x += gridDim.x * kMapThreads) {
+    const int r = (int)x;
     int64_t slot = -1;
     int pos = -1;
     if (r < total) {
@@ -265,7 +267,8 @@ __device__ void truncate_impl(const MapArgs& A) {
   }
   __syncthreads();
   const int all = (int)S.all_a;
-  for (int e = blockIdx.x * kMapThreads + t; e < all; e += gridDim.x * kMapThreads) {
+  for (uint32_t x = blockIdx.x * kMapThreads + t; x < (uint32_t)all; x += gridDim.x * kMapThreads) {
+    const int e = (int)x;
     const int i = map_find(s_gone, A.batch, e);
     int32_t* const entry = A.tables + i * A.table_stride + s_left[i] + (e - s_gone[i]);
     // entry e of the pages in table order is the (all - 1 - e)-th to go back

@@ -1,5 +1,5 @@
 // luc_kv4.cpp -- host side of the page maps on the GPU, the normed appends and the
-// 4-bit cache (include/luc_attn.h, "Serving over a 4-bit cache"): argument checks, work
+// 4-bit cache (include/luc_attn.h, "Serving over a paged cache held on the GPU"): argument checks, work
 // splits and launches of block_map.hip, norm_append.hip and kv4_attention.hip.  Nothing here
 // allocates device memory or synchronises.
 #include "luc_internal.h"
@@ -15,6 +15,8 @@ const char* dt_name(int dtype) { return dtype == LUC_F16 ? "f16" : "bf16"; }
 constexpr int kGroup4 = 32;             // values of a 4-bit group (kernels/kv4.h)
 constexpr int kMaxMapBatch = 4096;      // block_map.hip: kMaxSeqs
 constexpr int kMaxTableStride = 1 << 26;  // positions stay below 2^30
+
+constexpr int kMaxHeads = 1 << 20;        // rows of heads stay within 32 bits
 
 int64_t align256(int64_t n) { return ceil_div(n, 256) * 256; }
 
@@ -80,6 +82,7 @@ int check_sizes(const luc_ctx* ctx, int dtype, int hq, int hkv, int head_dim, in
   if (head_dim != 64 && head_dim != 128)
     return fail(LUC_E_UNSUPPORTED, "unsupported head_dim %d (64 or 128)", head_dim);
   if (hq <= 0 || hkv <= 0) return fail(LUC_E_INVALID, "head counts must be positive");
+  if (hq > kMaxHeads) return fail(LUC_E_INVALID, "num_q_heads %d above %d", hq, kMaxHeads);
   if (hq % hkv) return fail(LUC_E_INVALID, "num_q_heads %d not a multiple of num_kv_heads %d", hq, hkv);
   if (hq / hkv > 8) return fail(LUC_E_UNSUPPORTED, "group size %d > 8", hq / hkv);
   if (block_size != LUC_BLOCK_SIZE)
@@ -313,7 +316,8 @@ int luc_kv4_append(luc_ctx* ctx, void* stream, int dtype, const void* q, const v
 size_t luc_kv4_workspace_size(int batch, int total_rows, int max_rows, int max_ctx, int num_q_heads,
                               int num_kv_heads, int head_dim) {
   if (batch <= 0 || total_rows <= 0 || max_rows <= 0 || max_ctx <= 0 || max_ctx > kMaxCtx || num_q_heads <= 0 ||
-      num_kv_heads <= 0 || num_q_heads % num_kv_heads || num_q_heads / num_kv_heads > 8 ||
+      num_kv_heads <= 0 || num_q_heads > kMaxHeads || num_q_heads % num_kv_heads ||
+      num_q_heads / num_kv_heads > 8 || (int64_t)total_rows * num_q_heads > INT32_MAX ||
       (head_dim != 64 && head_dim != 128))
     return 0;
   const int group = num_q_heads / num_kv_heads;
@@ -354,12 +358,12 @@ int luc_kv4_attention(luc_ctx* ctx, void* stream, int dtype, void* out, int64_t 
     return fail(LUC_E_WORKSPACE, "workspace %zu bytes, %zu needed", workspace_bytes, need);
   if (need && !aligned(workspace, 256)) return fail(LUC_E_INVALID, "workspace must be 256-byte aligned");
   const int64_t units = (int64_t)batch * num_kv_heads * plan.tiles;
-  if (plan.tokens && plan.splits > 1 && units > kMaxArrivals)
-    return fail(LUC_E_UNSUPPORTED, "split attention of %lld (sequence, kv head) units above %lld", (long long)units,
-                (long long)kMaxArrivals);
   if ((int64_t)num_layers * num_kv_heads * 10 * head_dim > UINT32_MAX)
     return fail(LUC_E_INVALID, "num_layers x num_kv_heads too large");
-  if (units * plan.splits * 256 > UINT32_MAX) return fail(LUC_E_INVALID, "batch x kv heads x rows too large");
+  const int64_t threads = !plan.tokens && head_dim == 128 ? 512 : 256;
+  const int64_t items = (int64_t)total_rows * num_q_heads;  // of the merge, head_dim / 4 threads each
+  if (units * plan.splits * threads > UINT32_MAX || (!plan.tokens && plan.splits > 1 && items * (head_dim / 4) > UINT32_MAX))
+    return fail(LUC_E_INVALID, "batch x kv heads x rows too large");
   if (int rc = check_device(ctx)) return rc;
   Kv4AttnArgs a{q, q_row_stride, out, out_row_stride, k_pool, v_pool, block_tables, table_stride, cu_seqlens,
                 start_pos, nullptr, nullptr, nullptr, batch, total_rows, max_rows, max_ctx, layer, num_layers,
@@ -377,9 +381,8 @@ int luc_kv4_attention(luc_ctx* ctx, void* stream, int dtype, void* out, int64_t 
   if (int rc = get_fn(ctx, (plan.tokens ? "luc_kv4_tokens_" : "luc_kv4_columns_") + suffix, &fn)) return rc;
   if (int rc = get_fn(ctx, "luc_kv4_merge_" + suffix, &merge)) return rc;
   void* args[] = {&a};
-  if (int rc = launch(fn, dim3((unsigned)(units * plan.splits)), dim3(!plan.tokens && head_dim == 128 ? 512 : 256), stream, args)) return rc;
+  if (int rc = launch(fn, dim3((unsigned)(units * plan.splits)), dim3((unsigned)threads), stream, args)) return rc;
   if (plan.tokens || plan.splits == 1) return LUC_OK;
-  const int64_t items = (int64_t)total_rows * num_q_heads;
   return launch(merge, dim3((unsigned)ceil_div(items, 1024 / head_dim)), dim3(256), stream, args);
 }
 

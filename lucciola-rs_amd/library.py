@@ -383,11 +383,11 @@ class LucAttn:
     # than its checks on the host otherwise would)
     @staticmethod
     def _array(name, t, dtype, dev, least):
-        """An operand read as a flat array: contiguous, of `dtype`, on device `dev`, of at least
-        `least` elements."""
+        """An operand read as a flat array: contiguous, of `dtype`, on device `dev` (the library's), of
+        at least `least` elements."""
         if t.dtype is not dtype or t.get_device() != dev or t.numel() < least or not t.is_contiguous():
             raise ValueError(f"{name} {tuple(t.shape)} {t.dtype} on {t.device}: want contiguous {dtype} of at "
-                             f"least {least} elements on the call's device")
+                             f"least {least} elements on the library's device")
         return t.data_ptr()
 
     @staticmethod
@@ -396,7 +396,7 @@ class LucAttn:
         `width` consecutive elements."""
         shape, strides = t.shape, t.stride()
         if t.dtype is not dtype or t.get_device() != dev:
-            raise TypeError(f"{name} is {t.dtype} on {t.device}: want {dtype} on the call's device")
+            raise TypeError(f"{name} is {t.dtype} on {t.device}: want {dtype} on the library's device")
         if len(shape) == 2 and shape[1] == width and strides[1] == 1 or \
                 len(shape) == 3 and shape[1] * shape[2] == width and strides[1:] == (head_dim, 1) and shape[2] == head_dim:
             return shape[0], strides[0]
@@ -409,7 +409,7 @@ class LucAttn:
         slots int64 and positions int32 of one length, the most rows of the batch; the others
         int32 [B], cu_seqlens [B + 1]."""
         batch, stride = tables.shape
-        i32, rows, dev, arr = torch.int32, slots.numel(), tables.get_device(), self._array
+        i32, rows, dev, arr = torch.int32, slots.numel(), self.device, self._array
         blocks = free_list.numel()
         self._check(self.lib.luc_block_extend(
             self.ctx, _stream(stream), batch, arr("new_tokens", new_tokens, i32, dev, batch),
@@ -422,7 +422,7 @@ class LucAttn:
         """luc_block_truncate: sequence b back to at most keep[b] tokens, its pages behind those
         to the free list."""
         batch, stride = tables.shape
-        i32, dev, arr = torch.int32, tables.get_device(), self._array
+        i32, dev, arr = torch.int32, self.device, self._array
         self._check(self.lib.luc_block_truncate(
             self.ctx, _stream(stream), batch, arr("keep", keep, i32, dev, batch),
             arr("lens", lens, i32, dev, batch), arr("tables", tables, i32, dev, 0), stride,
@@ -431,7 +431,7 @@ class LucAttn:
     def _append_args(self, q, k, v, cos, sin, positions, slots, hq, hkv, head_dim, q_norm, k_norm, eps,
                      q_bias, k_bias, v_bias, q_out, stream):
         """The arguments that both appends share, from ctx to q_out_stride, and (rows, dtype, device)."""
-        dtype, dev, arr, f32 = q.dtype, q.get_device(), self._array, torch.float32
+        dtype, dev, arr, f32 = q.dtype, self.device, self._array, torch.float32
         qw, kw = hq * head_dim, hkv * head_dim
         rows, stride = own = self._rows("q", q, qw, head_dim, dtype, dev)
         if rows and (self._rows("k", k, kw, head_dim, dtype, dev) != own or
@@ -531,7 +531,7 @@ class LucAttn:
                       workspace=None, block_size=16, stream=None, num_blocks=None):
         """luc_kv4_attention: out and q [rows, hq * d]; start_pos int32 [batch]; cu_seqlens int32
         [batch + 1], or None for one row a sequence; workspace from kv4_workspace."""
-        dtype, dev, arr, i32 = q.dtype, q.get_device(), self._array, torch.int32
+        dtype, dev, arr, i32 = q.dtype, self.device, self._array, torch.int32
         rows, q_stride = self._rows("q", q, hq * head_dim, head_dim, dtype, dev)
         o_rows, o_stride = self._rows("out", out, hq * head_dim, head_dim, dtype, dev)
         if rows < total_rows or o_rows < total_rows:

@@ -115,6 +115,7 @@ def test_attention_refusals(cdll):
     assert c(out_stride=13 * 64) == -1 and c(out_stride=14 * 64 + 2) == -1
     assert c(q=P(72)) == -1 and c(out=P(68)) == -1 and c(k_pool=P(72)) == -1 and c(v_pool=P(72)) == -1
     assert c(rows=1 << 28) == -1                           # rows x heads past 2^31
+    assert c(hq=1 << 21, hkv=1 << 20, q_stride=1 << 40, out_stride=1 << 40, rows=3, cu=None) == -1
     assert c(batch=0) == 0 and c(rows=0) == 0
     big = dict(stride=4096, max_ctx=65536)
     need = cdll.luc_kv4_workspace_size(3, 9, 4, 65536, 14, 2, 64)
@@ -131,7 +132,8 @@ def test_sizes(cdll):
     assert ws(1, 1, 1, 16, 14, 2, 64) == 0                 # one split
     for bad in ((0, 1, 1, 16, 14, 2, 64), (1, 0, 1, 16, 14, 2, 64), (1, 1, 0, 16, 14, 2, 64), (1, 1, 1, 0, 14, 2, 64),
                 (1, 1, 1, 9999, 15, 2, 64), (1, 1, 1, 9999, 18, 2, 64), (1, 1, 1, 9999, 14, 2, 96),
-                (1, 1, 1, (1 << 30) + 1, 14, 2, 64)):
+                (1, 1, 1, (1 << 30) + 1, 14, 2, 64), (1, 1 << 28, 1, 4096, 14, 2, 64), (9, 9, 1, 4096, 1 << 24, 1 << 24, 64),
+                ((1 << 31) - 1, (1 << 31) - 1, (1 << 31) - 1, 1 << 30, 8, 1, 64)):
         assert ws(*bad) == 0
     # the largest call's workspace: a few partials a CU, not one a page
     assert ws(64, 64, 1, 1 << 20, 28, 4, 128) < 1 << 28
@@ -141,7 +143,7 @@ def test_sizes(cdll):
 def test_binding_refusals():
     """Shapes, types and strides that the binding checks before a call (tensors on the CPU)."""
     lib = object.__new__(library.LucAttn)
-    lib.lib, lib.ctx, lib.device = library.load_cdll(), ctypes.c_void_p(), 0
+    lib.lib, lib.ctx, lib.device = library.load_cdll(), ctypes.c_void_p(), -1  # (what a CPU tensor's device is)
     stream = types.SimpleNamespace(cuda_stream=0)
     i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
     i64 = lambda *s: torch.zeros(s, dtype=torch.int64)  # noqa: E731
@@ -182,6 +184,11 @@ def test_binding_refusals():
             lib.kv4_attention(**(att | kw))
     with pytest.raises(library.LucError, match="null context"):
         lib.kv4_attention(**att)
+    lib.device = 0  # tensors of another device than the library's
+    for call in (lambda: lib.block_extend(**ext), lambda: lib.block_truncate(i32(2), i32(2), i32(2, 4), i32(8), i32(4), stream=stream),
+                 lambda: lib.kv4_append(**base), lambda: lib.kv4_attention(**att)):
+        with pytest.raises((TypeError, ValueError), match="library's device"):
+            call()
 
 
 def test_kernels_keep_their_values_in_registers():
