@@ -834,8 +834,9 @@ __device__ void kv4_tokens_impl(const Kv4AttnArgs& A) {
 //   512 rows after 8000, 12 and 2 of 128: fp16 65.7 with 7.6 in the merge of ten splits; bf16 45
 // Tried at the last three (bf16, bf16, bf16): 16 waves of one fragment 71.6, -, 54.9; 4 waves of four
 // fragments at 64 dimensions 65; 8 waves of one fragment there 52.8; reads of LDS as they are
-// needed 48.3, 77, 47; a raised wave priority around the products no gain; expansion by every
-// wave for itself 105, -, 91 (fp16).
+// needed 48.3, 77, 47; products of 32 x 32 x 16 with one chain, two, or both halves at once 50.0..52.7,
+// 69.8..74.7, 48.2..52.0 (two to seven in a hundred less for fp16); a raised wave priority around the products
+// no gain; expansion by every wave for itself 105, -, 91 (fp16).
 //   bf16 rows: K and V are n s + m in fp16, one rounding of 2^-12, far below the output's 2^-9.
 //   fp16 rows (EXACT): that rounding of K and P's own would each add an error as large as the output's.
 //     K is n, and a group's products are scaled by s in 32 bits; the group's sum of q times m, q's sums
@@ -1295,7 +1296,8 @@ __device__ void kv4_columns_impl(const Kv4AttnArgs& A) {
       const int64_t at = ((int64_t)split * A.total_rows + S.row0 + col / A.group) * hq + kvh * A.group + col % A.group;
       *(float2*)(A.ws_ml + at * 2) = make_float2(W.m[f], W.l[f][0]);
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (lanes read what others wrote)
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) {
       const int c = (64 / (D / 4)) * i + W.lane / (D / 4), part = W.lane % (D / 4);
@@ -1312,7 +1314,8 @@ __device__ void kv4_columns_impl(const Kv4AttnArgs& A) {
         *(float4*)(A.ws_o + (((int64_t)split * A.total_rows + row) * hq + head) * D + 4 * part) = x;
       }
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
