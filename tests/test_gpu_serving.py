@@ -277,6 +277,60 @@ def test_maps_and_normed_appends_over_a_16_bit_cache(luc, hq, hkv, d, dtype):
         ref.check(out[s:s + 1].view(1, hq, d), want, tol, dt, f"sequence {s} of {ctx[s]}")
 
 
+@pytest.mark.parametrize("rows", [[1, 1, 1], [40, 3, 65]])
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (12, 2, 128)])
+def test_sequences_that_share_pages(luc, hq, hkv, d, rows):
+    """A prefix's pages in several tables, as prefix caching leaves them: the same as copies of them."""
+    ctx = [700, 300, 1000]
+    c = Cache(ctx, hkv, d, seed=9)
+    shared = 15                                        # pages of sequence 0 in the other tables too
+    for b in (1, 2):
+        c.tables[b, :shared] = c.tables[0, :shared]
+        c.k[b][:shared * PAGE], c.v[b][:shared * PAGE] = c.k[0][:shared * PAGE], c.v[0][:shared * PAGE]
+    c.dev_tables = torch.from_numpy(c.tables).cuda()
+    q, out, scale = run(luc, c, rows, hq, "f16")
+    verify(c, rows, hq, "f16", q, out, scale)
+
+
+def test_two_streams_at_once(luc):
+    """Steps of two caches on two streams that overlap, with a workspace each: the bits of the same
+    steps in turn."""
+    hq, hkv, d, steps = 14, 2, 64, 12
+    rope = RopeCache(3000, d, lib=luc)
+    width = (hq + 2 * hkv) * d
+
+    def prepare(seed):
+        gen = torch.Generator().manual_seed(seed)
+        cache = Kv4Cache(1, hq, hkv, d, 400, 2, 3000, 2700, lib=luc)
+        rnd = lambda n: (torch.randn(n, width, generator=gen) * 1.4).half().cuda()  # noqa: E731
+        work = [(i32([1500 + 100 * seed, 900]), rnd(2400 + 100 * seed), 1700)] + [(i32([1, 1]), rnd(2), 1) for _ in range(steps)]
+        cache.workspace(2, 1, 3000)
+        cache.workspace(2400 + 100 * seed, 1700, 3000)
+        return cache, work, [torch.zeros(w.shape[0], hq * d, dtype=torch.float16, device="cuda") for _, w, _ in work]
+
+    def issue(cache, work, outs, i, stream):
+        new, qkv, most = work[i]
+        cache.extend(new, rows=qkv.shape[0], stream=stream)
+        q, k, v = qkv[:, :hq * d], qkv[:, hq * d:(hq + hkv) * d], qkv[:, (hq + hkv) * d:]
+        cache.append(0, q, k, v, rope, stream=stream)
+        cache.attend(0, outs[i], q, 3000, most, stream=stream)
+
+    results = []
+    for together in (False, True):
+        sets = [prepare(seed) for seed in (1, 2)]
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in sets] if together else [None, None]
+        for i in range(steps + 1):
+            for (cache, work, outs), stream in zip(sets, streams):
+                issue(cache, work, outs, i, stream)
+        torch.cuda.synchronize()
+        for cache, _, _ in sets:
+            cache.blocks.check()
+        results.append([o for _, _, outs in sets for o in outs])
+    for a, b in zip(*results):
+        assert torch.equal(a, b) and bool(a.isfinite().all())
+
+
 # ---- the model ------------------------------------------------------------------------------
 
 CFG = Qwen2Config(vocab_size=512, hidden_size=256, num_hidden_layers=3, num_attention_heads=4, num_key_value_heads=2,
