@@ -217,7 +217,7 @@ template <> struct Kv4Reads<128> {
   __device__ __attribute__((always_inline)) inline void read_v(uint32_t v_at, uint32_t vs_at, uint32_t vm_at, int) {
     asm volatile(
         "ds_read_b128 %0, %9 offset:2048\n\tds_read_b128 %1, %9 offset:2560\n\t"
-        "ds_read_b128 %2, %9 offset:3072\n\tds_read_b128 %3, %9 offset:3584\n\t"
+        "ds_read_b128 %2, %9 offset:2048+1024\n\tds_read_b128 %3, %9 offset:3584\n\t"
         "ds_read_b64 %4, %10 offset:4608\n\tds_read_b64 %5, %10 offset:4672\n\t"
         "ds_read_b64 %6, %10 offset:4736\n\tds_read_b64 %7, %10 offset:4800\n\t"
         "ds_read_b128 %8, %11 offset:4864\n\t"
