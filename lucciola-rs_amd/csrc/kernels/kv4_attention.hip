@@ -834,9 +834,9 @@ __device__ void kv4_tokens_impl(const Kv4AttnArgs& A) {
 //   512 rows after 8000, 12 and 2 of 128: fp16 65.7 with 7.6 in the merge of ten splits; bf16 45
 // Tried at the last three (bf16, bf16, bf16): 16 waves of one fragment 71.6, -, 54.9; 4 waves of four
 // fragments at 64 dimensions 65; 8 waves of one fragment there 52.8; reads of LDS as they are
-// needed 48.3, 77, 47; products of 32 x 32 x 16 with one chain, two, or both halves at once 50.0..52.7,
-// 69.8..74.7, 48.2..52.0 (two to seven in a hundred less for fp16); a raised wave priority around the products
-// no gain; expansion by every wave for itself 105, -, 91 (fp16).
+// needed 48.3, 77, 47; products of 32 x 32 x 16 in three forms 50.0..52.7, 69.8..74.7, 48.2..52.0, and with the
+// softmax between the products of the next 32 tokens 52.5, 70, 48; a raised wave priority around the
+// products no gain; expansion by every wave for itself 105, -, 91 (fp16).
 //   bf16 rows: K and V are n s + m in fp16, one rounding of 2^-12, far below the output's 2^-9.
 //   fp16 rows (EXACT): that rounding of K and P's own would each add an error as large as the output's.
 //     K is n, and a group's products are scaled by s in 32 bits; the group's sum of q times m, q's sums
