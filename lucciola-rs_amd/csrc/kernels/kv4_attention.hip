@@ -832,11 +832,12 @@ __device__ void kv4_tokens_impl(const Kv4AttnArgs& A) {
 //     more FMAs: EXACT); 12 and 2 of 128, bf16: 224 us, 700 TFLOP/s
 //   4 of them: 47.4, the longest columns' chain of 32 tiles at the end
 //   512 rows after 8000, 12 and 2 of 128: fp16 65.7 with 7.6 in the merge of ten splits; bf16 45
-// Tried at the last three (bf16, bf16, bf16): 16 waves of one fragment 71.6, -, 54.9; 4 waves of four
-// fragments at 64 dimensions 65; 8 waves of one fragment there 52.8; reads of LDS as they are
-// needed 48.3, 77, 47; products of 32 x 32 x 16 in three forms 50.0..52.7, 69.8..74.7, 48.2..52.0, and with the
-// softmax between the products of the next 32 tokens 52.5, 70, 48; a raised wave priority around the
-// products no gain; expansion by every wave for itself 105, -, 91 (fp16).
+// Tried, us for bf16 rows of 4 such prompts at 64 dimensions, at 128, and the 512 rows (47.6, 68, 45.6 as it
+// is): 16 waves of one fragment (two at 64) 71.6, 70, 47.2; 4 waves of four fragments at 64 65; 8 of one
+// there 52.8; reads of LDS as they are needed 48.3, 77, 47; products of 32 x 32 x 16 in three forms
+// 50.0..52.7, 69.8..74.7, 48.2..52.0, and with the softmax between the products of the next 32
+// tokens 52.5, 70, 48; a raised wave priority around the products no gain; expansion by every wave for
+// itself 105 at the first.
 //   bf16 rows: K and V are n s + m in fp16, one rounding of 2^-12, far below the output's 2^-9.
 //   fp16 rows (EXACT): that rounding of K and P's own would each add an error as large as the output's.
 //     K is n, and a group's products are scaled by s in 32 bits; the group's sum of q times m, q's sums
