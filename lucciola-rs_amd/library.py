@@ -393,13 +393,13 @@ class LucAttn:
     @staticmethod
     def _rows(name, t, width, head_dim, dtype, dev):
         """(rows, row stride) of an operand [rows, width] or [rows, heads, head_dim] whose rows are
-        `width` consecutive elements."""
+        `width` consecutive elements.  One row has no stride: 2^30 stands for any."""
         shape, strides = t.shape, t.stride()
         if t.dtype is not dtype or t.get_device() != dev:
             raise TypeError(f"{name} is {t.dtype} on {t.device}: want {dtype} on the library's device")
         if len(shape) == 2 and shape[1] == width and strides[1] == 1 or \
                 len(shape) == 3 and shape[1] * shape[2] == width and strides[1:] == (head_dim, 1) and shape[2] == head_dim:
-            return shape[0], strides[0]
+            return shape[0], strides[0] if shape[0] > 1 else 1 << 30
         raise ValueError(f"{name} {tuple(shape)} with strides {strides}: want rows of {width} consecutive elements")
 
     def block_extend(self, new_tokens, lens, tables, free_list, state, slots, positions, cu_seqlens,
@@ -519,7 +519,8 @@ class LucAttn:
             o_stride or 0, kp, vp, pages, layer, num_layers, hq, hkv, head_dim, block_size))
 
     def kv4_workspace(self, batch, total_rows, max_rows, max_ctx, hq, hkv, head_dim, device=None):
-        """A zero-filled workspace for kv4_attention calls of these sizes (None: none needed)."""
+        """A workspace for kv4_attention calls of these sizes, zero-filled on the current stream (None: none
+        needed)."""
         need = self.lib.luc_kv4_workspace_size(batch, total_rows, max_rows, max_ctx, hq, hkv, head_dim)
         if need == 0:
             return None

@@ -266,3 +266,19 @@ def test_another_stream_and_a_captured_append(luc):
         graph.replay()
         kp2, vp2 = other.run(luc, True, q0)
         assert torch.equal(q0, q1) and torch.equal(kp2, kp1) and torch.equal(vp2, vp1)
+
+
+@pytest.mark.parametrize("four", [False, True])
+def test_one_row_of_tensors_of_their_own(luc, four):
+    """A single token's q, k and v in three tensors: the row of a shared qkv tensor."""
+    c = Case(1, 14, 2, 64, "f16", True, True)
+    want = torch.empty(1, 14 * 64, dtype=c.dt, device="cuda")
+    pools = c.pools(four)
+    c.run(luc, four, q_out=want, pools=pools)
+    q, k, v = (x.clone() for x in c.views())
+    got, again = torch.empty_like(want), c.pools(four)
+    call = luc.kv4_append if four else luc.qk_norm_rope_append
+    call(q, k, v, c.cos, c.sin, c.pos, c.slots, *again, 1, c.layers, 14, 2, 64, q_out=got, **c.kw())
+    assert torch.equal(got, want)
+    for a, b in zip(pools, again):
+        assert torch.equal(a, b)

@@ -176,6 +176,13 @@ def test_binding_refusals():
         lib.qk_norm_rope_append(**(base | dict(k_pool=torch.zeros(2, 1, 2, 16, 64), v_pool=half(2, 1, 2, 16, 64))))
     with pytest.raises(library.LucError, match="null context"):  # what is right reaches the library
         lib.kv4_append(**base)
+    # one row from tensors of its own, or with any stride
+    one = dict(q=half(1, 256), k=half(1, 128), v=half(1, 131)[:, :128], positions=i32(1), slots=i64(1), k_out=half(1, 128),
+               v_out=half(1, 140)[:, :128])
+    with pytest.raises(library.LucError, match="null context"):
+        lib.kv4_append(**(base | one))
+    with pytest.raises(ValueError, match="stride differ"):
+        lib.kv4_append(**(base | dict(k=half(3, 128))))
     att = dict(out=half(3, 256), q=q, k_pool=pool4, v_pool=pool4, tables=i32(3, 2), start_pos=i32(3), batch=3,
                total_rows=3, max_rows=1, max_ctx=32, layer=0, num_layers=1, hq=4, hkv=2, head_dim=64, sm_scale=0.125, stream=stream)
     for kw in (dict(out=half(2, 256)), dict(out=torch.zeros(3, 256)), dict(q=half(3, 128)), dict(tables=i32(2, 2)),
