@@ -50,8 +50,14 @@ struct Kv4AttnArgs {
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 // The running maximum moves when a score (in powers of two) passes it by this: weights are at most
-// 8, and 8 s below fp16's limit for every s of the format (8000 at most).
+// 8 times what the largest had when it moved.
 constexpr float kKv4Lazy = 3.0f;
+// tokens: weights are held times 2^lift, so that neither those of a long tail nor their products with a
+// small step of V get lost below fp16's smallest, 2^-24.  A product is below 2^(12 - lift) 2^(3 + lift) = 2^15
+// for steps below 2^(12 - lift), and below 2^16 whatever the rounding of large scores adds: a column that meets a
+// longer step lowers its lift (-1 holds every s of the format, 8000 at most).
+constexpr int kKv4Lift = 12, kKv4LeastLift = -1;
+__device__ inline uint32_t kv4_steps(int lift) { return (uint32_t)(27 - lift) << 10; }  // fp16 bits of 2^(12 - lift)
 
 __device__ inline f32x4_t mfma16(uint4 a, uint4 b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
@@ -127,6 +133,15 @@ __device__ inline void ws_put(float* p, float x) {
 }
 __device__ inline float ws_get(const float* p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Of the two halves of a dword.
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+__device__ inline uint32_t max_u16(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
+}
+__device__ inline uint32_t sub_sat_u16(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
 }
 
 __device__ inline int pick2(bool c, int a, int b) {
@@ -274,9 +289,10 @@ template <int DT, int D> struct Kv4Row {
   // O^T: [group][c], rows 4 g + i of it are dimensions 16 (g % 2) + 4 i + 2 (g / 2) + c of the group, in
   // units of 2^-20; and the m term, whose rows are groups
   f32x4_t acc[NG][2], acc_m;
-  float m, l, scale;
+  float m, l, scale;  // m: less the column's lift
   float bar;       // products above it move m
   int limit;
+  int lift;        // of the column, see kKv4Lift
   int lane, n, g;
   uint32_t mask[2];  // of the pairs of fragment a's and b's tokens in P: the lane's or 0
   uint32_t kw_at, sm_at, am_at, v_at, vs_at, vm_at;  // LDS offsets of the lane's reads in a stage
@@ -345,6 +361,7 @@ template <int DT, int D> struct Kv4Row {
     const _Float16 hi = (_Float16)mine;
     const half2_t parts = {hi, (_Float16)(mine - (float)hi)};
     qsum = as_u(parts);
+    lift = kKv4Lift;
     m = -3.4028235e38f;
     bar = -INFINITY;
     l = 0.0f;
@@ -390,7 +407,7 @@ template <int DT, int D> struct Kv4Row {
     if (__any(top > bar)) {
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
-      const float mn = fmaxf(m, top * scale);
+      const float mn = fmaxf(m, fmaf(top, scale, -(float)lift));
       const float a = __builtin_amdgcn_exp2f(m - mn);
       bar = fmaxf(bar, top + kKv4Lazy / scale);
       m = mn;
@@ -418,11 +435,6 @@ template <int DT, int D> struct Kv4Row {
         l = __builtin_amdgcn_fdot2(h, (half2_t){(_Float16)1.0f, (_Float16)1.0f}, l, false);
       }
     }
-    uint32_t p[4] = {ph[0] & mask[0], ph[1] & mask[0], ph[0] & mask[1], ph[1] & mask[1]};
-    uint32_t p2[4];
-    if constexpr (HILO) {
-      p2[0] = pl[0] & mask[0]; p2[1] = pl[1] & mask[0]; p2[2] = pl[0] & mask[1]; p2[3] = pl[1] & mask[1];
-    }
     // ---- output: the weights times s are the operand of each group's n, as fp16 subnormals, and the
     // weights that of m
     R.read_v(lds + v_at, lds + vs_at, lds + vm_at, u);
@@ -445,6 +457,18 @@ template <int DT, int D> struct Kv4Row {
         const uint32_t nan = ((R.vm[i] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
         R.vm[i] &= live & ~((nan >> 15) * 0xffffu);
       }
+    }
+    uint32_t longest = R.vs[0][0];  // of the steps that the column sees, two fp16
+#pragma unroll
+    for (int j = 0; j < NG; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) longest = max_u16(longest, R.vs[j][i]);
+    const uint32_t most = kv4_steps(lift) - 1;
+    if (__any(sub_sat_u16(longest, most | most << 16))) lower(R, ph, pl);
+    uint32_t p[4] = {ph[0] & mask[0], ph[1] & mask[0], ph[0] & mask[1], ph[1] & mask[1]};
+    uint32_t p2[4];
+    if constexpr (HILO) {
+      p2[0] = pl[0] & mask[0]; p2[1] = pl[1] & mask[0]; p2[2] = pl[0] & mask[1]; p2[3] = pl[1] & mask[1];
     }
     const uint32_t groups = n < NG ? ~0u : 0u;
     const uint4 vm = make_uint4(R.vm[0] & groups, R.vm[1] & groups, R.vm[2] & groups, R.vm[3] & groups);
@@ -477,6 +501,36 @@ template <int DT, int D> struct Kv4Row {
       const uint4 b2 = make_uint4(w2[0], w2[1], w2[2], w2[3]);
       acc[j][0] = mfma16(x0, b2, acc[j][0]);
       acc[j][1] = mfma16(x1, b2, acc[j][1]);
+    }
+  }
+
+  // The column's lift down to what V's steps of its tokens allow, and with it what it has summed and the weights at
+  // hand.  (Steps that are NaN say nothing of the other groups.)
+  __device__ __attribute__((always_inline)) inline void lower(const Kv4Reads<D>& R, uint32_t (&ph)[2], uint32_t (&pl)[2]) {
+    uint32_t longest = 0;
+#pragma unroll
+    for (int j = 0; j < NG; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) longest = max_u16(longest, R.vs[j][i] & ~((kv4_nan(R.vs[j][i], 0) >> 15) * 0xffffu));
+    uint32_t s = max(longest & 0xffffu, longest >> 16);
+    s = max(s, (uint32_t)__shfl_xor((int)s, 16));
+    s = max(s, (uint32_t)__shfl_xor((int)s, 32));
+    const int down = max(lift - max(26 - (int)(s >> 10), kKv4LeastLift), 0);
+    lift -= down;
+    m += (float)down;
+    const float a = __uint_as_float((uint32_t)(127 - down) << 23);
+    l *= a;
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      acc[j][0] *= a;
+      acc[j][1] *= a;
+    }
+    acc_m *= a;
+    const half2_t a2 = {(_Float16)a, (_Float16)a};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      ph[i] = as_u(as_h2(ph[i]) * a2);
+      if constexpr (HILO) pl[i] = as_u(as_h2(pl[i]) * a2);
     }
   }
 

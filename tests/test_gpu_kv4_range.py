@@ -1,0 +1,166 @@
+"""luc_kv4_attention where K, V and the softmax's weights leave the size of a standard normal: V of small and of
+mixed sizes, long contexts whose weight is one token's but for a tail, many splits; with bounds without terms
+that grow with the context where the kernels' arithmetic has none."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import serving_ref as ref
+from test_gpu_kv4_attention import DT, PAGE, Cache, run
+
+pytestmark = pytest.mark.gpu
+GROUP = ref.GROUP
+
+
+def cache_of(ks, vs, seed=0):
+    """A Cache of sequences with the values ks[b], vs[b] (float32 [ctx, hkv, d]); every other byte 0xff."""
+    rng = np.random.default_rng(seed)
+    c = object.__new__(Cache)
+    c.ctx = [len(x) for x in ks]
+    c.hkv, c.d = ks[0].shape[1:]
+    c.layers, c.layer = 1, 0
+    pages = [-(-n // PAGE) for n in c.ctx]
+    c.pages = sum(pages) + 2
+    perm = rng.permutation(c.pages).astype(np.int32)
+    c.tables = np.full((len(ks), max(pages)), -7, np.int32)
+    kp = np.full((c.pages, 1, c.hkv, 10 * c.d), 0xFF, np.uint8)
+    vp = kp.copy()
+    c.k, c.v = [], []
+    at = 0
+    for b, n in enumerate(pages):
+        ids = perm[at:at + n]
+        at += n
+        c.tables[b, :n] = ids
+        for pool, given, is_v, keep in ((kp, ks[b], False, c.k), (vp, vs[b], True, c.v)):
+            x = np.full((n * PAGE, c.hkv, c.d), np.nan, np.float32)
+            x[:c.ctx[b]] = given
+            slabs, val = ref.pack_pool(np.ascontiguousarray(x.reshape(n, PAGE, c.hkv, c.d).swapaxes(1, 2)), is_v)
+            pool[ids, 0] = slabs
+            keep.append(torch.from_numpy(np.ascontiguousarray(val.swapaxes(1, 2)).reshape(-1, c.hkv, c.d)[:c.ctx[b]]).cuda())
+    c.kp, c.vp = torch.from_numpy(kp).cuda(), torch.from_numpy(vp).cuda()
+    c.dev_tables = torch.from_numpy(c.tables).cuda()
+    return c
+
+
+def bound(q, k, v, start, scale, dtype, few):
+    """(out, tolerance without the output's own rounding) of rows q [n, hq, d], all in float64; few: the call has so
+    few columns that waves split tokens.
+
+    Weights are held times 2^lift: 12 for few columns, less where V has steps of 1 and more (a weight times a step
+    stays below 2^15), and 7 for many.  Of the output:
+      sums: f32 sums and products in 16 and 32 steps, each of them relative to the sizes |n s| + |m| of its terms:
+        fewer than 64 roundings of 2^-24, and the matrix unit's alignment of subnormals (6 bits), 2^-17 in all
+      scores: the same of scale sum |q| (|n s| + |m|), 2^-18 in powers of e; few columns also take the sum of a group's
+        q in two fp16 parts, the second a multiple of 2^-24 where q's largest is 2^-10: half of that, so 2^-15 of q's
+        largest times |m| a group
+      weights, few columns: bf16 rows have them truncated to fp16 (as has their sum): uniform in 2^-10 of
+        themselves.  fp16 rows have two parts.  Either loses up to 2^-24 / 2^lift of the largest, and the product with
+        a step two roundings of 2^-25 / 2^lift, times n <= 15
+      many columns: V is rounded to fp16, half a step of 2^-11; bf16 rows' K and weights too.  Below 2^-14 weights
+        are multiples of 2^-24 / 2^lift
+    What is rounded independently for each token is summed as the root of the squares, six times that."""
+    n, hq, d = q.shape
+    ctx, hkv = k.shape[:2]
+    g = hq // hkv
+    out = torch.empty((n, hq, d), dtype=torch.float64, device=q.device)
+    tol = torch.empty_like(out)
+    at = torch.arange(ctx, device=q.device)
+
+    def groups(x):
+        x = x.unflatten(-1, (-1, GROUP))
+        return x, x.amin(-1, keepdim=True), x.amax(-1, keepdim=True)
+
+    half, many = 2.0 ** -11, 6 / math.sqrt(3)
+    for h in range(hkv):
+        (kx, km, _), (vx, vm, vtop) = groups(k[:, h]), groups(v[:, h])
+        k_size, v_size = ((x - m + m.abs()).flatten(-2) for x, m in ((kx, km), (vx, vm)))
+        step = float((vtop - vm).max()) / 15
+        lift = min(12, max(-1, 11 - math.floor(math.log2(max(step, 1e-9))))) if few else 7
+        floor = 2.0 ** -lift
+        for j in range(h * g, h * g + g):
+            for r in range(n):
+                x, seen = q[r, j], start + r + 1
+                kk, vv = k[:seen, h], v[:seen, h]
+                p = torch.softmax(kk @ x * scale, 0)
+                o = p @ vv
+                away = (vv - o).abs()
+                e = abs(scale) * 2.0 ** -18 * (k_size[:seen] @ x.abs()) + 2.0 ** -21
+                w2 = torch.zeros_like(p)
+                t = 2.0 ** -17 * (p @ v_size[:seen])
+                most = p.max() * seen
+                if few:
+                    e = e + abs(scale) * 2.0 ** -15 * x.abs().max() * km[:seen].abs().sum((1, 2))
+                    if dtype == "bf16":
+                        w2 = w2 + 2.0 ** -20 / 12
+                    t = t + most * floor * (2.0 ** -24 * vv.abs().max() + 15 * 2.0 ** -24)
+                else:
+                    t = t + many * half * torch.sqrt((p * p) @ (vv * vv))
+                    if dtype == "bf16":
+                        w2 = w2 + ((kk * kk) @ (x * x) * (scale * half) ** 2 + half ** 2) / 3
+                    t = t + many * p.max() * math.sqrt(seen) * 2.0 ** -25 * floor * vv.abs().max()
+                t = t + (p * e) @ away + 6 * torch.sqrt((p * p * w2) @ (away * away))
+                out[r, j], tol[r, j] = o, t
+    return out, tol
+
+
+def verify(c, rows, hq, dtype, q, out, scale, few, pick=None):
+    r0 = 0
+    for b, n in enumerate(rows):
+        which = list(range(n)) if pick is None else sorted({x % n for x in pick})
+        for r in which:
+            row = slice(r0 + r, r0 + r + 1)
+            want, tol = bound(q[row].double().view(1, hq, c.d), c.k[b], c.v[b], c.ctx[b] - n + r, scale, dtype, few)
+            ref.check(out[row].view(1, hq, c.d), want, tol, DT[dtype], f"sequence {b}, row {r} of {n} at {c.ctx[b]}")
+        r0 += n
+
+
+def normal(rng, ctx, hkv, d, std):
+    return rng.standard_normal((ctx, hkv, d), dtype=np.float32) * np.float32(std)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 60])
+@pytest.mark.parametrize("dtype,v_std", [("f16", 1e-2), ("f16", 1e-3), ("f16", 1e-4), ("bf16", 1e-3), ("bf16", 1e-5),
+                                         ("f16", 1.0), ("bf16", 40.0), ("f16", 1000.0)])
+@pytest.mark.parametrize("hq,hkv,d", [(10, 2, 64), (5, 1, 128)])
+def test_sizes_of_v(luc, hq, hkv, d, dtype, v_std, rows):
+    rng = np.random.default_rng(rows)
+    ctx = [300, 1100]
+    c = cache_of([normal(rng, n, hkv, d, 1.4) for n in ctx], [normal(rng, n, hkv, d, v_std) for n in ctx])
+    q, out, scale = run(luc, c, [rows, rows], hq, dtype)
+    verify(c, [rows, rows], hq, dtype, q, out, scale, rows < 10, pick=(0, 1, -1))
+
+
+@pytest.mark.parametrize("rows", [1, 2, 40])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_sizes_of_v_along_a_context(luc, d, dtype, rows):
+    """V of 0.01 at first, then of 1, 30 and 2000, then of 0.01 again; and in the other order."""
+    rng = np.random.default_rng(d)
+    sizes = np.repeat(np.float32([0.01, 1.0, 30.0, 2000.0, 0.01]), [130, 200, 37, 16, 217])[:, None, None]
+    ks = [normal(rng, 600, 2, d, 1.4) for _ in range(2)]
+    vs = [normal(rng, 600, 2, d, 1.0) * s for s in (sizes, sizes[::-1])]
+    c = cache_of(ks, vs)
+    q, out, scale = run(luc, c, [rows, rows], 6, dtype)
+    verify(c, [rows, rows], 6, dtype, q, out, scale, rows < 10, pick=(0, -1))
+
+
+@pytest.mark.parametrize("rows", [1])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("ctx,v_mean,v_std", [(30000, 1.0, 0.2), (30, 1000.0, 0.5)])
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (5, 1, 128)])
+def test_one_token_and_a_tail(luc, hq, hkv, d, ctx, v_mean, v_std, dtype, rows):
+    """Position 0 has nearly all the weight and V = 0; the others have 2^-25.5 of it each, and the output is theirs."""
+    rng = np.random.default_rng(d)
+    rows = min(rows, ctx - 5)
+    k, v = normal(rng, ctx, hkv, d, 0.05), normal(rng, ctx, hkv, d, v_std) + np.float32(v_mean)
+    scale = d ** -0.5
+    k[0] = 25.5 * math.log(2) / (scale * d)   # q is near 1 throughout
+    v[0] = 0
+    c = cache_of([k], [v])
+    gen = torch.Generator().manual_seed(2)
+    q = (1 + 0.02 * torch.randn(rows, hq * d, generator=gen)).to(DT[dtype]).cuda()
+    q, out, scale = run(luc, c, [rows], hq, dtype, q=q, scale=scale)
+    assert 2e-4 < float(out.double().mean()) < 2e-3
+    verify(c, [rows], hq, dtype, q, out, scale, rows < 10, pick=(0, 1, -1))
