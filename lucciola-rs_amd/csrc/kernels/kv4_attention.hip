@@ -59,6 +59,10 @@ constexpr float kKv4Lazy = 3.0f;
 constexpr int kKv4Lift = 12, kKv4LeastLift = -1;
 __device__ inline uint32_t kv4_steps(int lift) { return (uint32_t)(27 - lift) << 10; }  // fp16 bits of 2^(12 - lift)
 
+// columns: weights, at most 2^kLazyMax of that, are held times this power of two, 2^15 at most.  (V is
+// multiplied in the matrix unit.)
+constexpr float kKv4ColsLift = 15.0f - kLazyMax;
+
 __device__ inline f32x4_t mfma16(uint4 a, uint4 b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
                                                 __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -1032,7 +1036,7 @@ template <int DT, int D> struct Kv4Chunk {
   static constexpr bool AHEAD = !EXACT || D == 128;  // V is read before the softmax, where registers allow
   uint4 q[F][KS], qsum[EXACT ? F : 1];
   f32x4_t acc[F][NF], l[F];
-  float m[F], scale[F], bar[F];
+  float m[F], scale[F], bar[F];  // m: less kKv4ColsLift
   int limit[F];  // last position that the lane's column sees
   int lane, n, g;
 
@@ -1187,7 +1191,7 @@ template <int DT, int D> struct Kv4Chunk {
       for (int f = 0; f < F; ++f) {
         float t = fmaxf(top[f], __shfl_xor(top[f], 16));
         t = fmaxf(t, __shfl_xor(t, 32));
-        const float mn = fmaxf(m[f], t * scale[f]);
+        const float mn = fmaxf(m[f], fmaf(t, scale[f], -kKv4ColsLift));
         const float a = __builtin_amdgcn_exp2f(m[f] - mn);
         bar[f] = fmaxf(bar[f], t + kLazyMax / scale[f]);
         m[f] = mn;

@@ -146,7 +146,7 @@ def test_sizes_of_v_along_a_context(luc, d, dtype, rows):
     verify(c, [rows, rows], 6, dtype, q, out, scale, rows < 10, pick=(0, -1))
 
 
-@pytest.mark.parametrize("rows", [1])
+@pytest.mark.parametrize("rows", [1, 40])
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("ctx,v_mean,v_std", [(30000, 1.0, 0.2), (30, 1000.0, 0.5)])
 @pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (5, 1, 128)])
