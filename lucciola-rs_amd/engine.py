@@ -311,7 +311,8 @@ class Kv4Cache:
         shape = (num_physical_blocks, num_layers, num_kv_heads, 10 * head_dim)
         self.k_pool = torch.zeros(shape, dtype=torch.uint8, device=device)
         self.v_pool = torch.zeros(shape, dtype=torch.uint8, device=device)
-        self._workspaces = []  # the largest last; a captured graph may hold an earlier one
+        self._workspace = None
+        self._captured = []  # workspaces that captured graphs hold
 
     def extend(self, new_tokens, rows=None, stream=None):
         self.blocks.extend(new_tokens, rows, stream)
@@ -328,19 +329,35 @@ class Kv4Cache:
                             self.num_layers, self.num_q_heads, self.num_kv_heads, self.head_dim, q_norm, k_norm,
                             eps, q_bias, k_bias, v_bias, q_out, k_out, v_out, stream=stream)
 
+    @staticmethod
+    def _capturing(stream):
+        if stream is None:
+            return torch.cuda.is_current_stream_capturing()
+        with torch.cuda.stream(stream):
+            return torch.cuda.is_current_stream_capturing()
+
     def workspace(self, total_rows, max_rows, max_ctx, stream=None):
-        """The zero-filled workspace of `attend`, grown on demand (None: none needed).  Ask for it
-        before a capture that needs a larger one than there is."""
+        """The zero-filled workspace of `attend`, grown on demand by half at least (None: none needed).  Ask
+        for it before a capture that needs a larger one than there is.  A smaller one that it takes the
+        place of is freed, unless it was handed out during a capture (by `attend`; a program that captures
+        launches of its own on one holds it itself)."""
         need = self.lib.lib.luc_kv4_workspace_size(self.blocks.max_seqs, total_rows, max_rows, max_ctx,
                                                    self.num_q_heads, self.num_kv_heads, self.head_dim)
         if need == 0:
             return None
-        if not self._workspaces or self._workspaces[-1].numel() * 4 < need:
-            if torch.cuda.is_current_stream_capturing():
+        capturing = self._capturing(stream)
+        old = self._workspace
+        if old is None or old.numel() * 4 < need:
+            if capturing:
                 raise RuntimeError(f"Kv4Cache: a workspace of {need} bytes must be made before the capture")
+            size = need // 4 if old is None else max(need // 4, old.numel() * 3 // 2)
             with torch.cuda.stream(stream):  # (None: the current one) filled in the launch's order
-                self._workspaces.append(torch.zeros(need // 4, dtype=torch.float32, device=self.k_pool.device))
-        return self._workspaces[-1]
+                self._workspace = torch.zeros(size, dtype=torch.float32, device=self.k_pool.device)
+            if old is not None:  # launches before this one may still use it
+                old.record_stream(torch.cuda.current_stream() if stream is None else stream)
+        if capturing and not any(w is self._workspace for w in self._captured):
+            self._captured.append(self._workspace)
+        return self._workspace
 
     def attend(self, layer, out, q, max_ctx, max_rows=None, scale=None, stream=None):
         """Attention of the step's rows (luc_kv4_attention): q and out [rows, Hq * d]; max_ctx and max_rows

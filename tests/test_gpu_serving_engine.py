@@ -1,0 +1,45 @@
+"""Kv4Cache over steps whose sizes change: workspaces that captured graphs hold, buffers of earlier steps."""
+import pytest
+import torch
+
+from lucciola_rs_amd.engine import Kv4Cache, RopeCache
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def rows_of(gen, n, hq, hkv, d, dt):
+    qkv = (torch.randn(n, (hq + 2 * hkv) * d, generator=gen) * 1.4).to(dt).cuda()
+    a, b = hq * d, (hq + hkv) * d
+    return qkv[:, :a], qkv[:, a:b], qkv[:, b:]
+
+
+def test_a_graph_keeps_its_workspace(luc):
+    """A captured step's splits after the cache's workspace has grown past it and its like are reused."""
+    hq, hkv, d, ctx = 12, 2, 128, 6000
+    cache = Kv4Cache(1, hq, hkv, d, 800, 1, 8000, 6000, lib=luc)
+    rope = RopeCache(8000, d, lib=luc)
+    gen = torch.Generator().manual_seed(1)
+    cache.extend(i32([ctx]), rows=ctx)
+    cache.append(0, *rows_of(gen, ctx, hq, hkv, d, torch.bfloat16), rope)
+    q = rows_of(gen, 1, hq, hkv, d, torch.bfloat16)[0].contiguous()
+    blocks = cache.blocks
+    blocks.cu_seqlens.copy_(i32([0, 1]))
+    blocks.start_pos.fill_(ctx - 1)
+    out, want = torch.zeros_like(q), torch.zeros_like(q)
+    cache.attend(0, want, q, ctx)
+    size = cache.workspace(1, 1, ctx).numel()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.attend(0, out, q, ctx)
+    assert cache.workspace(500, 500, 8000).numel() > size
+    for i in range(4):
+        junk = [torch.full((size,), float("nan"), device="cuda") for _ in range(4)]
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and all(bool(x.isnan().all()) for x in junk)
