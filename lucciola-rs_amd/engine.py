@@ -234,8 +234,9 @@ class DeviceBlocks:
     (luc_block_extend, luc_block_truncate).  A fresh one hands out pages 0, 1,
     2, ... as BlockManager does.
 
-    After `extend`, `slots` and `positions` are the step's packed new rows,
-    `cu_seqlens` and `start_pos` each sequence's rows among them.  Neither call
+    After `extend`, the first `rows` of `slots` and `positions` are the step's
+    packed new rows (behind them lies what an earlier step left: no step may
+    have more), `cu_seqlens` and `start_pos` each sequence's rows among them.  Neither call
     waits for the GPU, so neither can raise for a step that could not be met;
     such a step takes nothing and has no rows, and `check()` raises for it.
     Calls must be in one stream's order."""
@@ -256,6 +257,7 @@ class DeviceBlocks:
         self.positions = torch.full((max_rows,), -1, **kw)
         self.cu_seqlens = torch.zeros(max_seqs + 1, **kw)
         self.start_pos = torch.zeros(max_seqs, **kw)
+        self.rows = max_rows  # of the last extend
 
     def extend(self, new_tokens, rows: int | None = None, stream=None) -> None:
         """Pages, slots and positions for new_tokens (device int32 [max_seqs]) more
@@ -266,6 +268,7 @@ class DeviceBlocks:
         self.lib.block_extend(new_tokens, self.lens, self.block_tables, self.free_list, self.state,
                               self.slots[:rows], self.positions[:rows], self.cu_seqlens,
                               self.start_pos, stream=stream)
+        self.rows = rows
 
     def truncate(self, keep, stream=None) -> None:
         """Every sequence back to at most keep (device int32 [max_seqs]) tokens, the pages
@@ -323,8 +326,11 @@ class Kv4Cache:
     def append(self, layer, q, k, v, rope, q_bias=None, k_bias=None, v_bias=None, q_norm=None, k_norm=None,
                eps=1e-6, q_out=None, k_out=None, v_out=None, stream=None):
         """Biases, head norms, RoPE and the cache write of the step's rows q [rows, Hq * d], k and v
-        [rows, Hkv * d] in `layer` (luc_kv4_append); q_out (default: q itself) gets q."""
+        [rows, Hkv * d] in `layer` (luc_kv4_append); q_out (default: q itself) gets q.  At most the
+        `rows` that the step's `extend` was given."""
         b = self.blocks
+        if q.shape[0] > b.rows:
+            raise ValueError(f"{q.shape[0]} rows to append: the step has {b.rows}")
         self.lib.kv4_append(q, k, v, rope.cos, rope.sin, b.positions, b.slots, self.k_pool, self.v_pool, layer,
                             self.num_layers, self.num_q_heads, self.num_kv_heads, self.head_dim, q_norm, k_norm,
                             eps, q_bias, k_bias, v_bias, q_out, k_out, v_out, stream=stream)

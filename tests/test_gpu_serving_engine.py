@@ -43,3 +43,27 @@ def test_a_graph_keeps_its_workspace(luc):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and all(bool(x.isnan().all()) for x in junk)
+
+
+def test_a_padded_append_after_a_longer_step(luc):
+    """A step of fewer rows than the one before it: an append of more of them is refused and writes nothing; one that
+    the step has room for leaves what it has no rows for alone."""
+    hq, hkv, d = 4, 2, 64
+    cache = Kv4Cache(1, hq, hkv, d, 20, 2, 128, 100, lib=luc)
+    rope = RopeCache(128, d, lib=luc)
+    gen = torch.Generator().manual_seed(2)
+    cache.extend(i32([60, 30]), rows=90)
+    cache.append(0, *rows_of(gen, 90, hq, hkv, d, torch.float16), rope)
+    was = cache.k_pool.clone(), cache.v_pool.clone()
+    cache.extend(i32([1, 1]), rows=2)
+    with pytest.raises(ValueError, match="the step has 2"):
+        cache.append(0, *rows_of(gen, 8, hq, hkv, d, torch.float16), rope)
+    assert torch.equal(cache.k_pool, was[0]) and torch.equal(cache.v_pool, was[1])
+    cache.truncate(i32([60, 30]))
+    cache.extend(i32([1, 1]), rows=8)  # rows for a batch padded to 8
+    cache.append(0, *rows_of(gen, 8, hq, hkv, d, torch.float16), rope)
+    slots = cache.blocks.slots[:8].tolist()
+    assert slots[2:] == [-1] * 6
+    changed = (cache.k_pool != was[0]).flatten(1).any(1).nonzero().flatten().tolist()
+    assert set(changed) <= {s // 16 for s in slots[:2]}
+    cache.blocks.check()

@@ -76,3 +76,24 @@ def test_workspaces_of_captures_are_kept(capturing):
     for _ in range(3):
         assert c.workspace(1000, 1000, 32768) is last
     assert [w is x for w, x in zip(c._captured, (small(), last))] == [True, True] and len(c._captured) == 2
+
+
+def test_an_append_of_more_rows_than_the_step_has(capturing):
+    """Slots behind the last extend's rows are an earlier step's: such a row is refused."""
+    c = cache(4, 2, 64, seqs=2, max_rows=10)
+    rope = types.SimpleNamespace(cos=None, sin=None)
+    new = torch.zeros(2, dtype=torch.int32)
+    q = [torch.zeros(n, 256) for n in range(11)]
+    for rows, most in ((8, 8), (2, 2), (0, 0), (None, 10)):
+        c.extend(new, rows=rows)
+        c.lib.calls.clear()
+        for n in range(11):
+            if n > most:
+                with pytest.raises(ValueError, match=f"{n} rows to append: the step has {most}"):
+                    c.append(0, q[n], q[n], q[n], rope)
+            else:
+                c.append(0, q[n], q[n], q[n], rope)
+        assert len(c.lib.calls) == most + 1
+    with pytest.raises(ValueError, match="outside"):  # a step that is refused changes nothing
+        c.extend(new, rows=11)
+    c.append(0, q[10], q[10], q[10], rope)
