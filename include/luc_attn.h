@@ -369,7 +369,8 @@ int luc_sort_and_sample(luc_ctx* ctx, void* stream, int dtype, const void* logit
  * rows (luc_block_extend), their norms, rotation and cache write
  * (luc_qk_norm_rope_append or luc_kv4_append), their attention
  * (luc_kv4_attention over a 4-bit cache).  Every call may be captured in a HIP
- * graph. */
+ * graph.  Arrays of a length that is 0 (rows, num_tokens, total_rows, batch) may
+ * be NULL. */
 
 /* Block tables, slots and positions of a batch's new rows, from lengths kept on
  * the device -- the free list and prepare_for_step of KVCache

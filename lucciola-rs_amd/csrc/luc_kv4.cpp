@@ -43,7 +43,7 @@ int check_map(const luc_ctx* ctx, const MapArgs& a, int table_stride) {
   if (table_stride <= 0 || table_stride > kMaxTableStride)
     return fail(LUC_E_INVALID, "table_stride %d outside [1, %d]", table_stride, kMaxTableStride);
   if (a.num_blocks < 1) return fail(LUC_E_INVALID, "num_blocks %d < 1", a.num_blocks);
-  if (!a.count || !a.lens || !a.tables || !a.free_list || !a.state)
+  if ((a.batch && (!a.count || !a.lens || !a.tables)) || !a.free_list || !a.state)
     return fail(LUC_E_INVALID, "null counts, lengths, tables, free list or state");
   return LUC_OK;
 }
@@ -99,7 +99,8 @@ int norm_append(luc_ctx* ctx, void* stream, int dtype, const char* kind, NormApp
     return rc;
   if (a.rows < 0) return fail(LUC_E_INVALID, "num_tokens %d < 0", a.rows);
   if (a.max_pos < 1) return fail(LUC_E_INVALID, "max_pos %d < 1", a.max_pos);
-  if (!a.q || !a.k || !a.v || !a.q_out || !a.cos_t || !a.sin_t || !a.positions || !a.slots || !a.k_pool || !a.v_pool)
+  if ((a.rows && (!a.q || !a.k || !a.v || !a.q_out || !a.positions || !a.slots)) || !a.cos_t || !a.sin_t ||
+      !a.k_pool || !a.v_pool)
     return fail(LUC_E_INVALID, "null q, k, v, q_out, rope table, positions, slots or pool");
   if (!a.q_norm != !a.k_norm) return fail(LUC_E_INVALID, "one of q_norm and k_norm without the other");
   // (a row of q, k and v each starts 16-byte loads)
@@ -255,7 +256,7 @@ int luc_block_extend(luc_ctx* ctx, void* stream, int batch, const int32_t* new_t
             positions,  cu_seqlens, start_pos, batch,      num_blocks, rows};
   if (int rc = check_map(ctx, a, table_stride)) return rc;
   if (rows < 0) return fail(LUC_E_INVALID, "rows %d < 0", rows);
-  if (!cu_seqlens || !start_pos || (rows && (!slots || !positions)))
+  if ((batch && (!cu_seqlens || !start_pos)) || (rows && (!slots || !positions)))
     return fail(LUC_E_INVALID, "null slots, positions, cu_seqlens or start_pos");
   if (!aligned(slots, 8)) return fail(LUC_E_INVALID, "slots must be 8-byte aligned");
   if (batch == 0) return LUC_OK;
@@ -337,7 +338,7 @@ int luc_kv4_attention(luc_ctx* ctx, void* stream, int dtype, void* out, int64_t 
   if (!cu_seqlens && total_rows != batch)
     return fail(LUC_E_INVALID, "no cu_seqlens: one row a sequence, not %d for %d", total_rows, batch);
   if (max_ctx <= 0 || max_ctx > kMaxCtx) return fail(LUC_E_INVALID, "max_ctx %d outside [1, %d]", max_ctx, kMaxCtx);
-  if (!out || !q || !k_pool || !v_pool || !block_tables || !start_pos)
+  if ((total_rows && (!out || !q)) || !k_pool || !v_pool || (batch && (!block_tables || !start_pos)))
     return fail(LUC_E_INVALID, "null out, q, pool, block table or start_pos");
   const int row = num_q_heads * head_dim;
   if (q_row_stride < row || out_row_stride < row)

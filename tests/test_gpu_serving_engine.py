@@ -67,3 +67,21 @@ def test_a_padded_append_after_a_longer_step(luc):
     changed = (cache.k_pool != was[0]).flatten(1).any(1).nonzero().flatten().tolist()
     assert set(changed) <= {s // 16 for s in slots[:2]}
     cache.blocks.check()
+
+
+def test_a_step_without_rows(luc):
+    hq, hkv, d = 4, 2, 128
+    cache = Kv4Cache(1, hq, hkv, d, 20, 2, 128, 100, lib=luc)
+    rope = RopeCache(128, d, lib=luc)
+    gen = torch.Generator().manual_seed(3)
+    cache.extend(i32([40, 0]), rows=40)
+    cache.append(0, *rows_of(gen, 40, hq, hkv, d, torch.bfloat16), rope)
+    was = cache.k_pool.clone(), cache.v_pool.clone(), cache.blocks.free_list.clone()
+    cache.extend(i32([0, 0]), rows=0)
+    q, k, v = rows_of(gen, 0, hq, hkv, d, torch.bfloat16)
+    cache.append(0, q, k, v, rope)
+    cache.attend(0, torch.empty_like(q), q, 128)
+    cache.blocks.check()
+    assert cache.blocks.lens.tolist() == [40, 0] and cache.blocks.cu_seqlens.tolist() == [0, 0, 0]
+    now = cache.k_pool, cache.v_pool, cache.blocks.free_list
+    assert all(torch.equal(a, b) for a, b in zip(was, now))
