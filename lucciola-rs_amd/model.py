@@ -434,6 +434,8 @@ class Qwen2Model:
             self._layer(cfg.num_hidden_layers - 1, h, attention, out=self.hidden)
             self.lib.argmax(self.logits(), self.idx)
             self.pos.add_(1)
+        if self.kv_bits == 16:
+            graph.workspace = ws  # (the cache's own is replaced when a longer context needs more)
         return graph
 
     def generate(self, prompt_ids, max_new_tokens: int, stop_at_eos: bool = True) -> list[int]:

@@ -1,8 +1,11 @@
 """Kv4Cache over steps whose sizes change: workspaces that captured graphs hold, buffers of earlier steps."""
+import weakref
+
 import pytest
 import torch
 
 from lucciola_rs_amd.engine import Kv4Cache, RopeCache
+from lucciola_rs_amd.model import Qwen2Config, Qwen2Model, random_weights
 
 pytestmark = pytest.mark.gpu
 
@@ -85,3 +88,31 @@ def test_a_step_without_rows(luc):
     assert cache.blocks.lens.tolist() == [40, 0] and cache.blocks.cu_seqlens.tolist() == [0, 0, 0]
     now = cache.k_pool, cache.v_pool, cache.blocks.free_list
     assert all(torch.equal(a, b) for a, b in zip(was, now))
+
+
+def test_a_decode_graph_keeps_its_workspace(luc):
+    """capture_decode over the 16-bit cache: the graph's split-K workspace outlives the cache's."""
+    cfg = Qwen2Config(vocab_size=256, hidden_size=256, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2,
+                      intermediate_size=512, max_position_embeddings=4096)
+    model = Qwen2Model(cfg, random_weights(cfg, seed=6, std=0.05), lib=luc)
+    prompt = [i * 7 % 256 for i in range(900)]
+    model.forward(prompt, 0)
+    graph = model.capture_decode(max_ctx=1024)
+    ws = weakref.ref(model.kv._workspace)
+    model.kv.workspace(cfg.num_attention_heads, 4096)
+    assert ws() is not None and ws() is not model.kv._workspace
+    want = None
+    for _ in range(3):
+        model.forward(prompt, 0)
+        model.idx.fill_(5)
+        model.pos.fill_(len(prompt))
+        tokens = []
+        for _ in range(8):
+            junk = [torch.full((ws().numel(),), float("nan"), device="cuda") for _ in range(3)]
+            graph.replay()
+            tokens.append(int(model.idx))
+            assert all(bool(x.isnan().all()) for x in junk)
+        want = want or tokens
+        assert tokens == want
+    del graph
+    assert ws() is None
