@@ -164,3 +164,57 @@ def test_one_token_and_a_tail(luc, hq, hkv, d, ctx, v_mean, v_std, dtype, rows):
     q, out, scale = run(luc, c, [rows], hq, dtype, q=q, scale=scale)
     assert 2e-4 < float(out.double().mean()) < 2e-3
     verify(c, [rows], hq, dtype, q, out, scale, rows < 10, pick=(0, 1, -1))
+
+
+def splits(luc, batch, total, max_rows, max_ctx, hq, hkv, d):
+    """Splits of a call with few columns, from its workspace: [counters][(m, l), o] of 8 columns a tile."""
+    tiles = -(-min(total, max_rows) * (hq // hkv) // 8)
+    size = luc.lib.luc_kv4_workspace_size(batch, total, max_rows, max_ctx, hq, hkv, d)
+    return max(0, size - (1 << 18)) // (batch * hkv * tiles * 8 * (8 + 4 * d))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("ctx,least", [(33001, 65), (70001, 129), (131072, 256)])
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (3, 1, 128)])
+def test_one_sequence_of_many_splits(luc, hq, hkv, d, ctx, least, dtype):
+    """More than 64 and more than 128 splits, and as many as there may be, merged by one workgroup, within a
+    bound that an output without one split's 512 tokens passes."""
+    rng = np.random.default_rng(ctx)
+    assert splits(luc, 1, 1, 1, ctx, hq, hkv, d) >= least
+    v = normal(rng, ctx, hkv, d, 1.0)
+    v += np.float32(3) * np.sin(np.arange(ctx, dtype=np.float32) * 0.01)[:, None, None]  # every split's part differs
+    c = cache_of([normal(rng, ctx, hkv, d, 0.5)], [v])
+    for rows in ([1], [2]):
+        q, out, scale = run(luc, c, rows, hq, dtype)
+        verify(c, rows, hq, dtype, q, out, scale, True)
+        want, tol = bound(q[:1].double().view(1, hq, d), c.k[0], c.v[0], ctx - rows[0], scale, dtype, True)
+        half = torch.finfo(DT[dtype]).eps / 2
+        # leaving 512 tokens near the start out
+        x = q[0].double().view(hq, d)
+        for j in range(hq):
+            p = torch.softmax(c.k[0][:ctx - rows[0] + 1, j // (hq // hkv)] @ x[j] * scale, 0)
+            p[512:1024] = 0
+            less = p @ c.v[0][:len(p), j // (hq // hkv)] / p.sum()
+            far = (less - want[0, j]).abs() / (tol[0, j] + half * want[0, j].abs())
+            assert float(far.max()) > 3
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("ctx", [[1, 40], [500, 3, 1000, 77], [5000], [2049, 700]], ids=lambda c: "_".join(map(str, c)))
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (12, 2, 128), (8, 8, 64), (28, 4, 128)])
+def test_a_bound_far_above_every_context(luc, hq, hkv, d, ctx, dtype):
+    """max_ctx as a captured step has it: launches with more splits than any context, for one row a sequence and for
+    several."""
+    rng = np.random.default_rng(len(ctx))
+    c = cache_of([normal(rng, n, hkv, d, 1.4) for n in ctx], [normal(rng, n, hkv, d, 1.0) for n in ctx])
+    wide = torch.full((len(ctx), 2500), -7, dtype=torch.int32, device="cuda")
+    wide[:, :c.tables.shape[1]] = c.dev_tables
+    for rows in (1, 2, 30):
+        counts = [min(rows, n) for n in ctx]
+        need = [luc.lib.luc_kv4_workspace_size(len(ctx), sum(counts), max(counts), m, hq, hkv, d)
+                for m in (max(ctx), 40000)]
+        assert need[1] > need[0]
+        q, out, scale = run(luc, c, counts, hq, dtype, max_ctx=40000, tables=wide)
+        units = len(ctx) * hkv * -(-max(counts) * (hq // hkv) // 8)
+        cols = max(counts) * (hq // hkv)
+        verify(c, counts, hq, dtype, q, out, scale, cols <= 16 or (cols <= 48 and units <= 512), pick=(0, -1))
