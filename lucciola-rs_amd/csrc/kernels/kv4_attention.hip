@@ -722,9 +722,8 @@ __device__ void kv4_tokens_impl(const Kv4AttnArgs& A) {
   Kv4Row<DT, D> W;
   W.begin(A, S.row0, kvh, S.start, S.ctx, col0, ncols);
   for (int i = 0; i < count; ++i) {
-    const int newer = min(count - 1 - i, R - 1);
-    if (newer >= 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * Stage::LOADS) : "memory");
-    else if (newer == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(Stage::LOADS) : "memory");
+    static_assert(R == 2, "at most one stage is under way behind this one");
+    if (i + 1 < count) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(Stage::LOADS) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     const int tok0 = begin + (i * NW + w) * Stage::TOKENS;
     const uint32_t lds = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)s_ring[w][i % R];
