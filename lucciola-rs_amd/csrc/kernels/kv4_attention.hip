@@ -289,7 +289,7 @@ template <int DT, int D> struct Kv4Row {
   static constexpr bool HILO = DT == kF16;  // weights in two fp16 parts: see step()
 
   uint4 q[2][NG];  // [fragment]; group j's dimensions 8 g .. + 7 of it, pairs (i, i + 4), i odd divided by 16
-  uint32_t qsum;   // k = 8 g, 8 g + 1: the sum of group g's dimensions, high and low part
+  uint32_t qsum;   // k = 8 g, 8 g + 1: the sum of group g's dimensions times 2^-9, high and low part
   // O^T: [group][c], rows 4 g + i of it are dimensions 16 (g % 2) + 4 i + 2 (g / 2) + c of the group, in
   // units of 2^-20; and the m term, whose rows are groups
   f32x4_t acc[NG][2], acc_m;
@@ -361,7 +361,7 @@ template <int DT, int D> struct Kv4Row {
       sum += __shfl_xor(sum, 32);
       mine = g == j ? sum : mine;
     }
-    mine *= 0x1p-24f;
+    mine *= 0x1p-9f;  // (at most 2^11; times 2^-24 the low part would be mostly lost below fp16's smallest)
     const _Float16 hi = (_Float16)mine;
     const half2_t parts = {hi, (_Float16)(mine - (float)hi)};
     qsum = as_u(parts);
@@ -396,7 +396,7 @@ template <int DT, int D> struct Kv4Row {
     float s[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      s[i] = mask[0] ? x[0][i] : x[1][i];  // (not a sum: m may be NaN in the other fragment)
+      s[i] = (mask[0] ? x[0][i] : x[1][i]) * 0x1p-15f;  // (not a sum: m may be NaN in the other fragment)
 #pragma unroll
       for (int j = 0; j < NG; ++j) s[i] = fmaf((float)as_h2(R.scale(i, j)).x, c[j][i], s[i]);
     }

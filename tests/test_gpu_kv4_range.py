@@ -52,9 +52,7 @@ def bound(q, k, v, start, scale, dtype, few):
     stays below 2^15), and 7 for many.  Of the output:
       sums: f32 sums and products in 16 and 32 steps, each of them relative to the sizes |n s| + |m| of its terms:
         fewer than 64 roundings of 2^-24, and the matrix unit's alignment of subnormals (6 bits), 2^-17 in all
-      scores: the same of scale sum |q| (|n s| + |m|), 2^-18 in powers of e; few columns also take the sum of a group's
-        q in two fp16 parts, the second a multiple of 2^-24 where q's largest is 2^-10: half of that, so 2^-15 of q's
-        largest times |m| a group
+      scores: the same of scale sum |q| (|n s| + |m|), 2^-18 in powers of e
       weights, few columns: bf16 rows have them truncated to fp16 (as has their sum): uniform in 2^-10 of
         themselves.  fp16 rows have two parts.  Either loses up to 2^-24 / 2^lift of the largest, and the product with
         a step two roundings of 2^-25 / 2^lift, times n <= 15
@@ -91,7 +89,6 @@ def bound(q, k, v, start, scale, dtype, few):
                 t = 2.0 ** -17 * (p @ v_size[:seen])
                 most = p.max() * seen
                 if few:
-                    e = e + abs(scale) * 2.0 ** -15 * x.abs().max() * km[:seen].abs().sum((1, 2))
                     if dtype == "bf16":
                         w2 = w2 + 2.0 ** -20 / 12
                     t = t + most * floor * (2.0 ** -24 * vv.abs().max() + 15 * 2.0 ** -24)
@@ -218,3 +215,54 @@ def test_a_bound_far_above_every_context(luc, hq, hkv, d, ctx, dtype):
         units = len(ctx) * hkv * -(-max(counts) * (hq // hkv) // 8)
         cols = max(counts) * (hq // hkv)
         verify(c, counts, hq, dtype, q, out, scale, cols <= 16 or (cols <= 48 and units <= 512), pick=(0, -1))
+
+
+@pytest.mark.parametrize("rows", [1, 2])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (5, 1, 128)])
+def test_keys_far_from_zero(luc, hq, hkv, d, dtype, rows):
+    """A group of K at 1000 cos(t) + N(0, 1.4), which q's own group, of mean 0, takes out of the scores: few columns
+    multiply m by the sum of q, which has to be as exact as q.
+
+    q is a multiple of 2^-14 (2^-6 in bf16) below 8, so 32 of it are summed exactly.  A score's error: roundings of
+    2^-24 of sum n s q and m sum q by group, fewer than 4; and in n q, whose products the matrix unit aligns by
+    fp16's smallest exponent, 2^-23 where q's largest is in [2^14, 2^15) and n is 2^-24 n, spread evenly."""
+    ctx = [300, 1000]
+    rng = np.random.default_rng(5)
+    ks = [normal(rng, n, hkv, d, 1.4) for n in ctx]
+    for k in ks:
+        k[:, :, 32:64] += 1000 * np.cos(np.arange(len(k), dtype=np.float32))[:, None, None]
+    c = cache_of(ks, [normal(rng, n, hkv, d, 1.0) for n in ctx])
+    gen = torch.Generator().manual_seed(3)
+    x = torch.randn(2 * rows, hq, d, generator=gen) * 1.4
+    x[:, :, 32:64] -= x[:, :, 32:64].mean(-1, keepdim=True)
+    fine = 2.0 ** (14 if dtype == "f16" else 6)
+    q = ((x * fine).round() / fine).reshape(2 * rows, hq * d).to(DT[dtype]).cuda()
+    if dtype == "bf16":  # (its rounding leaves a sum, which the last element takes)
+        y = q.view(2 * rows, hq, d)[:, :, 32:64].float()
+        y = (y * 8).round() / 8
+        y[..., 31] -= y.sum(-1)
+        q.view(2 * rows, hq, d)[:, :, 32:64] = y.to(q.dtype)
+    q, out, scale = run(luc, c, [rows, rows], hq, dtype, q=q)
+    for row in range(2 * rows):
+        b, seen = row // rows, ctx[row // rows] - rows + row % rows + 1
+        want = torch.empty((1, hq, d), dtype=torch.float64, device="cuda")
+        tol = torch.empty_like(want)
+        for j in range(hq):
+            qj = q[row].double().view(hq, d)[j]
+            k, v = (t[:seen, j // (hq // hkv)] for t in (c.k[b], c.v[b]))
+            kg = k.unflatten(-1, (-1, GROUP))
+            m = kg.amin(-1)
+            qg = qj.view(-1, GROUP)
+            ns = ((kg - m[..., None]) * qg).sum(-1).abs().sum(-1) + (m * qg.sum(-1)).abs().sum(-1)
+            step = (kg.amax(-1) - m).amax(-1) / 15
+            unit = 2.0 ** (math.floor(math.log2(float(qj.abs().max()))) - 13)
+            p = torch.softmax(k @ qj * scale, 0)
+            o = p @ v
+            away = (v - o).abs()
+            e = scale * 2.0 ** -22 * ns + 2.0 ** -21
+            w2 = (scale * step * unit) ** 2 * d / 12 + (2.0 ** -20 / 12 if dtype == "bf16" else 0)
+            want[0, j] = o
+            tol[0, j] = (p * e) @ away + 6 * torch.sqrt((p * p * w2) @ (away * away)) + \
+                2.0 ** -17 * (p @ (v.abs() + 2 * v.abs().amax(-1, keepdim=True)))
+        ref.check(out[row].view(1, hq, d), want, tol, DT[dtype], f"row {row}, {seen} tokens")
