@@ -9,9 +9,10 @@
 // In the accumulators a lane has one column throughout (column lane % 16), so maxima, sums and
 // rescaling are lane-local up to the four lanes that share it, and the scores of 32 tokens are
 // already the operand of the second product: lane l holds four tokens of either 16-token fragment.
-// q is taken to fp16 after a power of two brings its largest element near one, exactly unless an
-// element is 2^-14 of that.  The running maximum moves only when a score passes it by some powers
-// of two, so most tiles rescale nothing.
+// q is taken to fp16 after a power of two brings its largest element to [1, 2) (columns) or [2^14, 2^15)
+// (tokens, whose n are fp16 subnormals), exactly unless an element is below 2^-14 or 2^-24 of that.  The
+// running maximum moves only when a score passes it by some powers of two, so most tiles rescale nothing.
+// Weights are held times a power of two, far above fp16's smallest.
 //
 // Two kernels:
 //   tokens: 8 columns a workgroup; its 4 waves take stages of tokens in turn and merge in LDS.  Few
@@ -620,11 +621,11 @@ __device__ inline bool kv4_longest_first(const Kv4AttnArgs& A, Kv4Seq& S, int& s
 // ---- waves split tokens: one workgroup per (split, sequence, kv head, 8-column tile) ----
 //
 // What bounds it, us a launch:
-//   64 sequences of 1024..16384, 28 and 4 heads of 128: 87.4 for 383 MB, 4.4 TB/s of the 5.2 that a large copy
+//   64 sequences of 1024..16384, 28 and 4 heads of 128: 90 for 383 MB, 4.2 TB/s of the 5.2 that a large copy
 //     reaches; the stream alone takes 74, the rest is products that do not hide behind it
-//   8 of 32768, 12 and 2 of 128: 26.2 for 81 MB: stream 14, products 5, the waves' merge 1.4, partials and
-//     their arrival 2.4, the merge of 32 splits 3.7
-//   32 of 128..4096, 14 and 2 of 64: 12.7 for 13 MB; one of 512: 6.7: the chain of lengths, pages, stages and
+//   8 of 32768, 12 and 2 of 128: 26.6 for 81 MB (which the last-level cache holds from call to call): stream 14,
+//     products 5.5, the waves' merge 1.4, partials and their arrival 2.4, the merge of 32 splits 3.7
+//   32 of 128..4096, 14 and 2 of 64: 13.1 for 13 MB; one of 512: 7.0: the chain of lengths, pages, stages and
 //     arrivals, not bytes
 // Tried: equal runs of stages over all units (104..119 at the first; the prologue of every run), eight
 // waves a workgroup (24.8 at the second, slower elsewhere), a ring of three at less occupancy (103),
@@ -895,10 +896,15 @@ __device__ void kv4_tokens_impl(const Kv4AttnArgs& A) {
 // 50.0..52.7, 69.8..74.7, 48.2..52.0, and with the softmax between the products of the next 32
 // tokens 52.5, 70, 48; a raised wave priority around the products no gain; expansion by every wave for
 // itself 105 at the first.
-//   bf16 rows: K and V are n s + m in fp16, one rounding of 2^-12, far below the output's 2^-9.
+//   bf16 rows: K and V are n s + m in fp16, one rounding of 2^-12, far below the output's 2^-9 (and an eighth of
+//     what K in bf16 is off by).  Where a group of K lies far from 0 and q takes that out of the scores, what the
+//     rounding leaves is seen: 2.5e-3 of the output with the group at 10, 8e-3 at 50; n and m apart, as fp16 rows
+//     have them, would be 11 products for 9 of 32 tokens at 64 dimensions, 19 for 17 at 128.
 //   fp16 rows (EXACT): that rounding of K and P's own would each add an error as large as the output's.
 //     K is n, and a group's products are scaled by s in 32 bits; the group's sum of q times m, q's sums
-//     in two fp16 parts, are a product of their own.  P is two fp16 parts.  V stays n s + m.
+//     in two fp16 parts, are a product of their own.  P is two fp16 parts.  V stays n s + m in one fp16: a
+//     second part would be 8 more products than the 28 of 32 tokens at 128 dimensions and as much LDS again, for
+//     errors of 2.1e-4 at most (the output's own rounding) in place of 2.8e-4.
 template <int DT, int D> struct Kv4Tile {
   static constexpr bool EXACT = DT == kF16;
   static constexpr int KS = D / 32;   // k steps of a score

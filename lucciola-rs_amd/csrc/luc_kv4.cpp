@@ -151,10 +151,11 @@ struct Kv4AttnArgs {
 constexpr int kCUs = 256;
 constexpr int kTokCols = 8;                   // columns of a workgroup
 constexpr int kTokMaxSplits = 256;            // kv4_attention.hip
-constexpr int kTokSlots = 2 * kCUs;           // resident workgroups
+constexpr int kTokSlots = 2 * kCUs;           // workgroups that a launch is planned for: two a CU (128 dimensions
+                                              // hold two, 64 three, by their registers)
 // Split lengths of a tokens launch: what fills the chip once, but not shorter than is worth a merge
-// and not longer than lets mixed contexts end together.  us at fixed lengths, batch x context,
-// heads:
+// and not longer than lets mixed contexts end together.  us at fixed lengths (of one build, up to 2% below
+// the present one's), batch x context, heads:
 //   8 x 32768, 12 and 2 of 128: 40.3 at 512, 25.6 at 1024 (the rule's) and 2048
 //   32 x 128..4096, 14 and 2 of 64: 13.9 at 256, 13.2 at 512 (the rule's), 13.7 at 1024
 //   64 x 1024..16384, 28 and 4 of 128: 104 at 1024, 87.6 at 2048 (the rule's), 90.9 at 4096;
@@ -174,8 +175,8 @@ constexpr int kTokRounds = 8;  // rounds of workgroups balance any contexts: lon
 constexpr int kTokMostCols = 48;
 // Columns of a workgroup of the columns kernel (Kv4Cols).
 constexpr int kColsOf64 = 128, kColsOf128 = 256;
-// Its splits fill the chip (128: a workgroup a CU; 64: two) once, but are not shorter than pays for
-// their partials.  us:
+// Its splits fill the chip once, planned as a workgroup a CU (128) or two (64, whose registers hold three), but
+// are not shorter than pays for their partials.  us:
 //   512 rows after 8000, 12 and 2 of 128: 44.3 at 832 and 45.0 at 896 (the rule's), 71 at 768, where a
 //     second round begins; 64 rows: 26.0 at 256 (the rule's), 29.8 at 512
 //   14 and 2 of 64, 512 rows after 8000: 45.2 at 576, 36.5 at 640, 36.7 at 960 (the rule's), 38.4 at
