@@ -470,7 +470,8 @@ int luc_kv4_append(luc_ctx* ctx, void* stream, int dtype, const void* q, const v
  * cu_seqlens[batch] stay as they are.  A sequence beyond max_rows or max_ctx, or
  * at a negative position, gets NaN outputs; so do rows whose context reaches a
  * page outside [0, num_blocks).  What the cache holds behind a row's own
- * position (NaN too) does not reach the row.  q 16-byte aligned with a row stride
+ * position (NaN too) does not reach the row.  Scores, sm_scale q . k, stay below
+ * 2^26 in size.  q 16-byte aligned with a row stride
  * that is a multiple of 8; out 8-byte aligned and 4.  max_ctx <= 2^30.
  * The workspace holds luc_kv4_workspace_size bytes (0: none needed), 256-byte
  * aligned, zero-filled once before its first use; every launch leaves it ready

@@ -63,6 +63,11 @@ __device__ inline uint32_t kv4_steps(int lift) { return (uint32_t)(27 - lift) <<
 // columns: weights, at most 2^kLazyMax of that, are held times this power of two, 2^15 at most.  (V is
 // multiplied in the matrix unit.)
 constexpr float kKv4ColsLift = 15.0f - kLazyMax;
+// What a largest score (in powers of two) makes the running maximum, less the lift: none where a rounding of the
+// score itself is as much as the room that the lift leaves below 2^16.
+__device__ inline float kv4_reference(float score, float lift) {
+  return fabsf(score) < 0x1p23f ? score - lift : score;
+}
 
 __device__ inline f32x4_t mfma16(uint4 a, uint4 b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
@@ -412,7 +417,7 @@ template <int DT, int D> struct Kv4Row {
     if (__any(top > bar)) {
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
-      const float mn = fmaxf(m, fmaf(top, scale, -(float)lift));
+      const float mn = fmaxf(m, kv4_reference(top * scale, (float)lift));
       const float a = __builtin_amdgcn_exp2f(m - mn);
       bar = fmaxf(bar, top + kKv4Lazy / scale);
       m = mn;
@@ -1196,7 +1201,7 @@ template <int DT, int D> struct Kv4Chunk {
       for (int f = 0; f < F; ++f) {
         float t = fmaxf(top[f], __shfl_xor(top[f], 16));
         t = fmaxf(t, __shfl_xor(t, 32));
-        const float mn = fmaxf(m[f], fmaf(t, scale[f], -kKv4ColsLift));
+        const float mn = fmaxf(m[f], kv4_reference(t * scale[f], kKv4ColsLift));
         const float a = __builtin_amdgcn_exp2f(m[f] - mn);
         bar[f] = fmaxf(bar[f], t + kLazyMax / scale[f]);
         m[f] = mn;

@@ -266,3 +266,33 @@ def test_keys_far_from_zero(luc, hq, hkv, d, dtype, rows):
             tol[0, j] = (p * e) @ away + 6 * torch.sqrt((p * p * w2) @ (away * away)) + \
                 2.0 ** -17 * (p @ (v.abs() + 2 * v.abs().amax(-1, keepdim=True)))
         ref.check(out[row].view(1, hq, d), want, tol, DT[dtype], f"row {row}, {seen} tokens")
+
+
+@pytest.mark.parametrize("rows", [1, 3, 40])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("top", [2.0 ** 19, 2.0 ** 22, 2.0 ** 25, 2.0 ** 28])
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (5, 1, 128)])
+def test_scores_whose_roundings_are_powers_of_two(luc, hq, hkv, d, top, dtype, rows):
+    """Scores up to 2^26 (many columns 2^28), where a step of 32 bits is some powers of e: the largest one's V is the output, where the next lies
+    2^-8 of it behind (K in fp16, 2^-11 of each product, moves a score of many terms less)."""
+    rng = np.random.default_rng(7)
+    ctx = 900
+    top = top if rows == 40 else min(top, 2.0 ** 26)
+    k = normal(rng, ctx, hkv, d, 300.0) * (1 + np.arange(ctx, dtype=np.float32) / 300)[:, None, None]
+    c = cache_of([k], [normal(rng, ctx, hkv, d, 1.0)])
+    gen = torch.Generator().manual_seed(4)
+    q = (torch.randn(rows, hq * d, generator=gen) * 50).to(DT[dtype]).cuda()
+    hidden = torch.arange(ctx, device="cuda")[None] > ctx - rows + torch.arange(rows, device="cuda")[:, None]
+    score = torch.stack([(q.double().view(rows, hq, d)[:, j] @ c.k[0][:, j // (hq // hkv)].t().contiguous())
+                         .masked_fill(hidden, -math.inf) for j in range(hq)], 1)
+    scale = top / float(score.max())
+    q, out, _ = run(luc, c, [rows], hq, dtype, q=q, scale=scale)
+    best = score.topk(2, -1)
+    sure = best.values[..., 0] - best.values[..., 1] > 2.0 ** -8 * best.values[..., 0]
+    assert float(sure.double().mean()) > 0.8 and float(best.values.min()) * scale > top / 8
+    want = torch.stack([c.v[0][best.indices[:, j, 0], j // (hq // hkv)] for j in range(hq)], 1)
+    got = out.view(rows, hq, d)
+    assert bool(got.isfinite().all())
+    # V in fp16 (many columns) and the output's rounding
+    tol = (2.0 ** -11 + torch.finfo(DT[dtype]).eps / 2) * want.abs() * 1.01 + 2.0 ** -20
+    assert bool(((got.double() - want).abs() <= tol)[sure].all())
