@@ -298,7 +298,7 @@ class Kv4Cache:
     """A 4-bit paged cache of up to `max_seqs` sequences (pools of luc_kv4_append, 0.31 of the
     bytes of 16 bits) and the DeviceBlocks behind it.  A step: `extend`, then `append` and
     `attend` for every layer; all of it may be captured in a HIP graph, and so may `truncate`.
-    Calls must be in one stream's order."""
+    Calls, and replays of captured ones, must be in one stream's order: they share a workspace."""
 
     def __init__(self, num_layers, num_q_heads, num_kv_heads, head_dim, num_physical_blocks,
                  max_seqs, max_position_embeddings, max_rows=None, device="cuda", lib=None):
