@@ -25,7 +25,8 @@
 //
 // What bounds it.  8191 rows of 28 + 2 x 4 heads of 128, 16 bits: 35 us for 155 MB from HBM (4.4 TB/s; a copy of as
 // many bytes 31), 26.7 on buffers that the last-level cache holds from call to call (the copy 22);
-// 32 rows of 14 + 2 x 2 of 64: 3.4 us, 64 rows of 28 + 2 x 4 of 128 into 4 bits 4.9 us, the latency of a launch and of position -> row of the table -> slot.
+// 32 rows of 14 + 2 x 2 of 64: 3.4 us, 64 rows of 28 + 2 x 4 of 128 into 4 bits 4.9 us, the latency
+// of a launch and of position -> row of the table -> slot.
 #include "kv4.h"
 
 namespace luc {
