@@ -364,11 +364,11 @@ int luc_sort_and_sample(luc_ctx* ctx, void* stream, int dtype, const void* logit
                         float top_p, int top_k, float rand_val, void* sort_buffer,
                         size_t sort_buffer_bytes, uint32_t* out_idx);
 
-/* ---- Serving over a paged cache held on the GPU, in 16 or 4 bits ----------
+/* ---- Serving over a paged cache held on the GPU, in 16, 8 or 4 bits -------
  * A serving step with no host work between its launches: pages for the new
  * rows (luc_block_extend), their norms, rotation and cache write
- * (luc_qk_norm_rope_append or luc_kv4_append), their attention
- * (luc_kv4_attention over a 4-bit cache).  Every call may be captured in a HIP
+ * (luc_qk_norm_rope_append, luc_kv8_append or luc_kv4_append), their attention
+ * (luc_kv8_attention or luc_kv4_attention).  Every call may be captured in a HIP
  * graph.  Arrays of a length that is 0 (rows, num_tokens, total_rows, batch) may
  * be NULL. */
 
@@ -486,6 +486,84 @@ int luc_kv4_attention(luc_ctx* ctx, void* stream, int dtype, void* out, int64_t 
                       int max_rows, int max_ctx, int layer, int num_layers, int num_q_heads,
                       int num_kv_heads, int head_dim, int block_size, float sm_scale, void* workspace,
                       size_t workspace_bytes);
+
+/* ---- The 8-bit cache ------------------------------------------------------
+ * Pools are [num_blocks][num_layers][Hkv] slabs of 16 * head_dim e4m3 codes (half of 16 bits), a value code *
+ * scale:
+ *   K slab: [16 tokens][head_dim];  V slab: [4][head_dim][4 tokens], tokens 4 i .. 4 i + 3 of the page in block i
+ *   scales: f32 [num_blocks][num_layers][Hkv][2], of K and of V: the 16 tokens of a page share one a head
+ *   bounds: [num_blocks][num_layers][Hkv][2][head_dim] codes, the largest and the smallest of a page's keys by
+ *     dimension (for luc_kv8_select; 1/16 of the pools).
+ * Scales are powers of two: 2^e with the smallest e >= -64 that brings the page's largest value to at most 448.
+ *
+ * luc_kv8_append is luc_qk_norm_rope_append into such pools.  k and v, as they would go to a 16-bit pool, clamped to
+ * +-60000 (a NaN stays one), become the nearest codes, ties to even.  A row at offset 0 of its page begins the
+ * page anew: its scales and bounds are those of the call's rows.  Rows at later offsets join what the page
+ * holds: the scales grow where they need to (every code of the page is then rounded again), the bounds take them
+ * in (a NaN counts as 0).  Slots of one call are distinct, and those of one page (same slot / 16) lie in successive rows, in
+ * ascending order without gaps, as luc_block_extend gives them.  bounds may be NULL: none are kept. */
+int luc_kv8_append(luc_ctx* ctx, void* stream, int dtype, const void* q, const void* k, const void* v,
+                   int64_t row_stride, const void* q_bias, const void* k_bias, const void* v_bias,
+                   const void* q_norm, const void* k_norm, float eps, const float* cos_table,
+                   const float* sin_table, int max_pos, const int32_t* positions, const int64_t* slots,
+                   int num_tokens, void* q_out, int64_t q_out_stride, void* k_pool, void* v_pool, float* scales,
+                   void* bounds, int num_blocks, int layer, int num_layers, int num_q_heads, int num_kv_heads,
+                   int head_dim, int block_size);
+
+/* K and V of tokens of an 8-bit cache, rounded to dtype: row r of k_out and v_out (at + r * out_row_stride, [Hkv]
+ * [head_dim]) gets slot slots[r]; a slot outside [0, num_blocks * 16) leaves its row as it is.  Outputs
+ * 16-byte aligned, the stride a multiple of 8. */
+int luc_kv8_read(luc_ctx* ctx, void* stream, int dtype, void* k_out, void* v_out, int64_t out_row_stride,
+                 const int64_t* slots, int num_tokens, const void* k_pool, const void* v_pool, const float* scales,
+                 int num_blocks, int layer, int num_layers, int num_kv_heads, int head_dim, int block_size);
+
+/* luc_kv4_attention over an 8-bit cache: the same rows, bounds, outputs and workspace rules.  Values enter as dtype
+ * holds them. */
+size_t luc_kv8_workspace_size(int batch, int total_rows, int max_rows, int max_ctx, int num_q_heads,
+                              int num_kv_heads, int head_dim);
+int luc_kv8_attention(luc_ctx* ctx, void* stream, int dtype, void* out, int64_t out_row_stride,
+                      const void* q, int64_t q_row_stride, const void* k_pool, const void* v_pool,
+                      const float* scales, const int32_t* block_tables, int table_stride, int num_blocks,
+                      const int32_t* cu_seqlens, const int32_t* start_pos, int batch, int total_rows,
+                      int max_rows, int max_ctx, int layer, int num_layers, int num_q_heads,
+                      int num_kv_heads, int head_dim, int block_size, float sm_scale, void* workspace,
+                      size_t workspace_bytes);
+
+/* Attention over chosen pages of long contexts, for one row a sequence: a choice, and attention over it.
+ *
+ * luc_kv8_select writes to pages [batch][Hkv][budget], for each sequence and kv head, the numbers of the pages
+ * of its context (0 is positions 0 .. 15) that the row attends to, ascending, -1 behind the last: all of them, if there
+ * are no more than budget, else the first `first`, the last `recent` (the row's own page among them) and of the others
+ * those that score highest, equal scores to the lower page.  The score of a page is the largest over the group's heads of
+ *   (((S_0 2^e_0 + S_1 2^e_1) + S_2 2^e_2) + S_3 2^e_3) * scale_K    (head_dim / 32 terms; the additions in f32)
+ *   S_j = sum over dimensions i of 32 j .. 32 j + 31 of n_i * (n_i > 0 ? largest_i : smallest_i), a whole number
+ * with the page's bounds in whole code units (nearest, ties to even), n = rint(q 2^-e_j) and e_j the smallest that
+ * brings those 32 elements of q to at most 127: q . k of the page's keys is at most that, but for the roundings.  A page outside
+ * [0, num_blocks) scores lowest.  A NaN of q counts as 0, q is clamped to +-60000; a sequence without a row, or
+ * whose context is more than max_ctx, gets -1.
+ *
+ * luc_kv8_sparse_attention attends to positions 0 .. start_pos[b] that lie in `pages`, as luc_kv8_select writes them
+ * (with the same budget; min(budget, pages of the context) entries are read, the last of which is the
+ * row's own page; a list with another entry in its place, or one outside the context, gives NaN).
+ *
+ * Rows, cu_seqlens, start_pos, total_rows and max_ctx as in luc_kv4_attention, with at most one row a
+ * sequence (more: NaN).  Both use one workspace of luc_kv8_sparse_workspace_size bytes, 256-byte aligned,
+ * zero-filled once; one call after the other leaves it ready for the next. */
+size_t luc_kv8_sparse_workspace_size(int batch, int max_ctx, int budget, int num_q_heads, int num_kv_heads,
+                                     int head_dim);
+int luc_kv8_select(luc_ctx* ctx, void* stream, int dtype, int32_t* pages, int budget, int first, int recent,
+                   const void* q, int64_t q_row_stride, const void* bounds, const float* scales,
+                   const int32_t* block_tables, int table_stride, int num_blocks, const int32_t* cu_seqlens,
+                   const int32_t* start_pos, int batch, int total_rows, int max_ctx, int layer, int num_layers,
+                   int num_q_heads, int num_kv_heads, int head_dim, int block_size, void* workspace,
+                   size_t workspace_bytes);
+int luc_kv8_sparse_attention(luc_ctx* ctx, void* stream, int dtype, void* out, int64_t out_row_stride,
+                             const void* q, int64_t q_row_stride, const void* k_pool, const void* v_pool,
+                             const float* scales, const int32_t* block_tables, int table_stride, int num_blocks,
+                             const int32_t* pages, int budget, const int32_t* cu_seqlens,
+                             const int32_t* start_pos, int batch, int total_rows, int max_ctx, int layer,
+                             int num_layers, int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                             float sm_scale, void* workspace, size_t workspace_bytes);
 
 /* ---- Multi-sequence page allocator (host only: no GPU call, no ctx) ------
  * Generalises KVCache's free list and prepare_for_step

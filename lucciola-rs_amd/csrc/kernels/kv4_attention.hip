@@ -24,6 +24,7 @@
 // workspace; tokens: the last workgroup of a (sequence, kv head, column tile) to arrive
 // merges them; columns: a second launch does.
 #include "kv4.h"
+#include "kv_split.h"
 
 namespace luc {
 
@@ -47,8 +48,6 @@ struct Kv4AttnArgs {
   int32_t longest_first;
   float qk_scale_log2;
 };
-
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 // The running maximum moves when a score (in powers of two) passes it by this: weights are at most
 // 8 times what the largest had when it moved.
@@ -111,38 +110,6 @@ __device__ inline float max3(float a, float b, float c) {
 // infinities: an exponent of all ones is NaN).
 __device__ inline uint32_t kv4_nan(uint32_t s, uint32_t m) {
   return (((s & 0x7c007c00u) + 0x04000400u) | ((m & 0x7c007c00u) + 0x04000400u)) & 0x80008000u;
-}
-
-// A sequence's rows, the position of the first, and its context: 0 where that is longer, or the
-// rows are more, than the call allows, or the position is none.
-struct Kv4Seq {
-  int row0, rows, start, ctx;
-};
-__device__ inline Kv4Seq kv4_seq(const Kv4AttnArgs& A, int b) {
-  Kv4Seq s;
-  s.row0 = A.cu_seqlens ? A.cu_seqlens[b] : b;
-  const int end = A.cu_seqlens ? A.cu_seqlens[b + 1] : b + 1;
-  s.row0 = min(max(s.row0, 0), A.total_rows);
-  s.rows = max(min(end, A.total_rows) - s.row0, 0);
-  s.start = A.start_pos[b];
-  const int64_t ctx = (int64_t)s.start + s.rows;
-  s.ctx = s.start >= 0 && ctx <= A.max_ctx && s.rows <= A.max_rows ? (int)ctx : 0;
-  return s;
-}
-// The rows of a sequence without a context: NaN.
-template <int DT, int D>
-__device__ inline void kv4_no_context(const Kv4AttnArgs& A, const Kv4Seq& S, int kvh) {
-  const int width = A.group * D;
-  for (int64_t i = threadIdx.x; i < (int64_t)S.rows * width; i += blockDim.x)
-    A.out[(S.row0 + i / width) * A.out_stride + (int64_t)kvh * width + i % width] = St<DT>::store(__builtin_nanf(""));
-}
-
-// (agent scope: read by a workgroup of another XCD)
-__device__ inline void ws_put(float* p, float x) {
-  __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ inline float ws_get(const float* p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // Of the two halves of a dword.
@@ -564,65 +531,7 @@ template <int DT, int D> struct Kv4Row {
   }
 };
 
-// 16-byte agent-scope accesses of the workspace (sc1, as the scoped atomics above).
-__device__ inline __amdgpu_buffer_rsrc_t ws_rsrc(const float* p) {
-  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, 0x7fffffff, 0x00020000);
-}
-constexpr int kAuxSc1 = 16;
-__device__ inline float4 ws_get4(__amdgpu_buffer_rsrc_t r, int at) {  // at: floats
-  return __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(r, at * 4, 0, kAuxSc1));
-}
-__device__ inline void ws_put4(__amdgpu_buffer_rsrc_t r, int at, float4 x) {
-  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, x), r, at * 4, 0, kAuxSc1);
-}
-
-constexpr int kTokWaves = 4;
-constexpr int kTokCols = 8;   // columns of a workgroup
 constexpr int kTokRing = 2;  // stages of a wave
-constexpr int kTokMaxSplits = 256;
-
-// The work of workgroup blockIdx.x where there are more than fit the chip at once: full splits
-// first, then the sequences' last ones, longest first, so that the launch does not end on full splits
-// that started late (plain order deals a split of every sequence in turn).  At most 64 sequences, one a
-// lane; one tile a sequence.  False: no work.
-__device__ inline bool kv4_longest_first(const Kv4AttnArgs& A, Kv4Seq& S, int& split, int& b, int& kvh) {
-  const int lane = threadIdx.x & 63;
-  Kv4Seq own{};
-  if (lane < A.batch) own = kv4_seq(A, lane);
-  const int full = own.rows ? own.ctx / A.split_tokens : 0;
-  // (no context: the rows still get their NaN, from split 0)
-  const int rest = own.rows && (own.ctx == 0 || own.ctx % A.split_tokens) ? own.ctx % A.split_tokens : -1;
-  int end = full * A.hkv;
-#pragma unroll
-  for (int k = 1; k < 64; k <<= 1) {
-    const int y = __shfl_up(end, k);
-    if (lane >= k) end += y;
-  }
-  int i = blockIdx.x;
-  const int all = __builtin_amdgcn_readlane(end, 63);
-  if (i < all) {
-    b = __builtin_ctzll(__ballot(i < end));
-    i -= __builtin_amdgcn_readlane(end - full * A.hkv, b);
-    split = i / A.hkv;
-  } else {
-    i -= all;
-    int rank = 0;
-    for (int k = 0; k < A.batch; ++k) {
-      const int r = __builtin_amdgcn_readlane(rest, k);
-      rank += r > rest || (r == rest && k < lane);
-    }
-    const uint64_t at = __ballot(rest >= 0 && rank == i / A.hkv);
-    if (!at) return false;
-    b = __builtin_ctzll(at);
-    split = __builtin_amdgcn_readlane(full, b);
-  }
-  kvh = i % A.hkv;
-  S.row0 = __builtin_amdgcn_readlane(own.row0, b);
-  S.rows = __builtin_amdgcn_readlane(own.rows, b);
-  S.start = __builtin_amdgcn_readlane(own.start, b);
-  S.ctx = __builtin_amdgcn_readlane(own.ctx, b);
-  return true;
-}
 
 // ---- waves split tokens: one workgroup per (split, sequence, kv head, 8-column tile) ----
 //
@@ -654,9 +563,9 @@ __device__ void kv4_tokens_impl(const Kv4AttnArgs& A) {
   static_assert(NW * 2 * TC * OS * 4 <= (int)sizeof(s_ring) && NT * 16 + kTokMaxSplits * TC * 4 <= (int)sizeof(s_ring), "fits");
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int split, tile, b, kvh;
-  Kv4Seq S;
+  KvSeq S;
   if (A.longest_first) {
-    if (!kv4_longest_first(A, S, split, b, kvh)) return;
+    if (!kv_longest_first(A, S, split, b, kvh)) return;
     tile = 0;
   } else {
     const int units = A.batch * A.hkv * A.tiles;
@@ -665,13 +574,13 @@ __device__ void kv4_tokens_impl(const Kv4AttnArgs& A) {
     tile = u % A.tiles;
     b = u / A.tiles / A.hkv;
     kvh = u / A.tiles % A.hkv;
-    S = kv4_seq(A, b);
+    S = kv_seq(A, b);
   }
   const int unit = (b * A.hkv + kvh) * A.tiles + tile;
   const int col0 = tile * TC, ncols = S.rows * A.group;
   const int here = min(TC, ncols - col0);
   if (S.ctx == 0) {
-    if (split == 0 && tile == 0) kv4_no_context<DT, D>(A, S, kvh);
+    if (split == 0 && tile == 0) kv_no_context<DT, D>(A, S, kvh);
     return;
   }
   if (here <= 0) return;
@@ -1280,9 +1189,9 @@ __device__ void kv4_columns_impl(const Kv4AttnArgs& A) {
   const int split = blockIdx.x / (pairs * A.tiles), rest = blockIdx.x % (pairs * A.tiles);
   const int chunk = A.tiles - 1 - rest / pairs, bh = (rest + rest / pairs) % pairs;
   const int b = bh / A.hkv, kvh = bh % A.hkv;
-  const Kv4Seq S = kv4_seq(A, b);
+  const KvSeq S = kv_seq(A, b);
   if (S.ctx == 0) {
-    if (split == 0 && chunk == 0) kv4_no_context<DT, D>(A, S, kvh);
+    if (split == 0 && chunk == 0) kv_no_context<DT, D>(A, S, kvh);
     return;
   }
   const int ncols = S.rows * A.group;
@@ -1389,61 +1298,6 @@ __device__ void kv4_columns_impl(const Kv4AttnArgs& A) {
   }
 }
 
-// The partials of a columns launch: D / 4 lanes a (row, head).
-template <int DT, int D>
-__device__ void kv4_merge_impl(const Kv4AttnArgs& A) {
-  constexpr int LANES = D / 4;
-  const int hq = A.hkv * A.group;
-  const int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / LANES;
-  const int d = threadIdx.x % LANES * 4;
-  if (item >= (int64_t)A.total_rows * hq) return;
-  const int row = (int)(item / hq), head = (int)(item % hq);
-  int b = row;
-  if (A.cu_seqlens) {
-    int lo = 0, hi = A.batch - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (A.cu_seqlens[mid] <= row) lo = mid; else hi = mid - 1;
-    }
-    b = lo;
-  }
-  const Kv4Seq S = kv4_seq(A, b);
-  const int r = row - S.row0;
-  if (r < 0 || r >= S.rows || S.ctx == 0) return;  // no sequence's row, or written already
-  const int nsplit = min(A.splits, (S.start + r) / A.split_tokens + 1);
-  const int64_t step = (int64_t)A.total_rows * hq;
-  float M = -3.4028235e38f, L = 0.0f;
-  float4 o = make_float4(0, 0, 0, 0);
-  // eight splits' loads under way at once (those past the last read the last again, times 0)
-  for (int s0 = 0; s0 < nsplit; s0 += 8) {
-    float2 ml[8];
-    float4 x[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int64_t at = item + min(s0 + i, nsplit - 1) * step;
-      ml[i] = *(const float2*)(A.ws_ml + at * 2);
-      x[i] = *(const float4*)(A.ws_o + at * D + d);
-    }
-    float top = M;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = fmaxf(top, ml[i].x);
-    const float a = __builtin_amdgcn_exp2f(M - top);
-    M = top;
-    L *= a;
-    o.x *= a; o.y *= a; o.z *= a; o.w *= a;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float e = s0 + i < nsplit ? __builtin_amdgcn_exp2f(ml[i].x - M) : 0.0f;
-      L = fmaf(e, ml[i].y, L);
-      o.x = fmaf(e, x[i].x, o.x); o.y = fmaf(e, x[i].y, o.y); o.z = fmaf(e, x[i].z, o.z); o.w = fmaf(e, x[i].w, o.w);
-    }
-  }
-  const float inv = 1.0f / L;
-  const uint32_t a0 = St<DT>::store(o.x * inv) | (uint32_t)St<DT>::store(o.y * inv) << 16;
-  const uint32_t a1 = St<DT>::store(o.z * inv) | (uint32_t)St<DT>::store(o.w * inv) << 16;
-  *(uint2*)(A.out + row * A.out_stride + (int64_t)head * D + d) = make_uint2(a0, a1);
-}
-
 }  // namespace luc
 
 #define LUC_KV4_ATTENTION(DTN, DT, D)                                                            \
@@ -1454,7 +1308,7 @@ __device__ void kv4_merge_impl(const Kv4AttnArgs& A) {
     luc::kv4_columns_impl<luc::DT, D>(a);                                                        \
   }                                                                                              \
   extern "C" __global__ __launch_bounds__(256) void luc_kv4_merge_##DTN##_d##D(luc::Kv4AttnArgs a) {      \
-    luc::kv4_merge_impl<luc::DT, D>(a);                                                          \
+    luc::kv_merge_impl<luc::DT, D>(a);                                                          \
   }
 LUC_KV4_ATTENTION(bf16, kBF16, 64)
 LUC_KV4_ATTENTION(bf16, kBF16, 128)

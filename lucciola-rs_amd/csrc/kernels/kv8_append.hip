@@ -1,0 +1,258 @@
+// Appends into the 8-bit paged cache of kv8.h, and its tokens back in 16 bits (gfx950).
+//
+// Append: bias, head norms and RoPE as norm_append.hip has them (append_row.h); q in 16 bits to q_out; of k and v, as
+// they would go to a 16-bit pool, codes, scales and key bounds to the pages of the rows' slots:
+//   e = max(the page's exponent, the smallest that holds the new rows),   code = e4m3(x 2^-e)
+// A page begins anew with its first token: then only the new rows count.  Where a page's exponent grows, the
+// codes that it holds are rounded again, and its bounds with them (rounding keeps order, so the bounds stay those
+// of the codes).
+//
+// Runs.  Rows of one page follow one another with ascending slots.  A wave has one run of K or of V of one head: the
+// rows that go to one page, up to 16, D / 16 lanes a row.  Its extremes are a reduction of the wave; the codes
+// take their places by way of LDS, and 16 bytes a lane go out side by side.  A wave is launched for every
+// row, and those of rows that do not begin a run end at once.
+#include "append_row.h"
+#include "kv8.h"
+
+namespace luc {
+
+struct Kv8AppendArgs : NormAppendArgs {  // (k_out, v_out unused)
+  float* scales;
+  uint8_t* bounds;  // or null
+};
+
+constexpr int kAppendWaves = 4;
+
+template <int DT, int D>
+__device__ void kv8_append_impl(const Kv8AppendArgs& A) {
+#pragma clang fp contract(off)
+  constexpr int LANES = D / 16;
+  constexpr int ROWS = 64 / LANES, PASSES = 16 / ROWS;  // rows of a pass
+  constexpr int CHUNKS = D / 64;                        // 16 bytes of a slab a lane
+  __shared__ __attribute__((aligned(16))) uint8_t s_image[kAppendWaves][Kv8<D>::kSlab];
+  const uint32_t nq = (uint32_t)A.rows * A.hq;
+  const uint32_t q_blocks = (nq + 256 / LANES - 1) / (256 / LANES);
+  if (blockIdx.x < q_blocks) {
+    const uint32_t unit = (blockIdx.x * 256 + threadIdx.x) / LANES;
+    const int c = threadIdx.x % LANES;
+    if (unit >= nq) return;
+    const int row = unit / A.hq, hh = unit % A.hq;
+    const int pos = A.positions[row];
+    if (pos < 0 || pos >= A.max_pos) return;
+    float x[16];
+    append_head<DT, D>(A, 0, row, hh, c, pos, x);
+    uint16_t* const o = A.q_out + row * A.q_out_stride + hh * D;
+    *(uint4*)(o + 8 * c) = pack8<DT>(x);
+    *(uint4*)(o + D / 2 + 8 * c) = pack8<DT>(x + 8);
+    return;
+  }
+  // ---- one run of one head of k or v
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const uint32_t unit = (blockIdx.x - q_blocks) * kAppendWaves + w;  // (the grid's threads fit 32 bits)
+  if (unit >= 2u * A.hkv * A.rows) return;
+  const int row = unit % A.rows;
+  const int hh = unit / A.rows % A.hkv, is_v = unit / A.rows / A.hkv;
+  // lane i: row row - 1 + i; rows without a position or a slot belong to no run
+  int64_t slot = -1;
+  int pos = -1;
+  const int at = row - 1 + lane;
+  if (lane <= 16 && at >= 0 && at < A.rows) {
+    slot = A.slots[at];
+    pos = A.positions[at];
+    if (pos < 0 || pos >= A.max_pos || slot < 0 || slot >= A.num_slots) slot = -1;
+  }
+  const int64_t first = __shfl(slot, 1), before = __shfl(slot, 0);
+  const int off = (int)(first & (kPage - 1));
+  if (first < 0 || (off && before == first - 1)) return;
+  const uint64_t in = __ballot(lane >= 1 && slot == first + (lane - 1) && off + lane - 1 < kPage);
+  const int len = __builtin_ctzll(~(in >> 1));
+  const int64_t head = ((first >> 4) * A.num_layers + A.layer) * A.hkv + hh;
+  uint8_t* const slab = (uint8_t*)(is_v ? A.v_pool : A.k_pool) + head * Kv8<D>::kSlab;
+  float* const scale_at = A.scales + head * 2 + is_v;
+  const int held = off ? max(exp2of(*scale_at), kKv8LeastExp) : kKv8LeastExp;
+  // new tokens of the lane's chunks, a mask of bytes; where some bytes stay, they are read first
+  uint32_t fresh[CHUNKS];
+  uint4 old[CHUNKS];
+#pragma unroll
+  for (int i = 0; i < CHUNKS; ++i) {
+    const int b = 16 * (lane + 64 * i);
+    if (is_v) {
+      fresh[i] = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int t = b / (4 * D) * 4 + k;
+        if (t >= off && t < off + len) fresh[i] |= 0xffu << (8 * k);
+      }
+    } else {
+      fresh[i] = b / D >= off && b / D < off + len ? ~0u : 0u;
+    }
+    old[i] = make_uint4(0, 0, 0, 0);
+    if (fresh[i] != 0 && fresh[i] != ~0u) old[i] = *(const uint4*)(slab + b);
+  }
+  // ---- the rows' values, in 16 bits and back
+  const int c = lane % LANES, kind = 1 + is_v;
+  float x[PASSES][16];
+  float top = 0.0f;
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    const int j = p * ROWS + lane / LANES;
+    const int pj = __shfl(pos, j + 1);
+    if (j >= len) continue;
+    append_head<DT, D>(A, kind, row + j, hh, c, pj, x[p]);
+    const uint4 a = pack8<DT>(x[p]), b = pack8<DT>(x[p] + 8);
+    unpack8<DT>(a, x[p]);
+    unpack8<DT>(b, x[p] + 8);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float y = x[p][e];
+      x[p][e] = __builtin_isnan(y) ? y : fminf(fmaxf(y, -kKv8Limit), kKv8Limit);
+      top = fmaxf(top, fabsf(x[p][e]));
+    }
+  }
+  const int e = max(kv8_exponent(wave_max(top)), held);
+  const float up = pow2f(-e), less = pow2f(held - e);
+  const bool grown = off && e != held;
+  // ---- codes by way of LDS
+  uint8_t* const image = s_image[w];
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    const int j = p * ROWS + lane / LANES, t = off + j;
+    if (j >= len) continue;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t code[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float* const y = x[p] + 8 * h + 4 * k;
+        code[k] = kv8_encode4(y[0] * up, y[1] * up, y[2] * up, y[3] * up);
+      }
+      const int i = D / 2 * h + 8 * c;
+      if (is_v) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          image[Kv8<D>::v_at(t >> 2, i + k) + (t & 3)] = (uint8_t)(code[k >> 2] >> (8 * (k & 3)));
+      } else {
+        *(uint2*)(image + Kv8<D>::k_at(t, i)) = make_uint2(code[0], code[1]);
+      }
+    }
+  }
+  wave_lds_sync();
+#pragma unroll
+  for (int i = 0; i < CHUNKS; ++i) {
+    const int b = 16 * (lane + 64 * i);
+    uint32_t o[4] = {old[i].x, old[i].y, old[i].z, old[i].w};
+    if (grown && fresh[i] != ~0u) {
+      const uint4 y = *(const uint4*)(slab + b);
+      o[0] = kv8_rescale4(y.x, less); o[1] = kv8_rescale4(y.y, less);
+      o[2] = kv8_rescale4(y.z, less); o[3] = kv8_rescale4(y.w, less);
+    }
+    if (fresh[i] == 0 && !grown) continue;
+    const uint4 n = *(const uint4*)(image + b);
+    const uint32_t f = fresh[i];
+    *(uint4*)(slab + b) = make_uint4((n.x & f) | (o[0] & ~f), (n.y & f) | (o[1] & ~f), (n.z & f) | (o[2] & ~f),
+                                     (n.w & f) | (o[3] & ~f));
+  }
+  if (lane == 0) *scale_at = pow2f(e);
+  if (is_v || !A.bounds) return;
+  // ---- key bounds: a lane has 4 dimensions of every 256 / D'th token
+  constexpr int QUADS = D / 4, SETS = 64 / QUADS;
+  const int quad = lane % QUADS, set = lane / QUADS;
+  float hi[4], lo[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    hi[k] = -INFINITY;
+    lo[k] = INFINITY;
+  }
+  uint8_t* const bound = A.bounds + head * (2 * D) + 4 * quad;
+  auto take = [&](uint32_t word, uint32_t word_lo, float f) __attribute__((always_inline)) {
+    const float4 a = kv8_decode4(word), b = kv8_decode4(word_lo);
+    const float ya[4] = {a.x, a.y, a.z, a.w}, yb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      hi[k] = fmaxf(hi[k], __builtin_isnan(ya[k]) ? 0.0f : ya[k] * f);
+      lo[k] = fminf(lo[k], __builtin_isnan(yb[k]) ? 0.0f : yb[k] * f);
+    }
+  };
+  if (off && set == 0)  // (rounded again, as the codes are)
+    take(kv8_rescale4(*(const uint32_t*)bound, less), kv8_rescale4(*(const uint32_t*)(bound + D), less), 1.0f);
+#pragma unroll
+  for (int t0 = 0; t0 < kPage; t0 += SETS) {
+    const int t = t0 + set;
+    if (t < off || t >= off + len) continue;
+    const uint32_t y = *(const uint32_t*)(image + Kv8<D>::k_at(t, 4 * quad));
+    take(y, y, 1.0f);
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int s = QUADS; s < 64; s <<= 1) {
+      hi[k] = fmaxf(hi[k], __shfl_xor(hi[k], s));
+      lo[k] = fminf(lo[k], __shfl_xor(lo[k], s));
+    }
+  if (set == 0) {
+    *(uint32_t*)bound = kv8_encode4(hi[0], hi[1], hi[2], hi[3]);
+    *(uint32_t*)(bound + D) = kv8_encode4(lo[0], lo[1], lo[2], lo[3]);
+  }
+}
+
+// ---- tokens back in 16 bits: a thread has 8 dimensions of K or V of a row's head
+struct Kv8ReadArgs {
+  uint16_t* k_out;
+  uint16_t* v_out;
+  int64_t out_stride;
+  const int64_t* slots;
+  const uint8_t* k_pool;
+  const uint8_t* v_pool;
+  const float* scales;
+  int64_t num_slots;
+  int32_t rows, layer, num_layers, hkv;
+};
+
+template <int DT, int D>
+__device__ void kv8_read_impl(const Kv8ReadArgs& A) {
+  constexpr int T = D / 8;  // threads of a head
+  const uint32_t each = (uint32_t)A.rows * A.hkv * T;  // (twice that fits 32 bits)
+  uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  const bool is_v = i >= each;
+  if (is_v) i -= each;
+  if (i >= each) return;
+  const int c = i % T, hh = i / T % A.hkv, row = i / T / A.hkv;
+  const int64_t slot = A.slots[row];
+  if (slot < 0 || slot >= A.num_slots) return;
+  const int t = (int)(slot & (kPage - 1));
+  const int64_t head = ((slot >> 4) * A.num_layers + A.layer) * A.hkv + hh;
+  const float scale = A.scales[head * 2 + is_v];
+  uint32_t a, b;
+  if (is_v) {
+    const uint4* const p = (const uint4*)(A.v_pool + head * Kv8<D>::kSlab + Kv8<D>::v_at(t >> 2, 8 * c));
+    const uint4 u = p[0], v = p[1];
+    // byte t % 4 of every dword: of two dwords (selectors 0 .. 3 the second operand's, 4 .. 7 the first's), then of four
+    const uint32_t s = (uint32_t)(t & 3), sel = s | (s + 4) << 8;
+    a = __builtin_amdgcn_perm(u.y, u.x, sel) & 0xffffu;
+    a |= __builtin_amdgcn_perm(u.w, u.z, sel) << 16;
+    b = __builtin_amdgcn_perm(v.y, v.x, sel) & 0xffffu;
+    b |= __builtin_amdgcn_perm(v.w, v.z, sel) << 16;
+  } else {
+    const uint2 u = *(const uint2*)(A.k_pool + head * Kv8<D>::kSlab + Kv8<D>::k_at(t, 8 * c));
+    a = u.x;
+    b = u.y;
+  }
+  uint16_t* const o = (is_v ? A.v_out : A.k_out) + row * A.out_stride + hh * D + 8 * c;
+  *(uint4*)o = make_uint4(kv8_pair<DT, false>(a, scale), kv8_pair<DT, true>(a, scale), kv8_pair<DT, false>(b, scale),
+                          kv8_pair<DT, true>(b, scale));
+}
+
+}  // namespace luc
+
+#define LUC_KV8_APPEND(DTN, DT, D)                                                              \
+  extern "C" __global__ __launch_bounds__(256) void luc_kv8_append_##DTN##_d##D(                \
+      luc::Kv8AppendArgs a) {                                                                   \
+    luc::kv8_append_impl<luc::DT, D>(a);                                                        \
+  }                                                                                             \
+  extern "C" __global__ __launch_bounds__(256) void luc_kv8_read_##DTN##_d##D(luc::Kv8ReadArgs a) { \
+    luc::kv8_read_impl<luc::DT, D>(a);                                                          \
+  }
+LUC_KV8_APPEND(bf16, kBF16, 64)
+LUC_KV8_APPEND(bf16, kBF16, 128)
+LUC_KV8_APPEND(f16, kF16, 64)
+LUC_KV8_APPEND(f16, kF16, 128)

@@ -45,7 +45,8 @@ constexpr const char* kCodeObjects[] = {"rope_append.hsaco",   "paged_decode.hsa
                                          "model_ops.hsaco",     "prompt_gemm.hsaco",
                                          "sampling.hsaco",      "probe_gather.hsaco",
                                          "block_map.hsaco",     "norm_append.hsaco",
-                                         "kv4_attention.hsaco"};
+                                         "kv4_attention.hsaco", "kv8_append.hsaco",
+                                         "kv8_attention.hsaco", "kv8_select.hsaco"};
 
 // Kernel-side constants (kept in step with csrc/kernels/paged_decode.hip):
 // four waves per workgroup, which share one split; tiles of 64 tokens
@@ -624,6 +625,7 @@ int luc_init(int device, const char* code_object_dir, luc_ctx** out_ctx) {
         }
   }
   for (const std::string& n : luc_internal::kv4_kernel_names()) names.push_back(n);
+  for (const std::string& n : luc_internal::kv8_kernel_names()) names.push_back(n);
   for (const auto& n : names) {
     hipFunction_t fn = nullptr;
     for (hipModule_t m : ctx->modules)

@@ -10,15 +10,9 @@ using namespace luc_internal;
 
 namespace {
 
-const char* dt_name(int dtype) { return dtype == LUC_F16 ? "f16" : "bf16"; }
-
 constexpr int kGroup4 = 32;             // values of a 4-bit group (kernels/kv4.h)
 constexpr int kMaxMapBatch = 4096;      // block_map.hip: kMaxSeqs
 constexpr int kMaxTableStride = 1 << 26;  // positions stay below 2^30
-
-constexpr int kMaxHeads = 1 << 20;        // rows of heads stay within 32 bits
-
-int64_t align256(int64_t n) { return ceil_div(n, 256) * 256; }
 
 // luc::MapArgs of block_map.hip: the same fields in the same order.
 struct MapArgs {
@@ -48,75 +42,9 @@ int check_map(const luc_ctx* ctx, const MapArgs& a, int table_stride) {
   return LUC_OK;
 }
 
-// luc::NormAppendArgs of norm_append.hip: the same fields in the same order.
-struct NormAppendArgs {
-  const void* q;
-  const void* k;
-  const void* v;
-  int64_t row_stride;
-  const void* q_bias;
-  const void* k_bias;
-  const void* v_bias;
-  const void* q_norm;
-  const void* k_norm;
-  const float* cos_t;
-  const float* sin_t;
-  const int32_t* positions;
-  const int64_t* slots;
-  void* q_out;
-  int64_t q_out_stride;
-  void* k_out;
-  void* v_out;
-  int64_t kv_out_stride;
-  void* k_pool;
-  void* v_pool;
-  int64_t num_slots;
-  float eps;
-  int32_t rows, max_pos, layer, num_layers, hq, hkv;
-};
-
-int check_sizes(const luc_ctx* ctx, int dtype, int hq, int hkv, int head_dim, int block_size, int layer,
-                int num_layers, int num_blocks) {
-  if (!ctx) return fail(LUC_E_INVALID, "null context");
-  if (dtype != LUC_BF16 && dtype != LUC_F16) return fail(LUC_E_INVALID, "bad dtype %d", dtype);
-  if (head_dim != 64 && head_dim != 128)
-    return fail(LUC_E_UNSUPPORTED, "unsupported head_dim %d (64 or 128)", head_dim);
-  if (hq <= 0 || hkv <= 0) return fail(LUC_E_INVALID, "head counts must be positive");
-  if (hq > kMaxHeads) return fail(LUC_E_INVALID, "num_q_heads %d above %d", hq, kMaxHeads);
-  if (hq % hkv) return fail(LUC_E_INVALID, "num_q_heads %d not a multiple of num_kv_heads %d", hq, hkv);
-  if (hq / hkv > 8) return fail(LUC_E_UNSUPPORTED, "group size %d > 8", hq / hkv);
-  if (block_size != LUC_BLOCK_SIZE)
-    return fail(LUC_E_UNSUPPORTED, "block_size %d (only %d)", block_size, LUC_BLOCK_SIZE);
-  if (num_layers <= 0 || layer < 0 || layer >= num_layers)
-    return fail(LUC_E_INVALID, "layer %d outside [0, %d)", layer, num_layers);
-  if (num_blocks < 1) return fail(LUC_E_INVALID, "num_blocks %d < 1", num_blocks);
-  return LUC_OK;
-}
-
 int norm_append(luc_ctx* ctx, void* stream, int dtype, const char* kind, NormAppendArgs& a, int num_blocks,
                 int head_dim, int block_size) {
-  if (int rc = check_sizes(ctx, dtype, a.hq, a.hkv, head_dim, block_size, a.layer, a.num_layers, num_blocks))
-    return rc;
-  if (a.rows < 0) return fail(LUC_E_INVALID, "num_tokens %d < 0", a.rows);
-  if (a.max_pos < 1) return fail(LUC_E_INVALID, "max_pos %d < 1", a.max_pos);
-  if ((a.rows && (!a.q || !a.k || !a.v || !a.q_out || !a.positions || !a.slots)) || !a.cos_t || !a.sin_t ||
-      !a.k_pool || !a.v_pool)
-    return fail(LUC_E_INVALID, "null q, k, v, q_out, rope table, positions, slots or pool");
-  if (!a.q_norm != !a.k_norm) return fail(LUC_E_INVALID, "one of q_norm and k_norm without the other");
-  // (a row of q, k and v each starts 16-byte loads)
-  const int q_row = a.hq * head_dim, kv_row = a.hkv * head_dim;
-  if (a.row_stride < q_row || a.q_out_stride < q_row ||
-      ((a.k_out || a.v_out) && a.kv_out_stride < kv_row))
-    return fail(LUC_E_INVALID, "row stride smaller than a row (%d, %d)", q_row, kv_row);
-  if (a.row_stride % 8 || a.q_out_stride % 8 || ((a.k_out || a.v_out) && a.kv_out_stride % 8))
-    return fail(LUC_E_INVALID, "row strides must be multiples of 8 elements");
-  for (const void* p : {a.q, a.k, a.v, a.q_bias, a.k_bias, a.v_bias, a.q_norm, a.k_norm, (const void*)a.cos_t,
-                        (const void*)a.sin_t, (const void*)a.q_out, (const void*)a.k_out, (const void*)a.v_out,
-                        (const void*)a.k_pool, (const void*)a.v_pool})
-    if (!aligned(p, 16)) return fail(LUC_E_INVALID, "operands must be 16-byte aligned");
-  if (!aligned(a.slots, 8) || !aligned(a.positions, 4))
-    return fail(LUC_E_INVALID, "slots must be 8-byte aligned, positions 4-byte");
-  a.num_slots = (int64_t)num_blocks * LUC_BLOCK_SIZE;
+  if (int rc = check_append(ctx, dtype, a, num_blocks, head_dim, block_size)) return rc;
   if (a.rows == 0) return LUC_OK;
   if (int rc = check_device(ctx)) return rc;
   hipFunction_t fn;
@@ -184,7 +112,6 @@ constexpr int kColsOf64 = 128, kColsOf128 = 256;
 //   4 x 1531..2048 rows, 14 and 2 of 64: 67 at 1024, 47.6 whole (the rule's)
 constexpr int kColsMinSplit64 = 512, kColsMinSplit128 = 256, kColsMaxSplits = 32;
 constexpr int64_t kMaxArrivals = 1 << 16;     // (sequence, kv head, column tile)
-constexpr int kMaxCtx = 1 << 30;
 
 struct Kv4Plan {
   bool tokens = false;  // waves split tokens, else columns
@@ -236,6 +163,50 @@ size_t kv4_workspace_bytes(const Kv4Plan& p, int batch, int total_rows, int hkv,
 }  // namespace
 
 namespace luc_internal {
+int check_sizes(const luc_ctx* ctx, int dtype, int hq, int hkv, int head_dim, int block_size, int layer,
+                int num_layers, int num_blocks) {
+  if (!ctx) return fail(LUC_E_INVALID, "null context");
+  if (dtype != LUC_BF16 && dtype != LUC_F16) return fail(LUC_E_INVALID, "bad dtype %d", dtype);
+  if (head_dim != 64 && head_dim != 128)
+    return fail(LUC_E_UNSUPPORTED, "unsupported head_dim %d (64 or 128)", head_dim);
+  if (hq <= 0 || hkv <= 0) return fail(LUC_E_INVALID, "head counts must be positive");
+  if (hq > kMaxHeads) return fail(LUC_E_INVALID, "num_q_heads %d above %d", hq, kMaxHeads);
+  if (hq % hkv) return fail(LUC_E_INVALID, "num_q_heads %d not a multiple of num_kv_heads %d", hq, hkv);
+  if (hq / hkv > 8) return fail(LUC_E_UNSUPPORTED, "group size %d > 8", hq / hkv);
+  if (block_size != LUC_BLOCK_SIZE)
+    return fail(LUC_E_UNSUPPORTED, "block_size %d (only %d)", block_size, LUC_BLOCK_SIZE);
+  if (num_layers <= 0 || layer < 0 || layer >= num_layers)
+    return fail(LUC_E_INVALID, "layer %d outside [0, %d)", layer, num_layers);
+  if (num_blocks < 1) return fail(LUC_E_INVALID, "num_blocks %d < 1", num_blocks);
+  return LUC_OK;
+}
+
+int check_append(const luc_ctx* ctx, int dtype, NormAppendArgs& a, int num_blocks, int head_dim, int block_size) {
+  if (int rc = check_sizes(ctx, dtype, a.hq, a.hkv, head_dim, block_size, a.layer, a.num_layers, num_blocks))
+    return rc;
+  if (a.rows < 0) return fail(LUC_E_INVALID, "num_tokens %d < 0", a.rows);
+  if (a.max_pos < 1) return fail(LUC_E_INVALID, "max_pos %d < 1", a.max_pos);
+  if ((a.rows && (!a.q || !a.k || !a.v || !a.q_out || !a.positions || !a.slots)) || !a.cos_t || !a.sin_t ||
+      !a.k_pool || !a.v_pool)
+    return fail(LUC_E_INVALID, "null q, k, v, q_out, rope table, positions, slots or pool");
+  if (!a.q_norm != !a.k_norm) return fail(LUC_E_INVALID, "one of q_norm and k_norm without the other");
+  // (a row of q, k and v each starts 16-byte loads)
+  const int q_row = a.hq * head_dim, kv_row = a.hkv * head_dim;
+  if (a.row_stride < q_row || a.q_out_stride < q_row ||
+      ((a.k_out || a.v_out) && a.kv_out_stride < kv_row))
+    return fail(LUC_E_INVALID, "row stride smaller than a row (%d, %d)", q_row, kv_row);
+  if (a.row_stride % 8 || a.q_out_stride % 8 || ((a.k_out || a.v_out) && a.kv_out_stride % 8))
+    return fail(LUC_E_INVALID, "row strides must be multiples of 8 elements");
+  for (const void* p : {a.q, a.k, a.v, a.q_bias, a.k_bias, a.v_bias, a.q_norm, a.k_norm, (const void*)a.cos_t,
+                        (const void*)a.sin_t, (const void*)a.q_out, (const void*)a.k_out, (const void*)a.v_out,
+                        (const void*)a.k_pool, (const void*)a.v_pool})
+    if (!aligned(p, 16)) return fail(LUC_E_INVALID, "operands must be 16-byte aligned");
+  if (!aligned(a.slots, 8) || !aligned(a.positions, 4))
+    return fail(LUC_E_INVALID, "slots must be 8-byte aligned, positions 4-byte");
+  a.num_slots = (int64_t)num_blocks * LUC_BLOCK_SIZE;
+  return LUC_OK;
+}
+
 std::vector<std::string> kv4_kernel_names() {
   std::vector<std::string> names = {"luc_block_extend", "luc_block_truncate"};
   for (const char* dt : {"bf16", "f16"})

@@ -84,6 +84,22 @@ SIGNATURES = {
     "luc_kv4_attention": (_i32, [_vp, _vp, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _i32,
                                  _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
                                  _i32, _f32, _vp, _sz]),
+    "luc_kv8_append": (_i32, [_vp, _vp, _i32, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _f32,
+                              _vp, _vp, _i32, _vp, _vp, _i32, _vp, _i64, _vp, _vp, _vp, _vp, _i32,
+                              _i32, _i32, _i32, _i32, _i32, _i32]),
+    "luc_kv8_read": (_i32, [_vp, _vp, _i32, _vp, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _i32, _i32,
+                            _i32, _i32, _i32, _i32]),
+    "luc_kv8_workspace_size": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "luc_kv8_attention": (_i32, [_vp, _vp, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i32,
+                                 _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
+                                 _i32, _i32, _f32, _vp, _sz]),
+    "luc_kv8_sparse_workspace_size": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "luc_kv8_select": (_i32, [_vp, _vp, _i32, _vp, _i32, _i32, _i32, _vp, _i64, _vp, _vp, _vp, _i32,
+                              _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
+                              _vp, _sz]),
+    "luc_kv8_sparse_attention": (_i32, [_vp, _vp, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp,
+                                        _i32, _i32, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _i32,
+                                        _i32, _i32, _i32, _i32, _i32, _f32, _vp, _sz]),
     "luc_blocks_create": (_i32, [_i32, _i32, _i32, ctypes.POINTER(_vp)]),
     "luc_blocks_destroy": (None, [_vp]),
     "luc_blocks_reserve": (_i32, [_vp, _i32, _i32]),
@@ -547,6 +563,148 @@ class LucAttn:
             arr("start_pos", start_pos, i32, dev, batch), batch, total_rows, max_rows, max_ctx, layer, num_layers,
             hq, hkv, head_dim, block_size, sm_scale, ws,
             0 if ws is None else workspace.numel() * workspace.element_size()))
+
+    def _kv8_pools(self, k_pool, v_pool, scales, num_layers, hkv, head_dim, num_blocks, dev):
+        """(k address, v address, scales address, pages) of 8-bit pools: uint8 [pages, layers, kv heads,
+        16 * head_dim], scales float32 [pages, layers, kv heads, 2]."""
+        shape = k_pool.shape
+        if len(shape) != 4 or shape[1:] != (num_layers, hkv, 16 * head_dim) or v_pool.shape != shape:
+            raise ValueError(f"8-bit pools {tuple(shape)}, {tuple(v_pool.shape)}: want [pages, {num_layers}, {hkv}, "
+                             f"{16 * head_dim}]")
+        if scales.shape != (*shape[:3], 2):
+            raise ValueError(f"scales {tuple(scales.shape)}: want {(*shape[:3], 2)}")
+        return (self._array("k_pool", k_pool, torch.uint8, dev, 0), self._array("v_pool", v_pool, torch.uint8, dev, 0),
+                self._array("scales", scales, torch.float32, dev, 0), self._pages_of(shape[0], num_blocks))
+
+    @staticmethod
+    def _pages_of(pages, num_blocks):
+        if num_blocks is None:
+            return pages
+        if num_blocks > pages:
+            raise ValueError(f"num_blocks {num_blocks}: the pools hold {pages} pages")
+        return num_blocks
+
+    def _bounds(self, bounds, pages, num_layers, hkv, head_dim, dev):
+        want = (pages, num_layers, hkv, 2, head_dim)
+        if bounds.shape != want:
+            raise ValueError(f"bounds {tuple(bounds.shape)}: want {want}")
+        return self._array("bounds", bounds, torch.uint8, dev, 0)
+
+    def kv8_append(self, q, k, v, cos, sin, positions, slots, k_pool, v_pool, scales, layer, num_layers, hq, hkv,
+                   head_dim, bounds=None, q_norm=None, k_norm=None, eps=1e-6, q_bias=None, k_bias=None,
+                   v_bias=None, q_out=None, block_size=16, stream=None, num_blocks=None):
+        """luc_kv8_append: qk_norm_rope_append into 8-bit pools (uint8 [pages, layers, kv heads, 16 *
+        head_dim]) with their scales (float32 [pages, layers, kv heads, 2]) and, if given, key bounds
+        (uint8 [pages, layers, kv heads, 2, head_dim]).  The rows of a page follow one another, as
+        block_extend's do."""
+        args, rows, dtype, dev = self._append_args(q, k, v, cos, sin, positions, slots, hq, hkv, head_dim,
+                                                   q_norm, k_norm, eps, q_bias, k_bias, v_bias, q_out, stream)
+        kp, vp, sp, pages = self._kv8_pools(k_pool, v_pool, scales, num_layers, hkv, head_dim, num_blocks, dev)
+        bp = bounds if bounds is None else self._bounds(bounds, k_pool.shape[0], num_layers, hkv, head_dim, dev)
+        self._check(self.lib.luc_kv8_append(*args, kp, vp, sp, bp, pages, layer, num_layers, hq, hkv, head_dim,
+                                            block_size))
+
+    def kv8_read(self, k_out, v_out, slots, k_pool, v_pool, scales, layer, num_layers, hkv, head_dim,
+                 block_size=16, stream=None, num_blocks=None):
+        """luc_kv8_read: the tokens of `slots` (int64) to k_out and v_out [rows, hkv * d] (with one row stride)."""
+        dtype, dev, width = k_out.dtype, self.device, hkv * head_dim
+        rows, stride = own = self._rows("k_out", k_out, width, head_dim, dtype, dev)
+        if self._rows("v_out", v_out, width, head_dim, dtype, dev) != own:
+            raise ValueError("v_out's rows or their stride differ from k_out's")
+        kp, vp, sp, pages = self._kv8_pools(k_pool, v_pool, scales, num_layers, hkv, head_dim, num_blocks, dev)
+        self._check(self.lib.luc_kv8_read(
+            self.ctx, _stream(stream), dtype_code(k_out), k_out.data_ptr(), v_out.data_ptr(), stride,
+            self._array("slots", slots, torch.int64, dev, rows), rows, kp, vp, sp, pages, layer, num_layers, hkv,
+            head_dim, block_size))
+
+    def _zeros(self, need, device):
+        if need == 0:
+            return None
+        return torch.zeros(need // 4, dtype=torch.float32,
+                           device=device if device is not None else f"cuda:{self.device}")
+
+    def kv8_workspace(self, batch, total_rows, max_rows, max_ctx, hq, hkv, head_dim, device=None):
+        """A workspace for kv8_attention calls of these sizes, zero-filled on the current stream (None: none
+        needed)."""
+        return self._zeros(self.lib.luc_kv8_workspace_size(batch, total_rows, max_rows, max_ctx, hq, hkv, head_dim),
+                           device)
+
+    def kv8_sparse_workspace(self, batch, max_ctx, budget, hq, hkv, head_dim, device=None):
+        """The same for kv8_select and kv8_sparse_attention."""
+        return self._zeros(self.lib.luc_kv8_sparse_workspace_size(batch, max_ctx, budget, hq, hkv, head_dim), device)
+
+    def _batch_args(self, tables, start_pos, cu_seqlens, batch, dev):
+        arr, i32, stride = self._array, torch.int32, tables.shape[-1]
+        return (arr("tables", tables, i32, dev, batch * stride), stride,
+                cu_seqlens if cu_seqlens is None else arr("cu_seqlens", cu_seqlens, i32, dev, batch + 1),
+                arr("start_pos", start_pos, i32, dev, batch))
+
+    def _workspace_args(self, workspace, dev):
+        if workspace is None:
+            return None, 0
+        return (self._array("workspace", workspace, workspace.dtype, dev, 0),
+                workspace.numel() * workspace.element_size())
+
+    def kv8_attention(self, out, q, k_pool, v_pool, scales, tables, start_pos, batch, total_rows, max_rows,
+                      max_ctx, layer, num_layers, hq, hkv, head_dim, sm_scale, cu_seqlens=None,
+                      workspace=None, block_size=16, stream=None, num_blocks=None):
+        """luc_kv8_attention: kv4_attention over 8-bit pools and their scales; workspace from kv8_workspace."""
+        dtype, dev = q.dtype, self.device
+        rows, q_stride = self._rows("q", q, hq * head_dim, head_dim, dtype, dev)
+        o_rows, o_stride = self._rows("out", out, hq * head_dim, head_dim, dtype, dev)
+        if rows < total_rows or o_rows < total_rows:
+            raise ValueError(f"q and out have {rows} and {o_rows} rows, fewer than total_rows {total_rows}")
+        kp, vp, sp, pages = self._kv8_pools(k_pool, v_pool, scales, num_layers, hkv, head_dim, num_blocks, dev)
+        tp, stride, cu, start = self._batch_args(tables, start_pos, cu_seqlens, batch, dev)
+        self._check(self.lib.luc_kv8_attention(
+            self.ctx, _stream(stream), dtype_code(q), out.data_ptr(), o_stride, q.data_ptr(), q_stride, kp, vp, sp,
+            tp, stride, pages, cu, start, batch, total_rows, max_rows, max_ctx, layer, num_layers, hq, hkv, head_dim,
+            block_size, sm_scale, *self._workspace_args(workspace, dev)))
+
+    def _chosen(self, pages, batch, hkv, dev):
+        """(address, budget) of pages int32 [batch, hkv, budget]."""
+        if pages.dim() != 3 or pages.shape[:2] != (batch, hkv):
+            raise ValueError(f"pages {tuple(pages.shape)}: want [{batch}, {hkv}, budget]")
+        return self._array("pages", pages, torch.int32, dev, 0), pages.shape[2]
+
+    def kv8_select(self, pages, q, bounds, scales, tables, start_pos, batch, max_ctx, first, recent, layer,
+                   num_layers, hq, hkv, head_dim, cu_seqlens=None, workspace=None, block_size=16, stream=None,
+                   num_blocks=None):
+        """luc_kv8_select: into pages (int32 [batch, hkv, budget]) the pages that the rows q [rows, hq * d], at most
+        one a sequence, attend to; bounds and scales of the pools; workspace from kv8_sparse_workspace."""
+        dev = self.device
+        rows, q_stride = self._rows("q", q, hq * head_dim, head_dim, q.dtype, dev)
+        if cu_seqlens is None and rows < batch:
+            raise ValueError(f"q has {rows} rows, fewer than the batch's {batch}")
+        if scales.dim() != 4 or scales.shape[1:] != (num_layers, hkv, 2):
+            raise ValueError(f"scales {tuple(scales.shape)}: want [pages, {num_layers}, {hkv}, 2]")
+        bp = self._bounds(bounds, scales.shape[0], num_layers, hkv, head_dim, dev)
+        sp = self._array("scales", scales, torch.float32, dev, 0)
+        cp, budget = self._chosen(pages, batch, hkv, dev)
+        tp, stride, cu, start = self._batch_args(tables, start_pos, cu_seqlens, batch, dev)
+        self._check(self.lib.luc_kv8_select(
+            self.ctx, _stream(stream), dtype_code(q), cp, budget, first, recent, q.data_ptr(), q_stride, bp, sp, tp,
+            stride, self._pages_of(scales.shape[0], num_blocks), cu, start, batch,
+            batch if cu_seqlens is None else rows, max_ctx, layer, num_layers, hq, hkv, head_dim, block_size,
+            *self._workspace_args(workspace, dev)))
+
+    def kv8_sparse_attention(self, out, q, k_pool, v_pool, scales, tables, start_pos, pages, batch, max_ctx, layer,
+                             num_layers, hq, hkv, head_dim, sm_scale, cu_seqlens=None, workspace=None,
+                             block_size=16, stream=None, num_blocks=None):
+        """luc_kv8_sparse_attention: attention of out and q's rows, at most one a sequence, over the pages that
+        kv8_select wrote."""
+        dtype, dev = q.dtype, self.device
+        rows, q_stride = self._rows("q", q, hq * head_dim, head_dim, dtype, dev)
+        o_rows, o_stride = self._rows("out", out, hq * head_dim, head_dim, dtype, dev)
+        if o_rows < rows or cu_seqlens is None and rows < batch:
+            raise ValueError(f"q and out have {rows} and {o_rows} rows for a batch of {batch}")
+        kp, vp, sp, blocks = self._kv8_pools(k_pool, v_pool, scales, num_layers, hkv, head_dim, num_blocks, dev)
+        cp, budget = self._chosen(pages, batch, hkv, dev)
+        tp, stride, cu, start = self._batch_args(tables, start_pos, cu_seqlens, batch, dev)
+        self._check(self.lib.luc_kv8_sparse_attention(
+            self.ctx, _stream(stream), dtype_code(q), out.data_ptr(), o_stride, q.data_ptr(), q_stride, kp, vp, sp,
+            tp, stride, blocks, cp, budget, cu, start, batch, batch if cu_seqlens is None else rows, max_ctx, layer,
+            num_layers, hq, hkv, head_dim, block_size, sm_scale, *self._workspace_args(workspace, dev)))
 
     def gather_floor(self, k_pool, v_pool, tables, positions, batch, max_ctx, layer, num_layers,
                      hkv, head_dim, sink, stream=None):
