@@ -8,7 +8,7 @@ gfx950 code objects it loads.  This package binds it for Python callers:
 * ``engine``  -- the reference engine's host-side API for this path
   (RopeCache, KVCache, apply_rope, apply_flash_decoding), written over the
   binding, plus batched forms, page tables held on the GPU (DeviceBlocks) and
-  a 4-bit cache over them (Kv4Cache).
+  caches of 8 and 4 bits over them (Kv8Cache, Kv4Cache).
 
 There is no fallback: if the library is missing or fails to load, every call
 raises.
@@ -19,6 +19,7 @@ from .engine import (  # noqa: F401
     KVCache,
     DeviceBlocks,
     Kv4Cache,
+    Kv8Cache,
     apply_rope,
     apply_flash_decoding,
     decode_step,

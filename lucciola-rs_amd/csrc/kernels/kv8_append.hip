@@ -7,10 +7,10 @@
 // codes that it holds are rounded again, and its bounds with them (rounding keeps order, so the bounds stay those
 // of the codes).
 //
-// Runs.  Rows of one page follow one another with ascending slots.  A wave has one run of K or of V of one head: the
+// Runs.  The rows of one page lie within kAppendReach successive rows.  A wave has one run of K or of V of one head: the
 // rows that go to one page, up to 16, D / 16 lanes a row.  Its extremes are a reduction of the wave; the codes
 // take their places by way of LDS, and 16 bytes a lane go out side by side.  A wave is launched for every
-// row, and those of rows that do not begin a run end at once.
+// row, and those whose page an earlier row has end at once.
 #include "append_row.h"
 #include "kv8.h"
 
@@ -22,6 +22,7 @@ struct Kv8AppendArgs : NormAppendArgs {  // (k_out, v_out unused)
 };
 
 constexpr int kAppendWaves = 4;
+constexpr int kAppendReach = 32;  // (a wave sees as many rows before its own, and behind it)
 
 template <int DT, int D>
 __device__ void kv8_append_impl(const Kv8AppendArgs& A) {
@@ -52,24 +53,33 @@ __device__ void kv8_append_impl(const Kv8AppendArgs& A) {
   if (unit >= 2u * A.hkv * A.rows) return;
   const int row = unit % A.rows;
   const int hh = unit / A.rows % A.hkv, is_v = unit / A.rows / A.hkv;
-  // lane i: row row - 1 + i; rows without a position or a slot belong to no run
+  // lane i: row row - 31 + i; rows without a position or a slot belong to no run
+  constexpr int SELF = kAppendReach - 1;
   int64_t slot = -1;
   int pos = -1;
-  const int at = row - 1 + lane;
-  if (lane <= 16 && at >= 0 && at < A.rows) {
+  const int at = row - SELF + lane;
+  if (at >= 0 && at < A.rows) {
     slot = A.slots[at];
     pos = A.positions[at];
     if (pos < 0 || pos >= A.max_pos || slot < 0 || slot >= A.num_slots) slot = -1;
   }
-  const int64_t first = __shfl(slot, 1), before = __shfl(slot, 0);
-  const int off = (int)(first & (kPage - 1));
-  if (first < 0 || (off && before == first - 1)) return;
-  const uint64_t in = __ballot(lane >= 1 && slot == first + (lane - 1) && off + lane - 1 < kPage);
-  const int len = __builtin_ctzll(~(in >> 1));
+  const int64_t first = __shfl(slot, SELF);
+  if (first < 0) return;
+  const bool member = slot >= 0 && slot >> 4 == first >> 4;
+  const uint64_t in = __ballot(member);
+  if (in & ((1ull << SELF) - 1)) return;  // an earlier row begins the run
+  const int len = min(__builtin_popcountll(in), kPage);
+  // lane j < len: the j'th row of the run (of 64 lanes from SELF on), and the page's tokens that are new
+  const int rank = member ? __builtin_popcountll(in & (lane ? ~0ull >> (64 - lane) : 0ull)) : 63;
+  const int run = __builtin_amdgcn_ds_permute(min(rank, 63) * 4, lane);
+  uint32_t tokens = member ? 1u << (int)(slot & (kPage - 1)) : 0u;
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) tokens |= (uint32_t)__shfl_xor((int)tokens, k);
+  const bool joins = !(tokens & 1);  // what the page holds
   const int64_t head = ((first >> 4) * A.num_layers + A.layer) * A.hkv + hh;
   uint8_t* const slab = (uint8_t*)(is_v ? A.v_pool : A.k_pool) + head * Kv8<D>::kSlab;
   float* const scale_at = A.scales + head * 2 + is_v;
-  const int held = off ? max(exp2of(*scale_at), kKv8LeastExp) : kKv8LeastExp;
+  const int held = joins ? max(exp2of(*scale_at), kKv8LeastExp) : kKv8LeastExp;
   // new tokens of the lane's chunks, a mask of bytes; where some bytes stay, they are read first
   uint32_t fresh[CHUNKS];
   uint4 old[CHUNKS];
@@ -80,11 +90,10 @@ __device__ void kv8_append_impl(const Kv8AppendArgs& A) {
       fresh[i] = 0;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int t = b / (4 * D) * 4 + k;
-        if (t >= off && t < off + len) fresh[i] |= 0xffu << (8 * k);
+        if (tokens >> (b / (4 * D) * 4 + k) & 1) fresh[i] |= 0xffu << (8 * k);
       }
     } else {
-      fresh[i] = b / D >= off && b / D < off + len ? ~0u : 0u;
+      fresh[i] = tokens >> (b / D) & 1 ? ~0u : 0u;
     }
     old[i] = make_uint4(0, 0, 0, 0);
     if (fresh[i] != 0 && fresh[i] != ~0u) old[i] = *(const uint4*)(slab + b);
@@ -92,13 +101,16 @@ __device__ void kv8_append_impl(const Kv8AppendArgs& A) {
   // ---- the rows' values, in 16 bits and back
   const int c = lane % LANES, kind = 1 + is_v;
   float x[PASSES][16];
+  int place[PASSES];  // of the lane's row in the page
   float top = 0.0f;
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
     const int j = p * ROWS + lane / LANES;
-    const int pj = __shfl(pos, j + 1);
+    const int from = __shfl(run, j);
+    const int pj = __shfl(pos, from);
+    place[p] = (int)(__shfl((int)(slot & (kPage - 1)), from));
     if (j >= len) continue;
-    append_head<DT, D>(A, kind, row + j, hh, c, pj, x[p]);
+    append_head<DT, D>(A, kind, row - SELF + from, hh, c, pj, x[p]);
     const uint4 a = pack8<DT>(x[p]), b = pack8<DT>(x[p] + 8);
     unpack8<DT>(a, x[p]);
     unpack8<DT>(b, x[p] + 8);
@@ -111,12 +123,12 @@ __device__ void kv8_append_impl(const Kv8AppendArgs& A) {
   }
   const int e = max(kv8_exponent(wave_max(top)), held);
   const float up = pow2f(-e), less = pow2f(held - e);
-  const bool grown = off && e != held;
+  const bool grown = joins && e != held;
   // ---- codes by way of LDS
   uint8_t* const image = s_image[w];
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
-    const int j = p * ROWS + lane / LANES, t = off + j;
+    const int j = p * ROWS + lane / LANES, t = place[p];
     if (j >= len) continue;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -173,12 +185,12 @@ __device__ void kv8_append_impl(const Kv8AppendArgs& A) {
       lo[k] = fminf(lo[k], __builtin_isnan(yb[k]) ? 0.0f : yb[k] * f);
     }
   };
-  if (off && set == 0)  // (rounded again, as the codes are)
+  if (joins && set == 0)  // (rounded again, as the codes are)
     take(kv8_rescale4(*(const uint32_t*)bound, less), kv8_rescale4(*(const uint32_t*)(bound + D), less), 1.0f);
 #pragma unroll
   for (int t0 = 0; t0 < kPage; t0 += SETS) {
     const int t = t0 + set;
-    if (t < off || t >= off + len) continue;
+    if (!(tokens >> t & 1)) continue;
     const uint32_t y = *(const uint32_t*)(image + Kv8<D>::k_at(t, 4 * quad));
     take(y, y, 1.0f);
   }

@@ -252,14 +252,14 @@ int luc_kv8_append(luc_ctx* ctx, void* stream, int dtype, const void* q, const v
   if (int rc = check_pools(k_pool, v_pool, scales, num_layers, num_kv_heads, head_dim)) return rc;
   if (!aligned(bounds, 16)) return fail(LUC_E_INVALID, "bounds must be 16-byte aligned");
   if (num_tokens == 0) return LUC_OK;
-  if (int rc = check_device(ctx)) return rc;
-  hipFunction_t fn;
-  if (int rc = get_fn(ctx, std::string("luc_kv8_append_") + dt_name(dtype) + "_d" + std::to_string(head_dim), &fn))
-    return rc;
   // q: head_dim / 16 lanes a head; then a wave for every row's k and v heads
   const int64_t grid = ceil_div((int64_t)num_tokens * num_q_heads, 4096 / head_dim) +
                        ceil_div((int64_t)num_tokens * num_kv_heads * 2, 4);
   if (grid * 256 > UINT32_MAX) return fail(LUC_E_INVALID, "too many rows for one launch");
+  if (int rc = check_device(ctx)) return rc;
+  hipFunction_t fn;
+  if (int rc = get_fn(ctx, std::string("luc_kv8_append_") + dt_name(dtype) + "_d" + std::to_string(head_dim), &fn))
+    return rc;
   void* args[] = {&a};
   return launch(fn, dim3((unsigned)grid), dim3(256), stream, args);
 }

@@ -10,8 +10,8 @@ Mirrors, with the same names, argument meaning and error behaviour:
                               src/kernels.rs:248-320
 
 and adds the batched forms the kernels are built for (``decode_step``), page
-tables that live on the GPU (``DeviceBlocks``) and a 4-bit cache over them
-(``Kv4Cache``).
+tables that live on the GPU (``DeviceBlocks``) and caches of 8 and 4 bits over
+them (``Kv8Cache``, ``Kv4Cache``).
 Device memory comes from torch; every launch goes through liblucattn.so.
 """
 from __future__ import annotations
@@ -294,14 +294,12 @@ class DeviceBlocks:
         return int(self.state[0].item())
 
 
-class Kv4Cache:
-    """A 4-bit paged cache of up to `max_seqs` sequences (pools of luc_kv4_append, 0.31 of the
-    bytes of 16 bits) and the DeviceBlocks behind it.  A step: `extend`, then `append` and
-    `attend` for every layer; all of it may be captured in a HIP graph, and so may `truncate`.
-    Calls, and replays of captured ones, must be in one stream's order: they share a workspace."""
+class _QuantCache:
+    """Pools of a quantised cache of up to `max_seqs` sequences, the DeviceBlocks behind them and the
+    workspace of their attention.  `slab`: bytes of a page's K or V of one head, by dimension."""
 
-    def __init__(self, num_layers, num_q_heads, num_kv_heads, head_dim, num_physical_blocks,
-                 max_seqs, max_position_embeddings, max_rows=None, device="cuda", lib=None):
+    def __init__(self, slab, num_layers, num_q_heads, num_kv_heads, head_dim, num_physical_blocks,
+                 max_seqs, max_position_embeddings, max_rows, device, lib):
         self.lib = _lib(lib)
         if head_dim not in (64, 128):
             raise library.LucError(-2, f"Unsupported head dimension for attention kernel: {head_dim}")
@@ -311,7 +309,7 @@ class Kv4Cache:
         self.max_seq_len = max_position_embeddings
         self.blocks = DeviceBlocks(num_physical_blocks, max_seqs, ceil_div(max_position_embeddings, BLOCK_SIZE),
                                    max_rows or max_seqs, device, self.lib)
-        shape = (num_physical_blocks, num_layers, num_kv_heads, 10 * head_dim)
+        shape = (num_physical_blocks, num_layers, num_kv_heads, slab * head_dim)
         self.k_pool = torch.zeros(shape, dtype=torch.uint8, device=device)
         self.v_pool = torch.zeros(shape, dtype=torch.uint8, device=device)
         self._workspace = None
@@ -323,17 +321,9 @@ class Kv4Cache:
     def truncate(self, keep, stream=None):
         self.blocks.truncate(keep, stream)
 
-    def append(self, layer, q, k, v, rope, q_bias=None, k_bias=None, v_bias=None, q_norm=None, k_norm=None,
-               eps=1e-6, q_out=None, k_out=None, v_out=None, stream=None):
-        """Biases, head norms, RoPE and the cache write of the step's rows q [rows, Hq * d], k and v
-        [rows, Hkv * d] in `layer` (luc_kv4_append); q_out (default: q itself) gets q.  At most the
-        `rows` that the step's `extend` was given."""
-        b = self.blocks
-        if q.shape[0] > b.rows:
-            raise ValueError(f"{q.shape[0]} rows to append: the step has {b.rows}")
-        self.lib.kv4_append(q, k, v, rope.cos, rope.sin, b.positions, b.slots, self.k_pool, self.v_pool, layer,
-                            self.num_layers, self.num_q_heads, self.num_kv_heads, self.head_dim, q_norm, k_norm,
-                            eps, q_bias, k_bias, v_bias, q_out, k_out, v_out, stream=stream)
+    def _step_rows(self, q):
+        if q.shape[0] > self.blocks.rows:
+            raise ValueError(f"{q.shape[0]} rows to append: the step has {self.blocks.rows}")
 
     @staticmethod
     def _capturing(stream):
@@ -342,20 +332,16 @@ class Kv4Cache:
         with torch.cuda.stream(stream):
             return torch.cuda.is_current_stream_capturing()
 
-    def workspace(self, total_rows, max_rows, max_ctx, stream=None):
-        """The zero-filled workspace of `attend`, grown on demand by half at least (None: none needed).  Ask
-        for it before a capture that needs a larger one than there is.  A smaller one that it takes the
-        place of is freed, unless it was handed out during a capture (by `attend`; a program that captures
-        launches of its own on one holds it itself)."""
-        need = self.lib.lib.luc_kv4_workspace_size(self.blocks.max_seqs, total_rows, max_rows, max_ctx,
-                                                   self.num_q_heads, self.num_kv_heads, self.head_dim)
+    def _grown(self, need, stream):
+        """The workspace, of at least `need` bytes; None for 0."""
         if need == 0:
             return None
         capturing = self._capturing(stream)
         old = self._workspace
         if old is None or old.numel() * 4 < need:
             if capturing:
-                raise RuntimeError(f"Kv4Cache: a workspace of {need} bytes must be made before the capture")
+                raise RuntimeError(f"{type(self).__name__}: a workspace of {need} bytes must be made before the "
+                                   "capture")
             size = need // 4 if old is None else max(need // 4, old.numel() * 3 // 2)
             with torch.cuda.stream(stream):  # (None: the current one) filled in the launch's order
                 self._workspace = torch.zeros(size, dtype=torch.float32, device=self.k_pool.device)
@@ -364,6 +350,41 @@ class Kv4Cache:
         if capturing and not any(w is self._workspace for w in self._captured):
             self._captured.append(self._workspace)
         return self._workspace
+
+    def _scale(self, scale):
+        return sm_scale(self.head_dim) if scale is None else scale
+
+
+class Kv4Cache(_QuantCache):
+    """A 4-bit paged cache of up to `max_seqs` sequences (pools of luc_kv4_append, 0.31 of the
+    bytes of 16 bits) and the DeviceBlocks behind it.  A step: `extend`, then `append` and
+    `attend` for every layer; all of it may be captured in a HIP graph, and so may `truncate`.
+    Calls, and replays of captured ones, must be in one stream's order: they share a workspace."""
+
+    def __init__(self, num_layers, num_q_heads, num_kv_heads, head_dim, num_physical_blocks,
+                 max_seqs, max_position_embeddings, max_rows=None, device="cuda", lib=None):
+        super().__init__(10, num_layers, num_q_heads, num_kv_heads, head_dim, num_physical_blocks,
+                         max_seqs, max_position_embeddings, max_rows, device, lib)
+
+    def append(self, layer, q, k, v, rope, q_bias=None, k_bias=None, v_bias=None, q_norm=None, k_norm=None,
+               eps=1e-6, q_out=None, k_out=None, v_out=None, stream=None):
+        """Biases, head norms, RoPE and the cache write of the step's rows q [rows, Hq * d], k and v
+        [rows, Hkv * d] in `layer` (luc_kv4_append); q_out (default: q itself) gets q.  At most the
+        `rows` that the step's `extend` was given."""
+        b = self.blocks
+        self._step_rows(q)
+        self.lib.kv4_append(q, k, v, rope.cos, rope.sin, b.positions, b.slots, self.k_pool, self.v_pool, layer,
+                            self.num_layers, self.num_q_heads, self.num_kv_heads, self.head_dim, q_norm, k_norm,
+                            eps, q_bias, k_bias, v_bias, q_out, k_out, v_out, stream=stream)
+
+    def workspace(self, total_rows, max_rows, max_ctx, stream=None):
+        """The zero-filled workspace of `attend`, grown on demand by half at least (None: none needed).  Ask
+        for it before a capture that needs a larger one than there is.  A smaller one that it takes the
+        place of is freed, unless it was handed out during a capture (by `attend`; a program that captures
+        launches of its own on one holds it itself)."""
+        return self._grown(self.lib.lib.luc_kv4_workspace_size(
+            self.blocks.max_seqs, total_rows, max_rows, max_ctx, self.num_q_heads, self.num_kv_heads,
+            self.head_dim), stream)
 
     def attend(self, layer, out, q, max_ctx, max_rows=None, scale=None, stream=None):
         """Attention of the step's rows (luc_kv4_attention): q and out [rows, Hq * d]; max_ctx and max_rows
@@ -374,9 +395,81 @@ class Kv4Cache:
         max_rows = rows if max_rows is None else max_rows
         self.lib.kv4_attention(out, q, self.k_pool, self.v_pool, b.block_tables, b.start_pos, b.max_seqs, rows,
                                max_rows, max_ctx, layer, self.num_layers, self.num_q_heads, self.num_kv_heads,
-                               self.head_dim, sm_scale(self.head_dim) if scale is None else scale,
-                               cu_seqlens=b.cu_seqlens, workspace=self.workspace(rows, max_rows, max_ctx, stream),
-                               stream=stream)
+                               self.head_dim, self._scale(scale), cu_seqlens=b.cu_seqlens,
+                               workspace=self.workspace(rows, max_rows, max_ctx, stream), stream=stream)
+
+
+class Kv8Cache(_QuantCache):
+    """An 8-bit paged cache of up to `max_seqs` sequences (pools and scales of luc_kv8_append, half the
+    bytes of 16 bits) and the DeviceBlocks behind it: a step as Kv4Cache has it.  With `bounds` (1/16 of the
+    pools more) a step of at most one row a sequence may `attend_sparse`: to the pages of each context that
+    score highest, instead of to all of it.  One that was made without cannot."""
+
+    def __init__(self, num_layers, num_q_heads, num_kv_heads, head_dim, num_physical_blocks,
+                 max_seqs, max_position_embeddings, max_rows=None, bounds=False, device="cuda", lib=None):
+        super().__init__(16, num_layers, num_q_heads, num_kv_heads, head_dim, num_physical_blocks,
+                         max_seqs, max_position_embeddings, max_rows, device, lib)
+        shape = (num_physical_blocks, num_layers, num_kv_heads, 2)
+        self.scales = torch.zeros(shape, dtype=torch.float32, device=device)
+        self.bounds = torch.zeros((*shape, head_dim), dtype=torch.uint8, device=device) if bounds else None
+
+    def append(self, layer, q, k, v, rope, q_bias=None, k_bias=None, v_bias=None, q_norm=None, k_norm=None,
+               eps=1e-6, q_out=None, stream=None):
+        """Biases, head norms, RoPE and the cache write of the step's rows q [rows, Hq * d], k and v
+        [rows, Hkv * d] in `layer` (luc_kv8_append); q_out (default: q itself) gets q.  At most the
+        `rows` that the step's `extend` was given."""
+        b = self.blocks
+        self._step_rows(q)
+        self.lib.kv8_append(q, k, v, rope.cos, rope.sin, b.positions, b.slots, self.k_pool, self.v_pool, self.scales,
+                            layer, self.num_layers, self.num_q_heads, self.num_kv_heads, self.head_dim, self.bounds,
+                            q_norm, k_norm, eps, q_bias, k_bias, v_bias, q_out, stream=stream)
+
+    def read(self, layer, k_out, v_out, slots, stream=None):
+        """K and V of the tokens at `slots` (int64 [rows]: page * 16 + offset) in `layer`, in 16 bits, to k_out
+        and v_out [rows, Hkv * d] (luc_kv8_read)."""
+        self.lib.kv8_read(k_out, v_out, slots, self.k_pool, self.v_pool, self.scales, layer, self.num_layers,
+                          self.num_kv_heads, self.head_dim, stream=stream)
+
+    def workspace(self, total_rows, max_rows, max_ctx, budget=None, stream=None):
+        """The zero-filled workspace of `attend` or, with a budget, of `attend_sparse`, grown on demand by half
+        at least (None: none needed); one serves both.  Ask for it before a capture that needs a larger one than
+        there is, and as Kv4Cache.workspace otherwise."""
+        c, n, h = self.lib.lib, self.blocks.max_seqs, (self.num_q_heads, self.num_kv_heads, self.head_dim)
+        if budget is None:
+            return self._grown(c.luc_kv8_workspace_size(n, total_rows, max_rows, max_ctx, *h), stream)
+        return self._grown(c.luc_kv8_sparse_workspace_size(n, max_ctx, budget, *h), stream)
+
+    def attend(self, layer, out, q, max_ctx, max_rows=None, scale=None, stream=None):
+        """Attention of the step's rows (luc_kv8_attention): q and out [rows, Hq * d]; max_ctx and max_rows
+        (default: all of q's rows) bound a sequence's context, its new rows among it, and its new
+        rows; scale defaults to 1 / sqrt(d)."""
+        b = self.blocks
+        rows = q.shape[0]
+        max_rows = rows if max_rows is None else max_rows
+        self.lib.kv8_attention(out, q, self.k_pool, self.v_pool, self.scales, b.block_tables, b.start_pos, b.max_seqs,
+                               rows, max_rows, max_ctx, layer, self.num_layers, self.num_q_heads, self.num_kv_heads,
+                               self.head_dim, self._scale(scale), cu_seqlens=b.cu_seqlens,
+                               workspace=self.workspace(rows, max_rows, max_ctx, stream=stream), stream=stream)
+
+    def attend_sparse(self, layer, out, q, max_ctx, budget, first=1, recent=2, scale=None, pages=None, stream=None):
+        """Attention of a step with at most one row a sequence over `budget` pages of each context, chosen for
+        every kv head by score (luc_kv8_select, luc_kv8_sparse_attention), the first `first` and the
+        last `recent` always among them; the pages go to `pages` (int32 [max_seqs, Hkv, budget], default: a new
+        tensor) and are returned."""
+        if self.bounds is None:
+            raise ValueError("this cache keeps no key bounds: make it with bounds=True")
+        b, h = self.blocks, (layer, self.num_layers, self.num_q_heads, self.num_kv_heads, self.head_dim)
+        if pages is None:
+            with torch.cuda.stream(stream):  # (None: the current one)
+                pages = torch.empty((b.max_seqs, self.num_kv_heads, budget), dtype=torch.int32,
+                                    device=self.k_pool.device)
+        ws = self.workspace(q.shape[0], 1, max_ctx, budget, stream)
+        self.lib.kv8_select(pages, q, self.bounds, self.scales, b.block_tables, b.start_pos, b.max_seqs, max_ctx,
+                            first, recent, *h, cu_seqlens=b.cu_seqlens, workspace=ws, stream=stream)
+        self.lib.kv8_sparse_attention(out, q, self.k_pool, self.v_pool, self.scales, b.block_tables, b.start_pos,
+                                      pages, b.max_seqs, max_ctx, *h, self._scale(scale), cu_seqlens=b.cu_seqlens,
+                                      workspace=ws, stream=stream)
+        return pages
 
 
 def apply_rope(rope, qkv, q_start_idx, k_start_idx, q_bias, k_bias, pos_ptr, head_dim,
@@ -442,6 +535,6 @@ def ceil_div(a, b):
     return -(-a // b)
 
 
-__all__ = ["RopeCache", "KVCache", "DeviceBlocks", "Kv4Cache", "apply_rope", "apply_flash_decoding",
+__all__ = ["RopeCache", "KVCache", "DeviceBlocks", "Kv4Cache", "Kv8Cache", "apply_rope", "apply_flash_decoding",
            "decode_step", "decode_step_unfused",
            "sm_scale", "BLOCK_SIZE"]

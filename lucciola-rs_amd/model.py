@@ -23,8 +23,10 @@ then h = rmsnorm(h, norm) (models.rs:755-761, 814-820), logits = h @ lm_head^T
 sampling by luc_argmax (models.rs:385-405).
 The q/k biases enter in the RoPE step and the v bias in the cache write, as in
 the reference (models.rs:505-534).
-With kv_bits=4 the cache is a Kv4Cache (0.31 of the bytes): att is then
-luc_kv4_append and luc_kv4_attention, of prompts and single tokens alike.
+With kv_bits=4 or kv_format="e4m3" the cache is a Kv4Cache or a Kv8Cache (0.31 or
+half of the bytes): att is then luc_kv4_append and luc_kv4_attention, or their kv8 forms, of
+prompts and single tokens alike; with sparse_pages, too, single tokens attend to
+that many pages of their context (luc_kv8_select, luc_kv8_sparse_attention).
 
 Weights are bf16 in the reference's fused layout (models.rs:91-155):
 qkv_proj = [q; k; v] rows, qkv_bias likewise (zeros when the checkpoint has
@@ -40,7 +42,7 @@ import numpy as np
 import torch
 
 from . import library
-from .engine import KVCache, Kv4Cache, RopeCache, ceil_div, sm_scale
+from .engine import KVCache, Kv4Cache, Kv8Cache, RopeCache, ceil_div, sm_scale
 
 
 @dataclass(frozen=True)
@@ -146,14 +148,24 @@ class Qwen2Model:
     of luc_prompt_gemm and luc_prompt_mlp on the same weights, or, where
     prompt_kernels_win says so, hipBLASLt GEMMs on their transposes ("*_t": views,
     or contiguous copies where hidden or intermediate is not a multiple of 64).
-    kv_bits: 16, the reference's bf16 cache, or 4."""
+    kv_bits: 16, the reference's bf16 cache, or 4; kv_format "e4m3": 8 bits.  sparse_pages (of an e4m3 cache):
+    the pages of 16 tokens that a single token's row reads of a longer context, the first and the last two
+    among them (0: all)."""
 
     def __init__(self, cfg: Qwen2Config, weights: dict, num_blocks: int | None = None,
-                 max_positions: int | None = None, device="cuda", lib=None, kv_bits: int = 16):
+                 max_positions: int | None = None, device="cuda", lib=None, kv_bits: int = 16,
+                 kv_format: str | None = None, sparse_pages: int = 0):
         if kv_bits not in (4, 16):
-            raise ValueError(f"kv_bits {kv_bits} (4 or 16)")
+            raise ValueError(f"kv_bits {kv_bits} (4 or 16; 8 bits are kv_format \"e4m3\")")
+        if kv_format not in (None, "e4m3") or kv_format and kv_bits != 16:
+            raise ValueError(f"kv_format {kv_format!r} (None or \"e4m3\", in place of kv_bits)")
+        if kv_format:
+            kv_bits = 8
+        if sparse_pages and (kv_bits != 8 or sparse_pages < 3):
+            raise ValueError(f"sparse_pages {sparse_pages}: 3 or more, of an e4m3 cache")
         self.cfg = cfg
         self.kv_bits = kv_bits
+        self.sparse_pages = sparse_pages
         self.lib = lib if lib is not None else library.default(torch.cuda.current_device())
         self.device = torch.device(device)
         d = cfg.head_dim
@@ -193,9 +205,11 @@ class Qwen2Model:
         self.rope = RopeCache(max_pos, d, cfg.rope_theta, cfg.rope_scaling_factor, device=self.device,
                               lib=self.lib)
         blocks = num_blocks or (max_pos + 15) // 16
-        if kv_bits == 4:
-            self.kv = Kv4Cache(cfg.num_hidden_layers, cfg.num_attention_heads, cfg.num_key_value_heads, d,
-                               blocks, 1, max_pos, max_pos, self.device, self.lib)
+        if kv_bits != 16:
+            sizes = (cfg.num_hidden_layers, cfg.num_attention_heads, cfg.num_key_value_heads, d, blocks, 1, max_pos,
+                     max_pos)
+            self.kv = Kv4Cache(*sizes, self.device, self.lib) if kv_bits == 4 else \
+                Kv8Cache(*sizes, bool(sparse_pages), self.device, self.lib)
             self._count = torch.zeros(1, dtype=torch.int32, device=self.device)
             self._one = torch.ones(1, dtype=torch.int32, device=self.device)
         else:
@@ -238,12 +252,12 @@ class Qwen2Model:
                                cfg.num_key_value_heads, cfg.head_dim, sm_scale(cfg.head_dim), att)
         return att
 
-    def _extend4(self, cache_pos, rows):
-        """Pages, slots and positions of `rows` new tokens at cache_pos.. of the 4-bit cache, which
+    def _extend(self, cache_pos, rows):
+        """Pages, slots and positions of `rows` new tokens at cache_pos.. of the 8- or 4-bit cache, which
         forgets what it held from there on."""
         held = int(self.kv.blocks.lens.item())  # (replays of capture_decode's graph change it too)
         if cache_pos > held:
-            raise ValueError(f"position {cache_pos} past the {held} tokens of the 4-bit cache")
+            raise ValueError(f"position {cache_pos} past the {held} tokens of the {self.kv_bits}-bit cache")
         if ceil_div(cache_pos + rows, self.kv.block_size) > self.kv.blocks.num_blocks:
             raise RuntimeError("KVCache: Out of memory blocks")
         if cache_pos < held:
@@ -252,14 +266,17 @@ class Qwen2Model:
         self._count.fill_(rows)
         self.kv.extend(self._count, rows)
 
-    def _attention4(self, li, qkv, max_ctx):
+    def _attention_quant(self, li, qkv, max_ctx):
         cfg = self.cfg
         L = self.layers[li]
         H, kd = cfg.hidden_size, cfg.num_key_value_heads * cfg.head_dim
         q, k, v = qkv[:, :H], qkv[:, H:H + kd], qkv[:, H + kd:]
         self.kv.append(li, q, k, v, self.rope, L["q_bias"], L["k_bias"], L["v_bias"])
         att = torch.empty(qkv.shape[0], H, dtype=torch.bfloat16, device=self.device)
-        self.kv.attend(li, att, q, max_ctx)
+        if self.sparse_pages and qkv.shape[0] == 1:
+            self.kv.attend_sparse(li, att, q, max_ctx, self.sparse_pages)
+        else:
+            self.kv.attend(li, att, q, max_ctx)
         return att
 
     def _layer(self, li, h, attention, out=None):
@@ -330,9 +347,9 @@ class Qwen2Model:
         ids = torch.tensor([int(i) for i in input_ids], dtype=torch.int32, device=self.device)
         h = torch.empty(S, cfg.hidden_size, dtype=torch.bfloat16, device=self.device)
         self.lib.embedding(h, self.embed, ids)
-        if self.kv_bits == 4:
-            self._extend4(cache_pos, S)
-            self._decoder(h, lambda li, qkv: self._attention4(li, qkv, cache_pos + S))
+        if self.kv_bits != 16:
+            self._extend(cache_pos, S)
+            self._decoder(h, lambda li, qkv: self._attention_quant(li, qkv, cache_pos + S))
             return
         # the pages of every position first, and of those before it that no step
         # has reserved (prepare_for_step appends one page a call, whatever the gap)
@@ -394,24 +411,24 @@ class Qwen2Model:
         its pages are taken now, the split-K workspace is sized for it, and the
         attention launches are bounded by it (the kernels read the actual
         position from self.pos).  Set self.idx and self.pos before the first
-        replay.  With a 4-bit cache a replay itself takes the page that its token
+        replay.  With an 8- or 4-bit cache a replay itself takes the page that its token
         opens, and goes back to self.pos first where the cache holds more tokens;
         self.pos must not be past those."""
         cfg = self.cfg
         if max_ctx > self.max_positions:
             raise ValueError(f"max_ctx {max_ctx} exceeds {self.max_positions} positions")
-        if self.kv_bits == 4:
+        if self.kv_bits != 16:
             if ceil_div(max_ctx, self.kv.block_size) > self.kv.blocks.num_blocks:
                 raise RuntimeError("KVCache: Out of memory blocks")
-            self.kv.workspace(1, 1, max_ctx)
+            self.kv.workspace(1, 1, max_ctx, *([self.sparse_pages] if self.sparse_pages else []))
         else:
             for p in range(max_ctx):
                 self.kv.prepare_for_step(p)
             ws = self.kv.workspace(cfg.num_attention_heads, max_ctx)
 
         def attention(li, qkv):
-            if self.kv_bits == 4:
-                return self._attention4(li, qkv, max_ctx)
+            if self.kv_bits != 16:
+                return self._attention_quant(li, qkv, max_ctx)
             L = self.layers[li]
             att = torch.empty(1, cfg.hidden_size, dtype=torch.bfloat16, device=self.device)
             self.lib.decode_step(qkv, L["q_bias"], L["k_bias"], L["v_bias"], self.rope.cos,
@@ -426,7 +443,7 @@ class Qwen2Model:
         with torch.cuda.graph(graph):
             h = torch.empty(1, cfg.hidden_size, dtype=torch.bfloat16, device=self.device)
             self.lib.embedding(h, self.embed, self.idx)
-            if self.kv_bits == 4:
+            if self.kv_bits != 16:
                 self.kv.truncate(self.pos)
                 self.kv.extend(self._one, 1)
             for li in range(cfg.num_hidden_layers - 1):
