@@ -10,7 +10,8 @@
 // Runs.  The rows of one page lie within kAppendReach successive rows.  A wave has one run of K or of V of one head: the
 // rows that go to one page, up to 16, D / 16 lanes a row.  Its extremes are a reduction of the wave; the codes
 // take their places by way of LDS, and 16 bytes a lane go out side by side.  A wave is launched for every
-// row, and those whose page an earlier row has end at once.
+// row, and those whose page an earlier row has end at once; or, of many rows, for every 16, among which it looks for the
+// beginnings of runs.
 #include "append_row.h"
 #include "kv8.h"
 
@@ -19,40 +20,20 @@ namespace luc {
 struct Kv8AppendArgs : NormAppendArgs {  // (k_out, v_out unused)
   float* scales;
   uint8_t* bounds;  // or null
+  int32_t span;     // rows whose runs a wave has: 1 or 16
 };
 
 constexpr int kAppendWaves = 4;
 constexpr int kAppendReach = 32;  // (a wave sees as many rows before its own, and behind it)
 
+// The run that row `row` of a head of k (is_v 0) or v begins, if it does.  image: a slab of LDS, the wave's.
 template <int DT, int D>
-__device__ void kv8_append_impl(const Kv8AppendArgs& A) {
+__device__ __attribute__((always_inline)) inline void append_run(const Kv8AppendArgs& A, int row, int hh, int is_v, uint8_t* image) {
 #pragma clang fp contract(off)
   constexpr int LANES = D / 16;
   constexpr int ROWS = 64 / LANES, PASSES = 16 / ROWS;  // rows of a pass
   constexpr int CHUNKS = D / 64;                        // 16 bytes of a slab a lane
-  __shared__ __attribute__((aligned(16))) uint8_t s_image[kAppendWaves][Kv8<D>::kSlab];
-  const uint32_t nq = (uint32_t)A.rows * A.hq;
-  const uint32_t q_blocks = (nq + 256 / LANES - 1) / (256 / LANES);
-  if (blockIdx.x < q_blocks) {
-    const uint32_t unit = (blockIdx.x * 256 + threadIdx.x) / LANES;
-    const int c = threadIdx.x % LANES;
-    if (unit >= nq) return;
-    const int row = unit / A.hq, hh = unit % A.hq;
-    const int pos = A.positions[row];
-    if (pos < 0 || pos >= A.max_pos) return;
-    float x[16];
-    append_head<DT, D>(A, 0, row, hh, c, pos, x);
-    uint16_t* const o = A.q_out + row * A.q_out_stride + hh * D;
-    *(uint4*)(o + 8 * c) = pack8<DT>(x);
-    *(uint4*)(o + D / 2 + 8 * c) = pack8<DT>(x + 8);
-    return;
-  }
-  // ---- one run of one head of k or v
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const uint32_t unit = (blockIdx.x - q_blocks) * kAppendWaves + w;  // (the grid's threads fit 32 bits)
-  if (unit >= 2u * A.hkv * A.rows) return;
-  const int row = unit % A.rows;
-  const int hh = unit / A.rows % A.hkv, is_v = unit / A.rows / A.hkv;
+  const int lane = threadIdx.x & 63;
   // lane i: row row - 31 + i; rows without a position or a slot belong to no run
   constexpr int SELF = kAppendReach - 1;
   int64_t slot = -1;
@@ -125,7 +106,6 @@ __device__ void kv8_append_impl(const Kv8AppendArgs& A) {
   const float up = pow2f(-e), less = pow2f(held - e);
   const bool grown = joins && e != held;
   // ---- codes by way of LDS
-  uint8_t* const image = s_image[w];
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
     const int j = p * ROWS + lane / LANES, t = place[p];
@@ -204,6 +184,51 @@ __device__ void kv8_append_impl(const Kv8AppendArgs& A) {
   if (set == 0) {
     *(uint32_t*)bound = kv8_encode4(hi[0], hi[1], hi[2], hi[3]);
     *(uint32_t*)(bound + D) = kv8_encode4(lo[0], lo[1], lo[2], lo[3]);
+  }
+}
+
+template <int DT, int D>
+__device__ void kv8_append_impl(const Kv8AppendArgs& A) {
+  constexpr int LANES = D / 16;
+  __shared__ __attribute__((aligned(16))) uint8_t s_image[kAppendWaves][Kv8<D>::kSlab];
+  const uint32_t nq = (uint32_t)A.rows * A.hq;
+  const uint32_t q_blocks = (nq + 256 / LANES - 1) / (256 / LANES);
+  if (blockIdx.x < q_blocks) {
+    const uint32_t unit = (blockIdx.x * 256 + threadIdx.x) / LANES;
+    const int c = threadIdx.x % LANES;
+    if (unit >= nq) return;
+    const int row = unit / A.hq, hh = unit % A.hq;
+    const int pos = A.positions[row];
+    if (pos < 0 || pos >= A.max_pos) return;
+    float x[16];
+    append_head<DT, D>(A, 0, row, hh, c, pos, x);
+    uint16_t* const o = A.q_out + row * A.q_out_stride + hh * D;
+    *(uint4*)(o + 8 * c) = pack8<DT>(x);
+    *(uint4*)(o + D / 2 + 8 * c) = pack8<DT>(x + 8);
+    return;
+  }
+  // ---- the runs of one head of k or v that begin in `span` rows
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const uint32_t spans = ((uint32_t)A.rows + A.span - 1) / A.span;
+  const uint32_t unit = (blockIdx.x - q_blocks) * kAppendWaves + w;  // (the grid's threads fit 32 bits)
+  if (unit >= 2u * A.hkv * spans) return;
+  const int row0 = (int)(unit % spans) * A.span;
+  const int hh = unit / spans % A.hkv, is_v = unit / spans / A.hkv;
+  uint64_t begins = 2;
+  if (A.span > 1) {
+    // lane i: row row0 - 1 + i; one that follows another of its page begins no run
+    const int at = row0 - 1 + lane;
+    const int64_t page = lane <= A.span && at >= 0 && at < A.rows ? A.slots[at] >> 4 : -1;
+    const int64_t before = __shfl_up(page, 1);
+    // (behind a row without a position the page's run may begin)
+    begins = __ballot(lane > 0 && page >= 0 &&
+                      (page != before || at == 0 || A.positions[at - 1] < 0 || A.positions[at - 1] >= A.max_pos));
+  }
+  while (begins) {
+    const int i = __builtin_ctzll(begins);
+    begins &= begins - 1;
+    wave_lds_sync();  // (the image again)
+    append_run<DT, D>(A, row0 - 1 + i, hh, is_v, s_image[w]);
   }
 }
 

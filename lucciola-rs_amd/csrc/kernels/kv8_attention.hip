@@ -119,23 +119,26 @@ __device__ inline float score_scale(const Kv8AttnArgs& A) {
   return s == 0.0f ? 1e-37f : s;  // (a masked product, -inf, times 0 is NaN)
 }
 
-// ---- stages: what a wave loads ahead, 8 KB of 32 (D = 128) or 64 (D = 64) tokens, in operand order:
-// K token n of the page, dimensions 64 h + 16 g .. + 15; V dimensions 64 h + 4 n .. + 3 of tokens 4 g .. 4 g + 3.
+// ---- stages: what a wave takes at once, 8 KB of 32 (D = 128) or 64 (D = 64) tokens, in operand order: K token n of
+// the page, dimensions 64 h + 16 g .. + 15; V dimensions 64 h + 4 n .. + 3 of tokens 4 g .. 4 g + 3.
 template <int D> struct Kv8Stage {
   static constexpr int SUB = D == 128 ? 1 : 2;  // 32-token sub-tiles
   static constexpr int TOKENS = 32 * SUB, PAGES = 2 * SUB, H = D / 64;
-  uint4 k[PAGES][H], v[PAGES][H];
-  float2 scale[PAGES];
 };
+// Numbers that are alike in all lanes come by the scalar cache, past the queue of the cache's own loads.
+typedef __attribute__((address_space(4))) const int32_t scalar_i32;
+typedef __attribute__((address_space(4))) const float scalar_f32;
 
 // One wave's 8 columns over stages.  Of a fragment's 16 columns the lower 8 take the first page's tokens
 // and the upper 8, the same rows and heads again, the second's: a lane has 4 tokens of one column, and
 // softmax costs half of what 16 columns would.  The two halves of a column are partial results
 // like those of two waves.
 template <int DT, int D> struct Kv8Row {
-  static constexpr int KS = D / 32, NF = D / 16, H = D / 64;
+  using Stage = Kv8Stage<D>;
+  static constexpr int KS = D / 32, NF = D / 16, H = D / 64, SUB = Stage::SUB, PAGES = Stage::PAGES;
   uint4 q[KS];
   f32x4_t acc[NF];  // O^T: row 4 g + r of fragment 4 h + c is dimension 64 h + 16 g + 4 r + c
+  float s[SUB][4];  // scores of the stage
   float m, l, scale;  // m: less the lift
   float bar;          // products above it move m
   int limit;
@@ -162,30 +165,41 @@ template <int DT, int D> struct Kv8Row {
     for (int i = 0; i < NF; ++i) acc[i] = (f32x4_t){0, 0, 0, 0};
   }
 
-  // Pages 2 u and 2 u + 1 of a stage: tokens tok0 .. tok0 + 31.
-  __device__ __attribute__((always_inline)) inline void step(const Kv8Stage<D>& T, int u, int tok0, bool edge) {
-    f32x4_t x[2];
+  // Products with a stage's K; sk: its pages' scales.
+  __device__ __attribute__((always_inline)) inline void score(const uint4 (&k)[PAGES][H], const float (&sk)[PAGES]) {
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      x[b] = (f32x4_t){0, 0, 0, 0};
-      const float sk = T.scale[2 * u + b].x;
+    for (int u = 0; u < SUB; ++u) {
+      f32x4_t x[2];
 #pragma unroll
-      for (int h = 0; h < H; ++h) {
-        const uint4 w = T.k[2 * u + b][h];
-        x[b] = mfma16<DT>(expand8<DT>(w.x, w.y, sk), q[2 * h], x[b]);
-        x[b] = mfma16<DT>(expand8<DT>(w.z, w.w, sk), q[2 * h + 1], x[b]);
+      for (int b = 0; b < 2; ++b) {
+        x[b] = (f32x4_t){0, 0, 0, 0};
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          const uint4 w = k[2 * u + b][h];
+          x[b] = mfma16<DT>(expand8<DT>(w.x, w.y, sk[2 * u + b]), q[2 * h], x[b]);
+          x[b] = mfma16<DT>(expand8<DT>(w.z, w.w, sk[2 * u + b]), q[2 * h + 1], x[b]);
+        }
       }
-    }
-    float s[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = mask[0] ? x[0][i] : x[1][i];
-    const int room = limit - tok0 - 4 * g - (mask[0] ? 0 : kPage);  // the lane's tokens up to it are seen
-    if (edge) {
-      asm volatile("" ::: "memory");  // (stays a branch)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] = i <= room ? s[i] : -INFINITY;
+      for (int i = 0; i < 4; ++i) s[u][i] = mask[0] ? x[0][i] : x[1][i];
     }
-    float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+  }
+
+  // The lane's tokens up to this one of sub-tile u are seen (tok0: the stage's first).
+  __device__ inline int room(int tok0, int u) const { return limit - tok0 - 32 * u - 4 * g - (mask[0] ? 0 : kPage); }
+
+  // Softmax and the products with a stage's V; sv: its pages' scales.  EDGE: some column's limit lies before the
+  // stage's last token.
+  template <bool EDGE>
+  __device__ __attribute__((always_inline)) inline void add(const uint4 (&v)[PAGES][H], const float (&sv)[PAGES], int tok0) {
+    if constexpr (EDGE) {
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[u][i] = i <= room(tok0, u) ? s[u][i] : -INFINITY;
+    }
+    float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
+    if constexpr (SUB == 2) top = fmaxf(top, fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
     if (__any(top > bar)) {
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
@@ -197,43 +211,44 @@ template <int DT, int D> struct Kv8Row {
 #pragma unroll
       for (int i = 0; i < NF; ++i) acc[i] *= a;
     }
-    uint32_t p[4];
+    uint4 p[SUB];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float y = __builtin_amdgcn_exp2f(fmaf(s[2 * i], scale, -m));
-      const float z = __builtin_amdgcn_exp2f(fmaf(s[2 * i + 1], scale, -m));
-      const uint32_t w = pack2<DT>(y, z);
-      l = St<DT>::dot2(w, kOnes<DT>, l);
-      p[i] = w & mask[0];
-      p[2 + i] = w & mask[1];
-    }
-    const uint4 pp = make_uint4(p[0], p[1], p[2], p[3]);
-    const float sv0 = T.scale[2 * u].y, sv1 = T.scale[2 * u + 1].y;
+    for (int u = 0; u < SUB; ++u) {
+      uint32_t w[2];
 #pragma unroll
-    for (int h = 0; h < H; ++h) {
-      const uint4 wa = T.v[2 * u][h], wb = T.v[2 * u + 1][h];
-      const uint32_t a[4] = {wa.x, wa.y, wa.z, wa.w}, b[4] = {wb.x, wb.y, wb.z, wb.w};
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint4 vv = make_uint4(kv8_pair<DT, false>(a[c], sv0), kv8_pair<DT, true>(a[c], sv0),
-                              kv8_pair<DT, false>(b[c], sv1), kv8_pair<DT, true>(b[c], sv1));
-        if (edge) {
-          asm volatile("" ::: "memory");
-          const uint4 bad = not_finite4<DT>(vv);
-          if (__any((bad.x | bad.y | bad.z | bad.w) != 0)) {
-            const uint32_t lo = (0 <= room ? kOnes<DT> & 0xffffu : 0u) | (1 <= room ? kOnes<DT> & 0xffff0000u : 0u);
-            const uint32_t hi = (2 <= room ? kOnes<DT> & 0xffffu : 0u) | (3 <= room ? kOnes<DT> & 0xffff0000u : 0u);
-            const uint4 seen = make_uint4(lo & mask[0], hi & mask[0], lo & mask[1], hi & mask[1]);
-            const f32x4_t t = mfma16<DT>(make_uint4(bad.x & kOnes<DT>, bad.y & kOnes<DT>, bad.z & kOnes<DT>, bad.w & kOnes<DT>),
-                                         seen, (f32x4_t){0, 0, 0, 0});
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[4 * h + c][i] = t[i] > 0.0f ? __builtin_nanf("") : acc[4 * h + c][i];
-            vv = make_uint4(vv.x & ~bad.x, vv.y & ~bad.y, vv.z & ~bad.z, vv.w & ~bad.w);
-          }
-        }
-        acc[4 * h + c] = mfma16<DT>(vv, pp, acc[4 * h + c]);
+      for (int i = 0; i < 2; ++i) {
+        w[i] = pack2<DT>(__builtin_amdgcn_exp2f(fmaf(s[u][2 * i], scale, -m)), __builtin_amdgcn_exp2f(fmaf(s[u][2 * i + 1], scale, -m)));
+        l = St<DT>::dot2(w[i], kOnes<DT>, l);
       }
+      p[u] = make_uint4(w[0] & mask[0], w[1] & mask[0], w[0] & mask[1], w[1] & mask[1]);
     }
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        const uint4 wa = v[2 * u][h], wb = v[2 * u + 1][h];
+        const uint32_t a[4] = {wa.x, wa.y, wa.z, wa.w}, b[4] = {wb.x, wb.y, wb.z, wb.w};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint4 vv = make_uint4(kv8_pair<DT, false>(a[c], sv[2 * u]), kv8_pair<DT, true>(a[c], sv[2 * u]),
+                                kv8_pair<DT, false>(b[c], sv[2 * u + 1]), kv8_pair<DT, true>(b[c], sv[2 * u + 1]));
+          if constexpr (EDGE) {
+            const uint4 bad = not_finite4<DT>(vv);
+            if (__any((bad.x | bad.y | bad.z | bad.w) != 0)) {
+              const int r = room(tok0, u);
+              const uint32_t lo = (0 <= r ? kOnes<DT> & 0xffffu : 0u) | (1 <= r ? kOnes<DT> & 0xffff0000u : 0u);
+              const uint32_t hi = (2 <= r ? kOnes<DT> & 0xffffu : 0u) | (3 <= r ? kOnes<DT> & 0xffff0000u : 0u);
+              const uint4 seen = make_uint4(lo & mask[0], hi & mask[0], lo & mask[1], hi & mask[1]);
+              const f32x4_t t = mfma16<DT>(make_uint4(bad.x & kOnes<DT>, bad.y & kOnes<DT>, bad.z & kOnes<DT>, bad.w & kOnes<DT>),
+                                           seen, (f32x4_t){0, 0, 0, 0});
+#pragma unroll
+              for (int i = 0; i < 4; ++i) acc[4 * h + c][i] = t[i] > 0.0f ? __builtin_nanf("") : acc[4 * h + c][i];
+              vv = make_uint4(vv.x & ~bad.x, vv.y & ~bad.y, vv.z & ~bad.z, vv.w & ~bad.w);
+            }
+          }
+          acc[4 * h + c] = mfma16<DT>(vv, p[u], acc[4 * h + c]);
+        }
+      }
   }
 
   // After the last stage: l over the lanes of a column, NaN where it saw a page outside the pool
@@ -329,7 +344,7 @@ __device__ __attribute__((always_inline)) inline void kv_tokens_finish(const Arg
   // of a thread under way (the rounds of loads are what a merge takes)
   const int items = here * Q;
   const int sets = max(NT / items, 1);
-  constexpr int NB = 16;
+  constexpr int NB = 8;
   for (int i0 = 0; i0 < items; i0 += NT) {
     const int item = sets > 1 ? threadIdx.x % items : i0 + threadIdx.x;
     const int set = sets > 1 ? threadIdx.x / items : 0;
@@ -392,6 +407,8 @@ __device__ __attribute__((always_inline)) inline void kv_tokens_finish(const Arg
 
 // ---- waves split tokens: one workgroup per (split, sequence, kv head, 8-column tile).  CHOSEN: a sequence's tokens are
 // those of its chosen pages, side by side, the last of them its row's own page.
+constexpr int kAuxNt = 2;  // streamed: nothing of it is read again
+
 template <int DT, int D, bool CHOSEN>
 __device__ void kv8_tokens_impl(const Kv8AttnArgs& A) {
   constexpr int NW = kTokWaves, TC = kTokCols;
@@ -439,84 +456,115 @@ __device__ void kv8_tokens_impl(const Kv8AttnArgs& A) {
   // ---- the wave's stages: w, w + NW, ... of the split
   Kv8Row<DT, D> W;
   W.begin(A, S.row0, kvh, S.start, S.ctx, col0, ncols);
+  constexpr int PAGES = Stage::PAGES, H = Stage::H;
   const uint32_t page_stride = (uint32_t)(A.num_layers * A.hkv) * Kv8<D>::kSlab;
   const int64_t base = (int64_t)A.layer * A.hkv + kvh;
   const char* const kp = A.k_pool + base * Kv8<D>::kSlab;
   const char* const vp = A.v_pool + base * Kv8<D>::kSlab;
-  const float2* const sp = A.scales + base;
-  const int32_t* const table = A.tables + (int64_t)b * A.table_stride;
-  const int32_t* const chosen = CHOSEN ? A.chosen + ((int64_t)b * A.hkv + kvh) * A.budget : nullptr;
+  scalar_f32* const sp = (scalar_f32*)(A.scales + base);
+  scalar_i32* const table = (scalar_i32*)(A.tables + (int64_t)b * A.table_stride);
+  scalar_i32* const chosen = CHOSEN ? (scalar_i32*)(A.chosen + ((int64_t)b * A.hkv + kvh) * A.budget) : nullptr;
   const int stages = (end - begin + Stage::TOKENS - 1) / Stage::TOKENS;
   const int count = stages > w ? (stages - w + NW - 1) / NW : 0;
   const int min_limit = S.start + col0 / A.group;
+  const int last_page = (end - 1) / kPage;
   int bad_at = 0x7fffffff;
-  int pages[Stage::PAGES];  // of stage chunk + lane, and their scales
-  float2 scales[Stage::PAGES];
-  auto load_pages = [&](int chunk) __attribute__((always_inline)) {
-    const int lane = threadIdx.x & 63;
-    const int64_t tok = begin + ((int64_t)(chunk + lane) * NW + w) * Stage::TOKENS;
-    int bad = 0x7fffffff;
+  auto first_of = [&](int i) __attribute__((always_inline)) { return begin + (i * NW + w) * Stage::TOKENS; };
+  // Numbers of a stage's pages in the context, and in the pool (those behind the last: the last again).  All of
+  // these are loads of the scalar cache, whose results are used a stage later.
+  auto list = [&](int i, int (&at)[PAGES]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = Stage::PAGES - 1; i >= 0; --i) {
-      const int64_t at = tok + i * kPage;
-      bool ok = true;
-      int page = (int)(at / kPage);
-      if (CHOSEN && at < end) {
+    for (int k = 0; k < PAGES; ++k) {
+      const int p = min(first_of(min(i, count - 1)) / kPage + k, last_page);
+      at[k] = CHOSEN ? chosen[p] : p;
+    }
+  };
+  auto look_up = [&](int i, const int (&at)[PAGES], int (&id)[PAGES]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < PAGES; ++k) {
+      int p = at[k];
+      if constexpr (CHOSEN) {
         // a list that does not ascend to the row's own page is no selection
-        const bool own = page == last / kPage;
-        page = chosen[page];
-        ok = own ? page == own_page : page >= 0 && page < own_page;
+        const int j = min(first_of(min(i, count - 1)) / kPage + k, last_page);
+        const bool ok = j == last / kPage ? p == own_page : p >= 0 && p < own_page;
+        if (!ok) {
+          p = 0;
+          bad_at = 0;
+        }
       }
-      pages[i] = at < end && ok ? table[page] : 0;
-      // a page outside the pool is never an address: page 0 is read instead
-      if (!ok || pages[i] < 0 || pages[i] >= A.num_blocks) {
-        bad = (int)at;
-        pages[i] = 0;
+      id[k] = table[p];
+    }
+  };
+  // a page outside the pool is never an address: page 0 is read instead
+  auto check = [&](int i, int (&id)[PAGES]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < PAGES; ++k)
+      if (id[k] < 0 || id[k] >= A.num_blocks) {
+        id[k] = 0;
+        bad_at = min(bad_at, min(first_of(min(i, count - 1)) / kPage + k, last_page) * kPage);
       }
-    }
-#pragma unroll
-    for (int i = 0; i < Stage::PAGES; ++i) scales[i] = sp[(int64_t)pages[i] * (A.num_layers * A.hkv)];
-    if (__any(bad != 0x7fffffff)) {
-#pragma unroll
-      for (int k = 1; k < 64; k <<= 1) bad = min(bad, __shfl_xor(bad, k));
-      bad_at = min(bad_at, bad);
-    }
   };
   const int lane = threadIdx.x & 63;
   const int k_off = Kv8<D>::k_at(lane & 15, 16 * (lane >> 4)), v_off = Kv8<D>::v_at(lane >> 4, 4 * (lane & 15));
-  auto load = [&](Stage& T, int i) __attribute__((always_inline)) {
+  // loads of no bytes where there is no stage (on: 0): a branch around them would make every wait for them one for all
+  auto load = [&](uint4 (&x)[PAGES][H], const char* pool, int off, int step, const int (&id)[PAGES], bool on) __attribute__((always_inline)) {
 #pragma unroll
-    for (int k = 0; k < Stage::PAGES; ++k) {
-      const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(pages[k], i & 63) * page_stride;
+    for (int k = 0; k < PAGES; ++k) {
+      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(pool + (uint64_t)(uint32_t)id[k] * page_stride), 0, on ? Kv8<D>::kSlab : 0, 0x00020000);
 #pragma unroll
-      for (int h = 0; h < Stage::H; ++h) {
-        T.k[k][h] = *(const uint4*)(kp + at + k_off + 64 * h);
-        T.v[k][h] = *(const uint4*)(vp + at + v_off + 256 * h);
-      }
+      for (int h = 0; h < H; ++h)
+        x[k][h] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off + step * h, 0, kAuxNt));
     }
-#pragma unroll
-    for (int k = 0; k < Stage::PAGES; ++k)
-      T.scale[k] = make_float2(readlane(scales[k].x, i & 63), readlane(scales[k].y, i & 63));
   };
-  auto take = [&](const Stage& T, int i) __attribute__((always_inline)) {
-    const int tok0 = begin + (i * NW + w) * Stage::TOKENS;
+  auto scales_of = [&](const int (&id)[PAGES], float (&sk)[PAGES], float (&sv)[PAGES]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < Stage::SUB; ++u) {
-      const int t = tok0 + 32 * u;
-      if (t <= last) W.step(T, u, t, t + 31 > min_limit);
+    for (int k = 0; k < PAGES; ++k) {
+      scalar_f32* const x = sp + (int64_t)id[k] * (2 * A.num_layers * A.hkv);
+      sk[k] = x[0];
+      sv[k] = x[1];
     }
   };
   if (count) {
-    // one stage ahead; behind the last one it is read once more, so that no wait depends on a branch
-    Stage T[2];
-    load_pages(0);
-    load(T[0], 0);
-    for (int i = 0; i < count; i += 2) {
-      load(T[1], min(i + 1, count - 1));
-      take(T[0], i);
-      if (((i + 2) & 63) == 0 && i + 2 < count) load_pages(i + 2);
-      load(T[0], min(i + 2, count - 1));
-      if (i + 1 < count) take(T[1], i + 1);
+    uint4 K[PAGES][H], V[PAGES][H];
+    int at[PAGES], id[PAGES], next[PAGES];
+    float sk[PAGES], sv[PAGES];
+    list(0, at);
+    look_up(0, at, id);
+    list(1, at);
+    look_up(1, at, next);
+    check(0, id);
+    load(K, kp, k_off, 64, id, true);
+    __builtin_amdgcn_sched_barrier(0);  // (K's before V's, here as below)
+    load(V, vp, v_off, 256, id, true);
+    __builtin_amdgcn_sched_barrier(0);
+    scales_of(id, sk, sv);
+    list(2, at);
+    check(1, next);
+    for (int i = 0; i < count; ++i) {
+      // of the next stage its scales, of the one behind it its pages, on their way while this one is worked on
+      float sk2[PAGES], sv2[PAGES];
+      int after[PAGES];
+      scales_of(next, sk2, sv2);
+      look_up(i + 2, at, after);
+      list(i + 3, at);
+      W.score(K, sk);
+      __builtin_amdgcn_sched_barrier(0);
+      load(K, kp, k_off, 64, next, i + 1 < count);
+      __builtin_amdgcn_sched_barrier(0);
+      const int tok0 = first_of(i);
+      if (tok0 + Stage::TOKENS - 1 > min_limit) W.template add<true>(V, sv, tok0);
+      else W.template add<false>(V, sv, tok0);
+      __builtin_amdgcn_sched_barrier(0);
+      load(V, vp, v_off, 256, next, i + 1 < count);
+      __builtin_amdgcn_sched_barrier(0);
+      check(i + 2, after);
+#pragma unroll
+      for (int k = 0; k < PAGES; ++k) {
+        next[k] = after[k];
+        sk[k] = sk2[k];
+        sv[k] = sv2[k];
+      }
     }
   }
   W.finish(bad_at);
@@ -878,10 +926,10 @@ __device__ void kv8_columns_impl(const Kv8AttnArgs& A) {
 }  // namespace luc
 
 #define LUC_KV8_ATTENTION(DTN, DT, D)                                                            \
-  extern "C" __global__ __launch_bounds__(256, 2) void luc_kv8_tokens_##DTN##_d##D(luc::Kv8AttnArgs a) {  \
+  extern "C" __global__ __launch_bounds__(256, D == 64 ? 4 : 3) void luc_kv8_tokens_##DTN##_d##D(luc::Kv8AttnArgs a) {  \
     luc::kv8_tokens_impl<luc::DT, D, false>(a);                                                  \
   }                                                                                              \
-  extern "C" __global__ __launch_bounds__(256, 2) void luc_kv8_chosen_##DTN##_d##D(luc::Kv8AttnArgs a) {  \
+  extern "C" __global__ __launch_bounds__(256, D == 64 ? 4 : 3) void luc_kv8_chosen_##DTN##_d##D(luc::Kv8AttnArgs a) {  \
     luc::kv8_tokens_impl<luc::DT, D, true>(a);                                                   \
   }                                                                                              \
   extern "C" __global__ __launch_bounds__(64 * luc::Kv8Cols<D>::WAVES, D == 128 ? 2 : 3) void luc_kv8_columns_##DTN##_d##D(luc::Kv8AttnArgs a) { \

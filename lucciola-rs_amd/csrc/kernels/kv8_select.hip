@@ -9,14 +9,15 @@
 //   score = max over the group's heads of (((S_0 2^e_0 + S_1 2^e_1) + S_2 2^e_2) + S_3 2^e_3) * scale_K
 // rounds its few sums in f32, in that order: the choice is a function of the inputs, whatever computes it.
 //
-// A workgroup scores 128 pages of one (sequence, kv head); the last of them to arrive picks.  Lane (n, g) of a wave loads
+// A workgroup scores 128 pages of one (sequence, kv head) or more; the last of them to arrive picks.  Lane (n, g) of a wave loads
 // bounds 64 i + 16 g .. + 15 of page n of 16; those belong to group 2 i + g / 2, so of the 16 columns of
 // v_mfma_f32_16x16x32_f16 the lower 8 take the heads' even groups (q is 0 in lanes of the odd ones) and the upper
 // 8 the same heads' odd groups.
 //
-// The pick.  Scores become whole numbers of the same order (keys).  The budget'th largest is found 8 bits at a time by
-// a histogram in LDS; then every wave goes through its quarter of the pages in order and writes those above, and of those
-// equal to it the first, to their places.
+// The pick.  Scores become whole numbers of the same order (keys).  A histogram in LDS over 1024 equal parts of
+// the keys' range finds the part that the last chosen one lies in; the keys there, a few, are ranked by every wave for
+// itself (many: another histogram over that part).  Then every thread writes those above, and of those equal to it the
+// first, to their places, which sums over the threads before it give.
 #include "kv8.h"
 #include "kv_split.h"
 
@@ -33,15 +34,17 @@ struct Kv8SelectArgs {
   const int32_t* start_pos;
   int32_t* pages;             // [batch][hkv][budget]
   int32_t* ws_cnt;
-  uint32_t* ws_key;           // [batch][hkv][max_pages]
+  uint32_t* ws_key;           // [batch][hkv][max_pages], that a multiple of 4
   int32_t batch, total_rows, max_rows, max_ctx, layer, num_layers, hkv, group, num_blocks;
   int32_t budget, first, recent, chunks, max_pages;
+  int32_t tiles;  // of 16 pages a wave: a multiple of kSelTiles
 };
 
 constexpr int kSelWaves = 4;
-constexpr int kSelTiles = 2;                                 // of 16 pages a wave
-constexpr int kSelChunk = kSelWaves * kSelTiles * 16;        // pages of a workgroup
-constexpr int kSelLdsKeys = 8192;                            // keys of a pick that LDS holds
+constexpr int kSelTiles = 2;  // of 16 pages, whose bounds a wave loads at once
+constexpr int kDppRowRor8 = 0x128;
+constexpr int kSelBatch = 4 * 64 * kSelWaves, kSelBatches = 4;  // keys that a pick reads at once
+constexpr int kSelBinBits = 10, kSelBins = 1 << kSelBinBits;
 
 // Whole numbers as packed fp16: codes rounded to units.  |x| <= 448, and from 1024 to 2048 fp16 has no fractions.
 __device__ inline uint32_t whole2(uint32_t w) {
@@ -66,13 +69,206 @@ __device__ inline uint32_t score_key(float x) {
   return __builtin_isnan(x) ? 0u : k;
 }
 
+// ---- the pick: of `count` keys the `budget` largest, equal ones from the lowest place on
+struct SelectMem {
+  uint32_t hist[kSelBins];
+  uint32_t list[64];
+  uint32_t part[kSelWaves][kSelBatches];
+  uint32_t bin, before, length;
+};
+
+// Inclusive sums over the threads of the workgroup, of N numbers; a barrier inside.  total: of all threads.
+template <int N>
+__device__ __attribute__((always_inline)) inline void block_scan(uint32_t (&x)[N], uint32_t (&total)[N], uint32_t (&part)[kSelWaves][kSelBatches]) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1)
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const uint32_t y = __shfl_up(x[n], k);
+      if (lane >= k) x[n] += y;
+    }
+  if (lane == 63) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) part[w][n] = x[n];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    total[n] = 0;
+#pragma unroll
+    for (int k = 0; k < kSelWaves; ++k) {
+      const uint32_t y = part[k][n];
+      x[n] += k < w ? y : 0u;
+      total[n] += y;
+    }
+  }
+}
+
+// The threads' keys are read kSelBatch at a time, in kSelBatches rounds, four successive places a thread; as
+// many stay in registers (HELD), more are read again by every pass.  (hist is 0, and so is length.)  fixed: how
+// many of the keys are the highest one.
+template <bool HELD>
+__device__ __attribute__((always_inline)) inline void pick_pages(const uint32_t* keys, int count, int budget, int fixed, int32_t* out,
+                                                                 SelectMem& s) {
+  constexpr int NT = 64 * kSelWaves, EACH = kSelBins / NT, R = kSelBatches;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const __amdgpu_buffer_rsrc_t far = ws_rsrc((const float*)keys);  // (written on other XCDs)
+  uint32_t k[R][4];
+  auto read = [&](int base) __attribute__((always_inline)) {  // (the keys' room is whole fours)
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+      const float4 x = ws_get4(far, min(base + u * kSelBatch + 4 * tid, (count - 1) & ~3));
+      const u32x4_t y = __builtin_bit_cast(u32x4_t, x);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) k[u][r] = y[r];
+    }
+  };
+  // f(place, key) of every key, in rounds
+  auto pass = [&](auto&& f) __attribute__((always_inline)) {
+    for (int base = 0; base < (HELD ? 1 : count); base += R * kSelBatch) {
+      if constexpr (!HELD) read(base);
+#pragma unroll
+      for (int u = 0; u < R; ++u) {
+        if (base + u * kSelBatch >= count) break;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int at = base + u * kSelBatch + 4 * tid + r;
+          f(at, at < count ? k[u][r] : 0u, at < count);
+        }
+      }
+    }
+  };
+  if constexpr (HELD) read(0);
+  // the range of the keys; those of pages that are always chosen (the highest key) stand apart
+  uint32_t lo = ~0u, hi = 0;
+  pass([&](int, uint32_t x, bool on) __attribute__((always_inline)) {
+    lo = on ? min(lo, x) : lo;
+    hi = x == ~0u ? hi : max(hi, x);
+  });
+#pragma unroll
+  for (int n = 1; n < 64; n <<= 1) {
+    lo = min(lo, (uint32_t)__shfl_xor((int)lo, n));
+    hi = max(hi, (uint32_t)__shfl_xor((int)hi, n));
+  }
+  if (lane == 0) {
+    s.list[w] = lo;
+    s.list[kSelWaves + w] = hi;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < kSelWaves; ++n) {
+    lo = min(lo, s.list[n]);
+    hi = max(hi, s.list[kSelWaves + n]);
+  }
+  // bar: the want'th largest of the others; in steps of kSelBins equal bins of what is left of the range
+  uint32_t bar = ~0u, want = (uint32_t)(budget - fixed);
+  while (want) {
+    const int shift = max(32 - __builtin_clz((hi - lo) | 1) - kSelBinBits, 0);
+    pass([&](int, uint32_t x, bool on) __attribute__((always_inline)) {
+      if (on && x >= lo && x <= hi) atomicAdd(&s.hist[(x - lo) >> shift], 1u);
+    });
+    __syncthreads();
+    uint32_t c[EACH], up[1] = {0}, all[1];  // bins from the top, EACH a thread
+#pragma unroll
+    for (int n = 0; n < EACH; ++n) {
+      c[n] = s.hist[kSelBins - 1 - EACH * tid - n];
+      up[0] += c[n];
+    }
+    const uint32_t sum = up[0];
+    block_scan(up, all, s.part);
+    uint32_t before = up[0] - sum;
+    if (before < want && up[0] >= want) {
+      int at = 0;
+#pragma unroll
+      for (int n = 0; n < EACH - 1; ++n)
+        if (at == n && before + c[n] < want) {
+          before += c[n];
+          at = n + 1;
+        }
+      s.bin = kSelBins - 1 - EACH * tid - at;
+      s.before = before;
+    }
+    __syncthreads();
+    lo += s.bin << shift;
+    hi = min(hi, lo + ((1u << shift) - 1));
+    want -= s.before;
+    if (shift == 0) {
+      bar = lo;
+      break;
+    }
+    // few keys are left: every wave ranks them by itself
+    pass([&](int, uint32_t x, bool on) __attribute__((always_inline)) {
+      if (on && x >= lo && x <= hi) {
+        const uint32_t n = atomicAdd(&s.length, 1u);
+        if (n < 64) s.list[n] = x;
+      }
+    });
+#pragma unroll
+    for (int n = 0; n < EACH; ++n) s.hist[tid + NT * n] = 0;
+    __syncthreads();
+    const uint32_t length = s.length;
+    if (length <= 64) {
+      const uint32_t mine = lane < (int)length ? s.list[lane] : 0u;
+      uint32_t over = 0, same = 0;
+      for (uint32_t n = 0; n < length; ++n) {
+        const uint32_t x = (uint32_t)__builtin_amdgcn_readlane((int)mine, n);
+        over += x > mine;
+        same += x == mine;
+      }
+      const uint64_t at = __ballot(lane < (int)length && over < want && over + same >= want);
+      const int l = __builtin_ctzll(at);
+      bar = (uint32_t)__builtin_amdgcn_readlane((int)mine, l);
+      want -= (uint32_t)__builtin_amdgcn_readlane((int)over, l);
+      break;
+    }
+    __syncthreads();
+    if (tid == 0) s.length = 0;
+    __syncthreads();
+  }
+  // ---- places: behind those of earlier rounds, and of earlier threads in this one.  (Counts of a round fit 16 bits.)
+  uint32_t over = 0, same = 0;  // of earlier rounds
+  for (int base = 0; base < (HELD ? 1 : count); base += R * kSelBatch) {
+    if constexpr (!HELD) read(base);
+    uint32_t own[R], up[R], all[R];
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+      own[u] = 0;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const bool on = base + u * kSelBatch + 4 * tid + r < count;
+        const uint32_t x = k[u][r];
+        own[u] += on ? (x > bar || x == ~0u ? 1u : x == bar ? 1u << 16 : 0u) : 0u;
+      }
+      up[u] = own[u];
+    }
+    __syncthreads();  // (part)
+    block_scan(up, all, s.part);
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+      if (base + u * kSelBatch >= count) break;
+      const uint32_t before = up[u] - own[u];
+      uint32_t o = over + (before & 0xffffu), e = same + (before >> 16);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int at = base + u * kSelBatch + 4 * tid + r;
+        const uint32_t x = k[u][r];
+        const bool on = at < count, high = on && (x > bar || x == ~0u), equal = on && !high && x == bar;
+        if (high || (equal && e < want)) out[o + min(e, want)] = at;
+        o += high;
+        e += equal;
+      }
+      over += all[u] & 0xffffu;
+      same += all[u] >> 16;
+    }
+  }
+}
+
 template <int DT, int D>
 __device__ void kv8_select_impl(const Kv8SelectArgs& A) {
   constexpr int H = D / 64;
-  __shared__ uint32_t s_key[kSelLdsKeys];
-  __shared__ uint32_t s_hist[256];
-  __shared__ uint32_t s_pick[4];  // bits of the key so far, how many are wanted among those that share them
-  __shared__ int s_count[kSelWaves][2], s_last;
+  __shared__ SelectMem s;
+  __shared__ int s_last;
   // neighbours on one XCD (block x runs on XCD x % 8): the kv heads of the same pages, whose bounds lie side by side
   const int units = A.batch * A.chunks;  // (padded to whole eights)
   const int u = blockIdx.x / (8 * A.hkv) * 8 + blockIdx.x % 8, kvh = blockIdx.x / 8 % A.hkv;
@@ -87,19 +283,20 @@ __device__ void kv8_select_impl(const Kv8SelectArgs& A) {
       for (int i = threadIdx.x; i < A.budget; i += 64 * kSelWaves) out[i] = i < count ? i : -1;
     return;
   }
-  const int chunks = (count + kSelChunk - 1) / kSelChunk;
+  const int chunk_pages = 16 * kSelWaves * A.tiles;
+  const int chunks = (count + chunk_pages - 1) / chunk_pages;
   if (chunk >= chunks) return;
   uint32_t* const keys = A.ws_key + ((int64_t)b * A.hkv + kvh) * A.max_pages;
+  for (int i = threadIdx.x; i < kSelBins; i += 64 * kSelWaves) s.hist[i] = 0;
+  if (threadIdx.x == 0) s.length = 0;
 
-  // ---- scores of 16 pages at a time
+  // ---- scores of 16 pages at a time, kSelTiles times 16 with their bounds one step ahead
   {
-    const int n = lane & 15, g = lane >> 4, p0 = chunk * kSelChunk + w * (16 * kSelTiles);
+    const int n = lane & 15, g = lane >> 4, p0 = chunk * chunk_pages + w * (16 * A.tiles);
+    const int last = min(count, p0 + 16 * A.tiles);
     const int32_t* const table = A.tables + (int64_t)b * A.table_stride;
     const int64_t base = (int64_t)A.layer * A.hkv + kvh;
     const int64_t stride = (int64_t)A.num_layers * A.hkv;
-    int page[kSelTiles];
-#pragma unroll
-    for (int t = 0; t < kSelTiles; ++t) page[t] = p0 + 16 * t + n < count ? table[p0 + 16 * t + n] : 0;
     // q of head n % 8, dimensions 64 i + 16 g + 8 k .. + 7
     const int head = n & 7;
     const bool on = head < A.group;
@@ -109,22 +306,32 @@ __device__ void kv8_select_impl(const Kv8SelectArgs& A) {
     for (int i = 0; i < H; ++i)
 #pragma unroll
       for (int k = 0; k < 2; ++k) raw[i][k] = on ? *(const uint4*)(src + 64 * i + 8 * k) : make_uint4(0, 0, 0, 0);
-    bool bad[kSelTiles];
-    uint4 hi[kSelTiles][H], lo[kSelTiles][H];
-    float scale[kSelTiles];
+    struct Step {
+      uint4 hi[kSelTiles][H], lo[kSelTiles][H];
+      float scale[kSelTiles];
+      bool bad[kSelTiles];
+    };
+    int pages = 0;  // of the wave's next 64
+    auto load = [&](Step& T, int t0) __attribute__((always_inline)) {
+      const int first = p0 + 16 * t0;
+      if (t0 % 4 == 0) pages = first + lane < last ? table[first + lane] : 0;
 #pragma unroll
-    for (int t = 0; t < kSelTiles; ++t) {
-      // a page outside the pool is never an address: page 0 is read instead, and the page comes last
-      bad[t] = page[t] < 0 || page[t] >= A.num_blocks;
-      const int64_t at = (int64_t)(bad[t] ? 0 : page[t]) * stride + base;
-      const uint8_t* const p = A.bounds + at * (2 * D) + 16 * g;
+      for (int t = 0; t < kSelTiles; ++t) {
+        const int page = __shfl(pages, 16 * ((t0 + t) & 3) + n);
+        // a page outside the pool is never an address: page 0 is read instead, and the page comes last
+        T.bad[t] = page < 0 || page >= A.num_blocks;
+        const int64_t at = (int64_t)(T.bad[t] ? 0 : page) * stride + base;
+        const uint8_t* const p = A.bounds + at * (2 * D) + 16 * g;
 #pragma unroll
-      for (int i = 0; i < H; ++i) {
-        hi[t][i] = *(const uint4*)(p + 64 * i);
-        lo[t][i] = *(const uint4*)(p + D + 64 * i);
+        for (int i = 0; i < H; ++i) {
+          T.hi[t][i] = *(const uint4*)(p + 64 * i);
+          T.lo[t][i] = *(const uint4*)(p + D + 64 * i);
+        }
+        T.scale[t] = A.scales[at].x;
       }
-      scale[t] = A.scales[at].x;
-    }
+    };
+    Step T[2];
+    if (p0 < last) load(T[0], 0);
     uint4 qp[H][2], qn[H][2];  // n where it is positive, and where it is negative
     float unit[H];             // of the lane's column: group 2 i + n / 8
     const bool mine = (g >> 1) == (n >> 3);
@@ -165,41 +372,50 @@ __device__ void kv8_select_impl(const Kv8SelectArgs& A) {
         qn[i][k] = make_uint4(wn[0], wn[1], wn[2], wn[3]);
       }
     }
+    auto score = [&](const Step& T, int t0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < kSelTiles; ++t) {
-      f32x4_t sum[H];
-#pragma unroll
-      for (int i = 0; i < H; ++i) {
-        sum[i] = (f32x4_t){0, 0, 0, 0};
-        sum[i] = mfma_f16(whole8(hi[t][i].x, hi[t][i].y), qp[i][0], sum[i]);
-        sum[i] = mfma_f16(whole8(hi[t][i].z, hi[t][i].w), qp[i][1], sum[i]);
-        sum[i] = mfma_f16(whole8(lo[t][i].x, lo[t][i].y), qn[i][0], sum[i]);
-        sum[i] = mfma_f16(whole8(lo[t][i].z, lo[t][i].w), qn[i][1], sum[i]);
-      }
-      // rows 4 g + r are pages; columns n < 8 the even groups' sums, n >= 8 the odd ones'
-      float best[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float score = 0.0f;
+      for (int t = 0; t < kSelTiles; ++t) {
+        f32x4_t sum[H];
 #pragma unroll
         for (int i = 0; i < H; ++i) {
-          const float own = sum[i][r] * unit[i], other = __shfl_xor(own, 8);
-          const float even = n < 8 ? own : other, odd = n < 8 ? other : own;
-          score = i == 0 ? even + odd : (score + even) + odd;
+          sum[i] = (f32x4_t){0, 0, 0, 0};
+          sum[i] = mfma_f16(whole8(T.hi[t][i].x, T.hi[t][i].y), qp[i][0], sum[i]);
+          sum[i] = mfma_f16(whole8(T.hi[t][i].z, T.hi[t][i].w), qp[i][1], sum[i]);
+          sum[i] = mfma_f16(whole8(T.lo[t][i].x, T.lo[t][i].y), qn[i][0], sum[i]);
+          sum[i] = mfma_f16(whole8(T.lo[t][i].z, T.lo[t][i].w), qn[i][1], sum[i]);
         }
-        best[r] = on ? score : -INFINITY;
-      }
+        // rows 4 g + r are pages; columns n < 8 the even groups' sums, n >= 8 the odd ones'
+        float best[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) best[r] = row_max16(best[r]);
-      // lane n < 4 of a row stores page 4 g + n
-      const int r = n & 3, at = 4 * g + r, p = p0 + 16 * t + at;
-      const float top = r == 0 ? best[0] : r == 1 ? best[1] : r == 2 ? best[2] : best[3];
-      const float s = __shfl(scale[t], at);
-      const bool none = __shfl((int)bad[t], at);
-      if (n < 4 && p < count) {
-        const bool always = p < A.first || p >= count - A.recent;
-        __hip_atomic_store(keys + p, always ? ~0u : none ? 0u : score_key(top * s), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (int r = 0; r < 4; ++r) {
+          float all = 0.0f;
+#pragma unroll
+          for (int i = 0; i < H; ++i) {
+            const float own = sum[i][r] * unit[i], other = dpp_mov<kDppRowRor8>(own);
+            const float even = n < 8 ? own : other, odd = n < 8 ? other : own;
+            all = i == 0 ? even + odd : (all + even) + odd;
+          }
+          best[r] = on ? all : -INFINITY;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) best[r] = row_max16(best[r]);
+        // lane n < 4 of a row stores page 4 g + n
+        const int r = n & 3, at = 4 * g + r, p = p0 + 16 * (t0 + t) + at;
+        const float top = r == 0 ? best[0] : r == 1 ? best[1] : r == 2 ? best[2] : best[3];
+        const float sk = __shfl(T.scale[t], at);
+        const bool none = __shfl((int)T.bad[t], at);
+        if (n < 4 && p < count) {
+          const bool always = p < A.first || p >= count - A.recent;
+          __hip_atomic_store(keys + p, always ? ~0u : none ? 0u : score_key(top * sk), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
       }
+    };
+    const int steps = (last - p0 + 16 * kSelTiles - 1) / (16 * kSelTiles);  // (none: below 1)
+    for (int i = 0; i < steps; i += 2) {
+      if (i + 1 < steps) load(T[1], (i + 1) * kSelTiles);
+      score(T[0], i * kSelTiles);
+      if (i + 2 < steps) load(T[0], (i + 2) * kSelTiles);
+      if (i + 1 < steps) score(T[1], (i + 1) * kSelTiles);
     }
   }
   // ---- the last workgroup of the (sequence, kv head) to arrive picks
@@ -209,90 +425,11 @@ __device__ void kv8_select_impl(const Kv8SelectArgs& A) {
     int32_t* const cnt = A.ws_cnt + b * A.hkv + kvh;
     s_last = __hip_atomic_fetch_add(cnt, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == chunks - 1;
     if (s_last) __hip_atomic_store(cnt, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    s_pick[0] = 0;
-    s_pick[1] = A.budget;
   }
   __syncthreads();
   if (!s_last) return;
-  const bool lds = count <= kSelLdsKeys;
-  auto key = [&](int i) __attribute__((always_inline)) {
-    return lds ? s_key[i] : __hip_atomic_load(keys + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  };
-  if (lds) {
-    for (int i = threadIdx.x; i < count; i += 64 * kSelWaves)
-      s_key[i] = __hip_atomic_load(keys + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-  }
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += 64 * kSelWaves) s_hist[i] = 0;
-    __syncthreads();
-    const uint32_t above = s_pick[0], mask = shift == 24 ? 0u : ~0u << (shift + 8);
-    for (int i = threadIdx.x; i < count; i += 64 * kSelWaves) {
-      const uint32_t k = key(i);
-      if ((k & mask) == above) atomicAdd(&s_hist[k >> shift & 255], 1u);
-    }
-    __syncthreads();
-    if (w == 0) {  // lane l: digits 255 - 4 l and the three below it
-      const uint32_t want = s_pick[1];
-      uint32_t c[4], sum = 0;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        c[r] = s_hist[255 - 4 * lane - r];
-        sum += c[r];
-      }
-      uint32_t up = sum;  // of the lane's digits and all above
-#pragma unroll
-      for (int k = 1; k < 64; k <<= 1) {
-        const uint32_t y = __shfl_up(up, k);
-        if (lane >= k) up += y;
-      }
-      uint32_t before = up - sum;
-      if (before < want && up >= want) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (before < want && before + c[r] >= want) {
-            s_pick[0] = above | (uint32_t)(255 - 4 * lane - r) << shift;
-            s_pick[1] = want - before;
-            before = want;  // (found)
-          } else {
-            before += c[r];
-          }
-        }
-      }
-    }
-    __syncthreads();
-  }
-  const uint32_t bar = s_pick[0];
-  const int want = (int)s_pick[1];  // of those equal to it
-  const int span = ((count + kSelWaves - 1) / kSelWaves + 63) / 64 * 64;
-  const int from = w * span, to = min(count, from + span);
-  int over = 0, same = 0;
-  for (int i = from; i < to; i += 64) {
-    const uint32_t k = i + lane < to ? key(i + lane) : 0u;
-    over += __builtin_popcountll(__ballot(i + lane < to && k > bar));
-    same += __builtin_popcountll(__ballot(i + lane < to && k == bar));
-  }
-  if (lane == 0) {
-    s_count[w][0] = over;
-    s_count[w][1] = same;
-  }
-  __syncthreads();
-  over = same = 0;
-  for (int k = 0; k < w; ++k) {
-    over += s_count[k][0];
-    same += s_count[k][1];
-  }
-  const uint64_t below = lane ? ~0ull >> (64 - lane) : 0ull;
-  for (int i = from; i < to; i += 64) {
-    const uint32_t k = i + lane < to ? key(i + lane) : 0u;
-    const uint64_t o = __ballot(i + lane < to && k > bar), e = __ballot(i + lane < to && k == bar);
-    const int o_at = over + __builtin_popcountll(o & below), e_at = same + __builtin_popcountll(e & below);
-    const bool take = i + lane < to && (k > bar || (k == bar && e_at < want));
-    const int to_at = o_at + min(e_at, want);
-    if (take) out[to_at] = i + lane;
-    over += __builtin_popcountll(o);
-    same += __builtin_popcountll(e);
-  }
+  if (count <= kSelBatch * kSelBatches) pick_pages<true>(keys, count, A.budget, A.first + A.recent, out, s);
+  else pick_pages<false>(keys, count, A.budget, A.first + A.recent, out, s);
 }
 
 }  // namespace luc

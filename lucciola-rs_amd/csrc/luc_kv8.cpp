@@ -13,6 +13,7 @@ namespace {
 struct Kv8AppendArgs : NormAppendArgs {
   float* scales;
   void* bounds;
+  int32_t span;
 };
 
 // luc::Kv8ReadArgs of kv8_append.hip: the same fields in the same order.
@@ -64,10 +65,12 @@ struct Kv8SelectArgs {
   int32_t* ws_cnt;
   uint32_t* ws_key;
   int32_t batch, total_rows, max_rows, max_ctx, layer, num_layers, hkv, group, num_blocks;
-  int32_t budget, first, recent, chunks, max_pages;
+  int32_t budget, first, recent, chunks, max_pages, tiles;
 };
 
 constexpr int kCUs = 256;
+// Rows from which a wave of an append looks through 16 rows for runs, instead of through its own.
+constexpr int kAppendSpanRows = 512;
 constexpr int kTokCols = 8;            // columns of a workgroup
 constexpr int kTokMaxSplits = 256;     // kv_split.h
 constexpr int kTokSlots = 2 * kCUs;    // workgroups that a launch is planned for: two a CU
@@ -84,7 +87,8 @@ constexpr int kColsOf64 = 128, kColsOf128 = 256;
 // are not shorter than pays for their partials.
 constexpr int kColsMinSplit64 = 512, kColsMinSplit128 = 256, kColsMaxSplits = 32;
 constexpr int64_t kMaxArrivals = 1 << 16;  // (sequence, kv head, column tile)
-constexpr int kSelChunk = 128;             // kv8_select.hip
+constexpr int kSelPages = 4 * 16;          // pages of a workgroup's waves at once (kv8_select.hip)
+constexpr int kSelWorkgroups = 4 * kCUs;   // of a selection, before they take more pages each
 
 struct Kv8Plan {
   bool tokens = false;  // waves split tokens, else columns
@@ -135,7 +139,7 @@ size_t kv8_workspace_bytes(const Kv8Plan& p, int batch, int total_rows, int hkv,
 // Of a selection: scores are needed where a context may have more pages than the budget.
 size_t select_workspace_bytes(int batch, int max_ctx, int budget, int hkv) {
   const int64_t pages = ceil_div(max_ctx, LUC_BLOCK_SIZE);
-  return pages <= budget ? 0 : (size_t)(kMaxArrivals * 4 + (int64_t)batch * hkv * pages * 4);
+  return pages <= budget ? 0 : (size_t)(kMaxArrivals * 4 + (int64_t)batch * hkv * ceil_div(pages, 4) * 16);
 }
 // Positions among the chosen pages' tokens.
 int chosen_ctx(int max_ctx, int budget) { return (int)std::min<int64_t>(max_ctx, (int64_t)budget * LUC_BLOCK_SIZE); }
@@ -247,14 +251,14 @@ int luc_kv8_append(luc_ctx* ctx, void* stream, int dtype, const void* q, const v
   Kv8AppendArgs a{{q, k, v, row_stride, q_bias, k_bias, v_bias, q_norm, k_norm, cos_table, sin_table, positions,
                    slots, q_out, q_out_stride, nullptr, nullptr, 0, k_pool, v_pool, 0, eps, num_tokens, max_pos,
                    layer, num_layers, num_q_heads, num_kv_heads},
-                  scales, bounds};
+                  scales, bounds, num_tokens > kAppendSpanRows ? 16 : 1};
   if (int rc = check_append(ctx, dtype, a, num_blocks, head_dim, block_size)) return rc;
   if (int rc = check_pools(k_pool, v_pool, scales, num_layers, num_kv_heads, head_dim)) return rc;
   if (!aligned(bounds, 16)) return fail(LUC_E_INVALID, "bounds must be 16-byte aligned");
   if (num_tokens == 0) return LUC_OK;
-  // q: head_dim / 16 lanes a head; then a wave for every row's k and v heads
+  // q: head_dim / 16 lanes a head; then a wave for every span of rows of every k and v head
   const int64_t grid = ceil_div((int64_t)num_tokens * num_q_heads, 4096 / head_dim) +
-                       ceil_div((int64_t)num_tokens * num_kv_heads * 2, 4);
+                       ceil_div(ceil_div(num_tokens, a.span) * num_kv_heads * 2, 4);
   if (grid * 256 > UINT32_MAX) return fail(LUC_E_INVALID, "too many rows for one launch");
   if (int rc = check_device(ctx)) return rc;
   hipFunction_t fn;
@@ -353,14 +357,16 @@ int luc_kv8_select(luc_ctx* ctx, void* stream, int dtype, int32_t* pages, int bu
   if (batch == 0) return LUC_OK;
   const size_t need = select_workspace_bytes(batch, max_ctx, budget, num_kv_heads);
   if (int rc = check_workspace(workspace, workspace_bytes, need)) return rc;
-  const int max_pages = (int)ceil_div(max_ctx, LUC_BLOCK_SIZE);
-  const int64_t chunks = need ? ceil_div(max_pages, kSelChunk) : 1;
+  const int max_pages = (int)ceil_div(max_ctx, 4 * LUC_BLOCK_SIZE) * 4;
+  int tiles = 2;
+  while (tiles < 16 && (int64_t)batch * num_kv_heads * ceil_div(max_pages, kSelPages * tiles) > kSelWorkgroups) tiles *= 2;
+  const int64_t chunks = need ? ceil_div(max_pages, kSelPages * tiles) : 1;
   const int64_t grid = ceil_div(batch * chunks, 8) * 8 * num_kv_heads;
   if (grid * 256 > UINT32_MAX) return fail(LUC_E_INVALID, "batch x kv heads x max_ctx too large");
   if (int rc = check_device(ctx)) return rc;
   Kv8SelectArgs a{q, q_row_stride, bounds, scales, block_tables, table_stride, cu_seqlens, start_pos, pages, nullptr,
                   nullptr, batch, total_rows, 1, max_ctx, layer, num_layers, num_kv_heads, num_q_heads / num_kv_heads,
-                  num_blocks, budget, first, recent, (int)chunks, max_pages};
+                  num_blocks, budget, first, recent, (int)chunks, max_pages, tiles};
   if (need) {
     a.ws_cnt = static_cast<int32_t*>(workspace);
     a.ws_key = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + kMaxArrivals * 4);
