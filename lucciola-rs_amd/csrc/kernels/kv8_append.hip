@@ -20,7 +20,7 @@ namespace luc {
 struct Kv8AppendArgs : NormAppendArgs {  // (k_out, v_out unused)
   float* scales;
   uint8_t* bounds;  // or null
-  int32_t span;     // rows whose runs a wave has: 1 or 16
+  uint32_t every;   // a block of runs comes first of so many
 };
 
 constexpr int kAppendWaves = 4;
@@ -81,7 +81,7 @@ __device__ __attribute__((always_inline)) inline void append_run(const Kv8Append
   }
   // ---- the rows' values, in 16 bits and back
   const int c = lane % LANES, kind = 1 + is_v;
-  float x[PASSES][16];
+  uint4 x[PASSES][2];
   int place[PASSES];  // of the lane's row in the page
   float top = 0.0f;
 #pragma unroll
@@ -91,17 +91,19 @@ __device__ __attribute__((always_inline)) inline void append_run(const Kv8Append
     const int pj = __shfl(pos, from);
     place[p] = (int)(__shfl((int)(slot & (kPage - 1)), from));
     if (j >= len) continue;
-    append_head<DT, D>(A, kind, row - SELF + from, hh, c, pj, x[p]);
-    const uint4 a = pack8<DT>(x[p]), b = pack8<DT>(x[p] + 8);
-    unpack8<DT>(a, x[p]);
-    unpack8<DT>(b, x[p] + 8);
+    float y[16];
+    append_head<DT, D>(A, kind, row - SELF + from, hh, c, pj, y);
+    x[p][0] = pack8<DT>(y);
+    x[p][1] = pack8<DT>(y + 8);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float y = x[p][e];
-      x[p][e] = __builtin_isnan(y) ? y : fminf(fmaxf(y, -kKv8Limit), kKv8Limit);
-      top = fmaxf(top, fabsf(x[p][e]));
+    for (int h = 0; h < 2; ++h) {
+      unpack8<DT>(x[p][h], y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(y[e]));  // (a NaN is passed over)
     }
+    asm volatile("" : "+v"(x[p][0].x), "+v"(x[p][1].x)::"memory");
   }
+  top = fminf(top, kKv8Limit);
   const int e = max(kv8_exponent(wave_max(top)), held);
   const float up = pow2f(-e), less = pow2f(held - e);
   const bool grown = joins && e != held;
@@ -112,12 +114,11 @@ __device__ __attribute__((always_inline)) inline void append_run(const Kv8Append
     if (j >= len) continue;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      uint32_t code[2];
+      float y[8];
+      unpack8<DT>(x[p][h], y);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const float* const y = x[p] + 8 * h + 4 * k;
-        code[k] = kv8_encode4(y[0] * up, y[1] * up, y[2] * up, y[3] * up);
-      }
+      for (int e = 0; e < 8; ++e) y[e] = __builtin_isnan(y[e]) ? y[e] : fminf(fmaxf(y[e], -kKv8Limit), kKv8Limit) * up;
+      const uint32_t code[2] = {kv8_encode4(y[0], y[1], y[2], y[3]), kv8_encode4(y[4], y[5], y[6], y[7])};
       const int i = D / 2 * h + 8 * c;
       if (is_v) {
 #pragma unroll
@@ -187,14 +188,18 @@ __device__ __attribute__((always_inline)) inline void append_run(const Kv8Append
   }
 }
 
-template <int DT, int D>
+// MANY: a wave has the runs that begin in 16 rows, else in one.
+template <int DT, int D, bool MANY>
 __device__ void kv8_append_impl(const Kv8AppendArgs& A) {
-  constexpr int LANES = D / 16;
+  constexpr int LANES = D / 16, SPAN = MANY ? 16 : 1;
   __shared__ __attribute__((aligned(16))) uint8_t s_image[kAppendWaves][Kv8<D>::kSlab];
   const uint32_t nq = (uint32_t)A.rows * A.hq;
-  const uint32_t q_blocks = (nq + 256 / LANES - 1) / (256 / LANES);
-  if (blockIdx.x < q_blocks) {
-    const uint32_t unit = (blockIdx.x * 256 + threadIdx.x) / LANES;
+  const uint32_t spans = ((uint32_t)A.rows + SPAN - 1) / SPAN;
+  // blocks of runs among those of q, evenly: they wait more than they move
+  const uint32_t run_blocks = (2u * A.hkv * spans + kAppendWaves - 1) / kAppendWaves;
+  const uint32_t turn = blockIdx.x / A.every, before = min(turn + (blockIdx.x % A.every != 0), run_blocks);
+  if (blockIdx.x % A.every != 0 || turn >= run_blocks) {
+    const uint32_t unit = ((blockIdx.x - before) * 256 + threadIdx.x) / LANES;
     const int c = threadIdx.x % LANES;
     if (unit >= nq) return;
     const int row = unit / A.hq, hh = unit % A.hq;
@@ -203,22 +208,29 @@ __device__ void kv8_append_impl(const Kv8AppendArgs& A) {
     float x[16];
     append_head<DT, D>(A, 0, row, hh, c, pos, x);
     uint16_t* const o = A.q_out + row * A.q_out_stride + hh * D;
-    *(uint4*)(o + 8 * c) = pack8<DT>(x);
-    *(uint4*)(o + D / 2 + 8 * c) = pack8<DT>(x + 8);
+    const uint4 o1 = pack8<DT>(x), o2 = pack8<DT>(x + 8);
+    if constexpr (MANY) {
+      // q is more than the caches keep beside the pools.  8191 rows of 28 + 2 x 4 heads of 128: 29.1 us,
+      // 38.6 with ordinary stores (the attention behind it then finds q nearer: of both together, 189 and 187)
+      __builtin_nontemporal_store(__builtin_bit_cast(u32x4_t, o1), (u32x4_t*)(o + 8 * c));
+      __builtin_nontemporal_store(__builtin_bit_cast(u32x4_t, o2), (u32x4_t*)(o + D / 2 + 8 * c));
+    } else {
+      *(uint4*)(o + 8 * c) = o1;
+      *(uint4*)(o + D / 2 + 8 * c) = o2;
+    }
     return;
   }
-  // ---- the runs of one head of k or v that begin in `span` rows
+  // ---- the runs of one head of k or v that begin in SPAN rows
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const uint32_t spans = ((uint32_t)A.rows + A.span - 1) / A.span;
-  const uint32_t unit = (blockIdx.x - q_blocks) * kAppendWaves + w;  // (the grid's threads fit 32 bits)
+  const uint32_t unit = turn * kAppendWaves + w;  // (the grid's threads fit 32 bits)
   if (unit >= 2u * A.hkv * spans) return;
-  const int row0 = (int)(unit % spans) * A.span;
+  const int row0 = (int)(unit % spans) * SPAN;
   const int hh = unit / spans % A.hkv, is_v = unit / spans / A.hkv;
   uint64_t begins = 2;
-  if (A.span > 1) {
+  if constexpr (MANY) {
     // lane i: row row0 - 1 + i; one that follows another of its page begins no run
     const int at = row0 - 1 + lane;
-    const int64_t page = lane <= A.span && at >= 0 && at < A.rows ? A.slots[at] >> 4 : -1;
+    const int64_t page = lane <= SPAN && at >= 0 && at < A.rows ? A.slots[at] >> 4 : -1;
     const int64_t before = __shfl_up(page, 1);
     // (behind a row without a position the page's run may begin)
     begins = __ballot(lane > 0 && page >= 0 &&
@@ -228,6 +240,7 @@ __device__ void kv8_append_impl(const Kv8AppendArgs& A) {
     const int i = __builtin_ctzll(begins);
     begins &= begins - 1;
     wave_lds_sync();  // (the image again)
+    asm volatile("" ::: "memory");  // (norms and biases stay loads of every run: held in registers they cost occupancy)
     append_run<DT, D>(A, row0 - 1 + i, hh, is_v, s_image[w]);
   }
 }
@@ -275,8 +288,10 @@ __device__ void kv8_read_impl(const Kv8ReadArgs& A) {
     b = u.y;
   }
   uint16_t* const o = (is_v ? A.v_out : A.k_out) + row * A.out_stride + hh * D + 8 * c;
-  *(uint4*)o = make_uint4(kv8_pair<DT, false>(a, scale), kv8_pair<DT, true>(a, scale), kv8_pair<DT, false>(b, scale),
+  // (streamed: 32701 rows of 4 heads of 128 take 19.3 us, 23.8 with ordinary stores)
+  const uint4 y = make_uint4(kv8_pair<DT, false>(a, scale), kv8_pair<DT, true>(a, scale), kv8_pair<DT, false>(b, scale),
                           kv8_pair<DT, true>(b, scale));
+  __builtin_nontemporal_store(__builtin_bit_cast(u32x4_t, y), (u32x4_t*)o);
 }
 
 }  // namespace luc
@@ -284,7 +299,11 @@ __device__ void kv8_read_impl(const Kv8ReadArgs& A) {
 #define LUC_KV8_APPEND(DTN, DT, D)                                                              \
   extern "C" __global__ __launch_bounds__(256) void luc_kv8_append_##DTN##_d##D(                \
       luc::Kv8AppendArgs a) {                                                                   \
-    luc::kv8_append_impl<luc::DT, D>(a);                                                        \
+    luc::kv8_append_impl<luc::DT, D, false>(a);                                                 \
+  }                                                                                             \
+  extern "C" __global__ __launch_bounds__(256) void luc_kv8_append_many_##DTN##_d##D(           \
+      luc::Kv8AppendArgs a) {                                                                   \
+    luc::kv8_append_impl<luc::DT, D, true>(a);                                                  \
   }                                                                                             \
   extern "C" __global__ __launch_bounds__(256) void luc_kv8_read_##DTN##_d##D(luc::Kv8ReadArgs a) { \
     luc::kv8_read_impl<luc::DT, D>(a);                                                          \

@@ -845,7 +845,11 @@ __device__ void kv8_columns_impl(const Kv8AttnArgs& A) {
   // The chunks that see the longest contexts first, and split 0, which every chunk has, before the
   // others; neighbours of a pair on different XCDs (block x runs on XCD x % 8).
   const int pairs = A.batch * A.hkv;
-  const int split = blockIdx.x / (pairs * A.tiles), rest = blockIdx.x % (pairs * A.tiles);
+  const int split = blockIdx.x / (pairs * A.tiles);
+  int rest = blockIdx.x % (pairs * A.tiles);
+  // Every other 256 of them (a workgroup a CU) in reverse, so that the longest of one lot meet the shortest of
+  // the next: 4 x 1531..2048 rows, 14 and 2 heads of 64, 40.6 us, 42.6 without
+  if ((rest >> 8 & 1) && (rest | 255) < pairs * A.tiles) rest ^= 248;
   const int chunk = A.tiles - 1 - rest / pairs, bh = (rest + rest / pairs) % pairs;
   const int b = bh / A.hkv, kvh = bh % A.hkv;
   const KvSeq S = kv_seq(A, b);

@@ -77,17 +77,28 @@ struct SelectMem {
   uint32_t bin, before, length;
 };
 
+// x of the lanes that a DPP control names, `none` where it names no lane.
+template <int CTRL, int ROWS>
+__device__ inline uint32_t dpp_u32(uint32_t none, uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)x, CTRL, ROWS, 0xf, false);
+}
+// Inclusive f over the lanes before and of a lane: shifts inside rows of 16, then the rows' last lanes to those behind.
+template <class F>
+__device__ __attribute__((always_inline)) inline uint32_t wave_scan(uint32_t x, uint32_t none, F&& f) {
+  x = f(x, dpp_u32<0x111, 0xf>(none, x));
+  x = f(x, dpp_u32<0x112, 0xf>(none, x));
+  x = f(x, dpp_u32<0x114, 0xf>(none, x));
+  x = f(x, dpp_u32<0x118, 0xf>(none, x));
+  x = f(x, dpp_u32<0x142, 0xa>(none, x));
+  return f(x, dpp_u32<0x143, 0xc>(none, x));
+}
+
 // Inclusive sums over the threads of the workgroup, of N numbers; a barrier inside.  total: of all threads.
 template <int N>
 __device__ __attribute__((always_inline)) inline void block_scan(uint32_t (&x)[N], uint32_t (&total)[N], uint32_t (&part)[kSelWaves][kSelBatches]) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
 #pragma unroll
-  for (int k = 1; k < 64; k <<= 1)
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const uint32_t y = __shfl_up(x[n], k);
-      if (lane >= k) x[n] += y;
-    }
+  for (int n = 0; n < N; ++n) x[n] = wave_scan(x[n], 0, [](uint32_t a, uint32_t b) { return a + b; });
   if (lane == 63) {
 #pragma unroll
     for (int n = 0; n < N; ++n) part[w][n] = x[n];
@@ -146,12 +157,9 @@ __device__ __attribute__((always_inline)) inline void pick_pages(const uint32_t*
     lo = on ? min(lo, x) : lo;
     hi = x == ~0u ? hi : max(hi, x);
   });
-#pragma unroll
-  for (int n = 1; n < 64; n <<= 1) {
-    lo = min(lo, (uint32_t)__shfl_xor((int)lo, n));
-    hi = max(hi, (uint32_t)__shfl_xor((int)hi, n));
-  }
-  if (lane == 0) {
+  lo = wave_scan(lo, ~0u, [](uint32_t a, uint32_t b) { return min(a, b); });
+  hi = wave_scan(hi, 0, [](uint32_t a, uint32_t b) { return max(a, b); });
+  if (lane == 63) {
     s.list[w] = lo;
     s.list[kSelWaves + w] = hi;
   }
@@ -275,6 +283,10 @@ __device__ void kv8_select_impl(const Kv8SelectArgs& A) {
   if (u >= units) return;
   const int b = u % A.batch, chunk = u / A.batch;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int chunk_pages = 16 * kSelWaves * A.tiles;
+  const int p0 = chunk * chunk_pages + w * (16 * A.tiles);
+  const int32_t* const table = A.tables + (int64_t)b * A.table_stride;
+  int pages = table[min(p0 + lane, (A.max_ctx - 1) / kPage)];  // of the wave's next 64 (on their way beside the lengths)
   const KvSeq S = kv_seq(A, b);
   int32_t* const out = A.pages + ((int64_t)b * A.hkv + kvh) * A.budget;
   const int count = S.ctx == 0 || S.rows == 0 ? 0 : S.start / kPage + 1;  // pages of the context
@@ -283,7 +295,6 @@ __device__ void kv8_select_impl(const Kv8SelectArgs& A) {
       for (int i = threadIdx.x; i < A.budget; i += 64 * kSelWaves) out[i] = i < count ? i : -1;
     return;
   }
-  const int chunk_pages = 16 * kSelWaves * A.tiles;
   const int chunks = (count + chunk_pages - 1) / chunk_pages;
   if (chunk >= chunks) return;
   uint32_t* const keys = A.ws_key + ((int64_t)b * A.hkv + kvh) * A.max_pages;
@@ -292,9 +303,8 @@ __device__ void kv8_select_impl(const Kv8SelectArgs& A) {
 
   // ---- scores of 16 pages at a time, kSelTiles times 16 with their bounds one step ahead
   {
-    const int n = lane & 15, g = lane >> 4, p0 = chunk * chunk_pages + w * (16 * A.tiles);
+    const int n = lane & 15, g = lane >> 4;
     const int last = min(count, p0 + 16 * A.tiles);
-    const int32_t* const table = A.tables + (int64_t)b * A.table_stride;
     const int64_t base = (int64_t)A.layer * A.hkv + kvh;
     const int64_t stride = (int64_t)A.num_layers * A.hkv;
     // q of head n % 8, dimensions 64 i + 16 g + 8 k .. + 7
@@ -311,10 +321,9 @@ __device__ void kv8_select_impl(const Kv8SelectArgs& A) {
       float scale[kSelTiles];
       bool bad[kSelTiles];
     };
-    int pages = 0;  // of the wave's next 64
     auto load = [&](Step& T, int t0) __attribute__((always_inline)) {
       const int first = p0 + 16 * t0;
-      if (t0 % 4 == 0) pages = first + lane < last ? table[first + lane] : 0;
+      if (t0 && t0 % 4 == 0) pages = table[min(first + lane, last - 1)];
 #pragma unroll
       for (int t = 0; t < kSelTiles; ++t) {
         const int page = __shfl(pages, 16 * ((t0 + t) & 3) + n);

@@ -636,6 +636,7 @@ int luc_init(int device, const char* code_object_dir, luc_ctx** out_ctx) {
     }
     ctx->fns[n] = fn;
   }
+  for (const std::string& n : luc_internal::kv8_kernel_names()) ctx->kv8.push_back(ctx->fns[n]);
   if (hipDeviceGetAttribute(&ctx->num_cus, hipDeviceAttributeMultiprocessorCount, device) !=
           hipSuccess ||
       ctx->num_cus < 1)

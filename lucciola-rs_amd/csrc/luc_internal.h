@@ -16,6 +16,7 @@ struct luc_ctx {
   void* scratch = nullptr;  // this device's copy of the library scratch (luc_scratch.hip)
   std::vector<hipModule_t> modules;
   std::unordered_map<std::string, hipFunction_t> fns;
+  std::vector<hipFunction_t> kv8;  // of kv8_kernel_names(), in its order
 };
 
 namespace luc_internal {

@@ -13,7 +13,7 @@ namespace {
 struct Kv8AppendArgs : NormAppendArgs {
   float* scales;
   void* bounds;
-  int32_t span;
+  uint32_t every;
 };
 
 // luc::Kv8ReadArgs of kv8_append.hip: the same fields in the same order.
@@ -70,7 +70,7 @@ struct Kv8SelectArgs {
 
 constexpr int kCUs = 256;
 // Rows from which a wave of an append looks through 16 rows for runs, instead of through its own.
-constexpr int kAppendSpanRows = 512;
+constexpr int kAppendManyRows = 512;
 constexpr int kTokCols = 8;            // columns of a workgroup
 constexpr int kTokMaxSplits = 256;     // kv_split.h
 constexpr int kTokSlots = 2 * kCUs;    // workgroups that a launch is planned for: two a CU
@@ -88,7 +88,10 @@ constexpr int kColsOf64 = 128, kColsOf128 = 256;
 constexpr int kColsMinSplit64 = 512, kColsMinSplit128 = 256, kColsMaxSplits = 32;
 constexpr int64_t kMaxArrivals = 1 << 16;  // (sequence, kv head, column tile)
 constexpr int kSelPages = 4 * 16;          // pages of a workgroup's waves at once (kv8_select.hip)
-constexpr int kSelWorkgroups = 4 * kCUs;   // of a selection, before they take more pages each
+// Workgroups of a selection before they take more pages each, up to 16 times kSelPages.  64 contexts of 1024 to 16384
+// tokens, 8 kv heads, selection and attention over 96 pages: 45.5 us; planned for 256 49.9, 1024 47.2, 2048 49.4
+// (few end late, many start late).
+constexpr int kSelWorkgroups = 2 * kCUs;
 
 struct Kv8Plan {
   bool tokens = false;  // waves split tokens, else columns
@@ -143,6 +146,14 @@ size_t select_workspace_bytes(int batch, int max_ctx, int budget, int hkv) {
 }
 // Positions among the chosen pages' tokens.
 int chosen_ctx(int max_ctx, int budget) { return (int)std::min<int64_t>(max_ctx, (int64_t)budget * LUC_BLOCK_SIZE); }
+
+// The kernels of a type and head dimension, in this order.
+enum Kernel { kAppend, kAppendMany, kRead, kTokens, kChosen, kColumns, kMerge, kSelect, kKernels };
+constexpr const char* kKernelNames[kKernels] = {"append", "append_many", "read", "tokens", "chosen", "columns", "merge", "select"};
+// (by place: looking up their names would be a tenth of a launch)
+hipFunction_t kernel(const luc_ctx* ctx, Kernel k, int dtype, int head_dim) {
+  return ctx->kv8[((dtype == LUC_F16) * 2 + (head_dim == 128)) * kKernels + k];
+}
 
 bool sizes_fit(int hq, int hkv, int head_dim) {
   return hq > 0 && hkv > 0 && hq <= kMaxHeads && hq % hkv == 0 && hq / hkv <= 8 && (head_dim == 64 || head_dim == 128);
@@ -212,15 +223,11 @@ int attend(luc_ctx* ctx, void* stream, int dtype, int head_dim, const Kv8Plan& p
     a.ws_o = reinterpret_cast<float*>(
         ws + kMaxArrivals * 4 + align256(kv8_partials(plan, a.batch, a.total_rows, a.hkv, a.group) * 8));
   }
-  const std::string suffix = std::string(dt_name(dtype)) + "_d" + std::to_string(head_dim);
-  hipFunction_t fn, merge;
-  const char* const kind = a.chosen ? "luc_kv8_chosen_" : plan.tokens ? "luc_kv8_tokens_" : "luc_kv8_columns_";
-  if (int rc = get_fn(ctx, kind + suffix, &fn)) return rc;
-  if (int rc = get_fn(ctx, "luc_kv8_merge_" + suffix, &merge)) return rc;
+  const hipFunction_t fn = kernel(ctx, a.chosen ? kChosen : plan.tokens ? kTokens : kColumns, dtype, head_dim);
   void* args[] = {&a};
   if (int rc = launch(fn, dim3((unsigned)(units * plan.splits)), dim3((unsigned)threads), stream, args)) return rc;
   if (plan.tokens || plan.splits == 1) return LUC_OK;
-  return launch(merge, dim3((unsigned)ceil_div(items, 1024 / head_dim)), dim3(256), stream, args);
+  return launch(kernel(ctx, kMerge, dtype, head_dim), dim3((unsigned)ceil_div(items, 1024 / head_dim)), dim3(256), stream, args);
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -232,9 +239,7 @@ std::vector<std::string> kv8_kernel_names() {
   std::vector<std::string> names;
   for (const char* dt : {"bf16", "f16"})
     for (const char* d : {"_d64", "_d128"})
-      for (const char* kind : {"luc_kv8_append_", "luc_kv8_read_", "luc_kv8_tokens_", "luc_kv8_chosen_",
-                               "luc_kv8_columns_", "luc_kv8_merge_", "luc_kv8_select_"})
-        names.push_back(std::string(kind) + dt + d);
+      for (const char* kind : kKernelNames) names.push_back(std::string("luc_kv8_") + kind + "_" + dt + d);
   return names;
 }
 }  // namespace luc_internal
@@ -251,19 +256,20 @@ int luc_kv8_append(luc_ctx* ctx, void* stream, int dtype, const void* q, const v
   Kv8AppendArgs a{{q, k, v, row_stride, q_bias, k_bias, v_bias, q_norm, k_norm, cos_table, sin_table, positions,
                    slots, q_out, q_out_stride, nullptr, nullptr, 0, k_pool, v_pool, 0, eps, num_tokens, max_pos,
                    layer, num_layers, num_q_heads, num_kv_heads},
-                  scales, bounds, num_tokens > kAppendSpanRows ? 16 : 1};
+                  scales, bounds, 1};
   if (int rc = check_append(ctx, dtype, a, num_blocks, head_dim, block_size)) return rc;
   if (int rc = check_pools(k_pool, v_pool, scales, num_layers, num_kv_heads, head_dim)) return rc;
   if (!aligned(bounds, 16)) return fail(LUC_E_INVALID, "bounds must be 16-byte aligned");
   if (num_tokens == 0) return LUC_OK;
-  // q: head_dim / 16 lanes a head; then a wave for every span of rows of every k and v head
-  const int64_t grid = ceil_div((int64_t)num_tokens * num_q_heads, 4096 / head_dim) +
-                       ceil_div(ceil_div(num_tokens, a.span) * num_kv_heads * 2, 4);
+  // q: head_dim / 16 lanes a head; a wave for every row, or 16, of every k and v head
+  const bool many = num_tokens > kAppendManyRows;
+  const int64_t runs = ceil_div(ceil_div(num_tokens, many ? 16 : 1) * num_kv_heads * 2, 4);
+  const int64_t grid = ceil_div((int64_t)num_tokens * num_q_heads, 4096 / head_dim) + runs;
+  // the blocks of runs evenly among q's, an odd number apart: block x runs on XCD x % 8
+  a.every = (uint32_t)std::min<int64_t>((grid / runs - 1) | 1, 1 << 30);
   if (grid * 256 > UINT32_MAX) return fail(LUC_E_INVALID, "too many rows for one launch");
   if (int rc = check_device(ctx)) return rc;
-  hipFunction_t fn;
-  if (int rc = get_fn(ctx, std::string("luc_kv8_append_") + dt_name(dtype) + "_d" + std::to_string(head_dim), &fn))
-    return rc;
+  const hipFunction_t fn = kernel(ctx, many ? kAppendMany : kAppend, dtype, head_dim);
   void* args[] = {&a};
   return launch(fn, dim3((unsigned)grid), dim3(256), stream, args);
 }
@@ -284,9 +290,7 @@ int luc_kv8_read(luc_ctx* ctx, void* stream, int dtype, void* k_out, void* v_out
   const int64_t threads = (int64_t)num_tokens * num_kv_heads * (head_dim / 8) * 2;
   if (threads + 256 > UINT32_MAX) return fail(LUC_E_INVALID, "too many rows for one launch");
   if (int rc = check_device(ctx)) return rc;
-  hipFunction_t fn;
-  if (int rc = get_fn(ctx, std::string("luc_kv8_read_") + dt_name(dtype) + "_d" + std::to_string(head_dim), &fn))
-    return rc;
+  const hipFunction_t fn = kernel(ctx, kRead, dtype, head_dim);
   Kv8ReadArgs a{k_out, v_out, out_row_stride, slots, k_pool, v_pool, scales, (int64_t)num_blocks * LUC_BLOCK_SIZE,
                 num_tokens, layer, num_layers, num_kv_heads};
   void* args[] = {&a};
@@ -371,9 +375,7 @@ int luc_kv8_select(luc_ctx* ctx, void* stream, int dtype, int32_t* pages, int bu
     a.ws_cnt = static_cast<int32_t*>(workspace);
     a.ws_key = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + kMaxArrivals * 4);
   }
-  hipFunction_t fn;
-  if (int rc = get_fn(ctx, std::string("luc_kv8_select_") + dt_name(dtype) + "_d" + std::to_string(head_dim), &fn))
-    return rc;
+  const hipFunction_t fn = kernel(ctx, kSelect, dtype, head_dim);
   void* args[] = {&a};
   return launch(fn, dim3((unsigned)grid), dim3(256), stream, args);
 }

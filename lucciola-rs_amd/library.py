@@ -567,14 +567,21 @@ class LucAttn:
     def _kv8_pools(self, k_pool, v_pool, scales, num_layers, hkv, head_dim, num_blocks, dev):
         """(k address, v address, scales address, pages) of 8-bit pools: uint8 [pages, layers, kv heads,
         16 * head_dim], scales float32 [pages, layers, kv heads, 2]."""
-        shape = k_pool.shape
-        if len(shape) != 4 or shape[1:] != (num_layers, hkv, 16 * head_dim) or v_pool.shape != shape:
-            raise ValueError(f"8-bit pools {tuple(shape)}, {tuple(v_pool.shape)}: want [pages, {num_layers}, {hkv}, "
-                             f"{16 * head_dim}]")
-        if scales.shape != (*shape[:3], 2):
-            raise ValueError(f"scales {tuple(scales.shape)}: want {(*shape[:3], 2)}")
-        return (self._array("k_pool", k_pool, torch.uint8, dev, 0), self._array("v_pool", v_pool, torch.uint8, dev, 0),
-                self._array("scales", scales, torch.float32, dev, 0), self._pages_of(shape[0], num_blocks))
+        pages, u8 = len(k_pool), torch.uint8
+        want = (pages, num_layers, hkv, 16 * head_dim)
+        if k_pool.shape != want or v_pool.shape != want:
+            raise ValueError(f"8-bit pools {tuple(k_pool.shape)}, {tuple(v_pool.shape)}: want {('pages', *want[1:])}")
+        if scales.shape != (pages, num_layers, hkv, 2):
+            raise ValueError(f"scales {tuple(scales.shape)}: want {(pages, num_layers, hkv, 2)}")
+        # (one test for the three: a call of its own for each would cost a fifth of a launch)
+        if k_pool.dtype is not u8 or v_pool.dtype is not u8 or scales.dtype is not torch.float32 or \
+                k_pool.get_device() != dev or v_pool.get_device() != dev or scales.get_device() != dev or \
+                not (k_pool.is_contiguous() and v_pool.is_contiguous() and scales.is_contiguous()):
+            for name, x, dtype in (("k_pool", k_pool, u8), ("v_pool", v_pool, u8), ("scales", scales, torch.float32)):
+                self._array(name, x, dtype, dev, 0)
+        if num_blocks is not None:
+            pages = self._pages_of(pages, num_blocks)
+        return k_pool.data_ptr(), v_pool.data_ptr(), scales.data_ptr(), pages
 
     @staticmethod
     def _pages_of(pages, num_blocks):
@@ -634,16 +641,22 @@ class LucAttn:
         return self._zeros(self.lib.luc_kv8_sparse_workspace_size(batch, max_ctx, budget, hq, hkv, head_dim), device)
 
     def _batch_args(self, tables, start_pos, cu_seqlens, batch, dev):
-        arr, i32, stride = self._array, torch.int32, tables.shape[-1]
-        return (arr("tables", tables, i32, dev, batch * stride), stride,
-                cu_seqlens if cu_seqlens is None else arr("cu_seqlens", cu_seqlens, i32, dev, batch + 1),
-                arr("start_pos", start_pos, i32, dev, batch))
+        i32, stride = torch.int32, tables.shape[-1]
+        if tables.dtype is not i32 or start_pos.dtype is not i32 or tables.get_device() != dev or \
+                start_pos.get_device() != dev or tables.numel() < batch * stride or start_pos.numel() < batch or \
+                not (tables.is_contiguous() and start_pos.is_contiguous()):
+            self._array("tables", tables, i32, dev, batch * stride)
+            self._array("start_pos", start_pos, i32, dev, batch)
+        return (tables.data_ptr(), stride,
+                cu_seqlens if cu_seqlens is None else self._array("cu_seqlens", cu_seqlens, i32, dev, batch + 1),
+                start_pos.data_ptr())
 
     def _workspace_args(self, workspace, dev):
         if workspace is None:
             return None, 0
-        return (self._array("workspace", workspace, workspace.dtype, dev, 0),
-                workspace.numel() * workspace.element_size())
+        if workspace.get_device() != dev or not workspace.is_contiguous():
+            self._array("workspace", workspace, workspace.dtype, dev, 0)
+        return workspace.data_ptr(), workspace.nbytes
 
     def kv8_attention(self, out, q, k_pool, v_pool, scales, tables, start_pos, batch, total_rows, max_rows,
                       max_ctx, layer, num_layers, hq, hkv, head_dim, sm_scale, cu_seqlens=None,
