@@ -428,9 +428,12 @@ __device__ void kv8_tokens_impl(const Kv8AttnArgs& A) {
     const int units = A.batch * A.hkv * A.tiles;
     split = blockIdx.x / units;
     const int u = blockIdx.x % units;
-    tile = u % A.tiles;
-    b = u / A.tiles / A.hkv;
-    kvh = u / A.tiles % A.hkv;
+    // the tiles of a (sequence, kv head) lie whole pairs apart: where there are eight, on one XCD, whose L2 has the pages
+    // for all but the first (two tiles over 16 x 4096 tokens of 8 heads of 128: 39.0 us, side by side 48.2)
+    const int pairs = A.batch * A.hkv;
+    tile = u / pairs;
+    b = u % pairs / A.hkv;
+    kvh = u % A.hkv;
     S = kv_seq(A, b);
   }
   const int unit = (b * A.hkv + kvh) * A.tiles + tile;

@@ -4,6 +4,7 @@
 #include "luc_internal.h"
 
 #include <algorithm>
+#include <cmath>
 
 using namespace luc_internal;
 
@@ -69,22 +70,34 @@ struct Kv8SelectArgs {
 };
 
 constexpr int kCUs = 256;
-// Rows from which a wave of an append looks through 16 rows for runs, instead of through its own.
+// Rows from which a wave of an append looks through 16 rows for runs, instead of through its own.  28 + 2 x 4 heads of
+// 128, us by either: 256 rows 6.1 and 5.8, 512 6.4 and 6.3, 1024 6.9 and 8.2, 4096 15.6 and 24.8.
 constexpr int kAppendManyRows = 512;
-constexpr int kTokCols = 8;            // columns of a workgroup
-constexpr int kTokMaxSplits = 256;     // kv_split.h
-constexpr int kTokSlots = 2 * kCUs;    // workgroups that a launch is planned for: two a CU
-// Split lengths of a tokens launch: what fills the chip once, but not shorter than is worth a merge
-// and not longer than lets mixed contexts end together.
-constexpr int kTokMinSplit = 256, kTokMaxSplit = 2048;
-constexpr int kTokRounds = 8;  // rounds of workgroups balance any contexts: longer splits beyond
-// Up to 16 columns go to the tokens kernel, which reads the cache once for each 8; up to 48 while its
-// tiles leave the chip room.
-constexpr int kTokMostCols = 48;
+constexpr int kTokCols = 8;          // columns of a workgroup
+constexpr int kTokMaxSplits = 256;   // kv_split.h
+constexpr int kTokSlots = 2 * kCUs;  // workgroups that a launch is planned for: two a CU (three or four: no faster)
+// Split lengths of a tokens launch: what fills the chip once, but not longer than lets mixed contexts end together (64
+// contexts of 8192, 7 heads of 64 a group: 24.3 us, 28.1 of splits to 1024; 128 mixed up to 8192, 7 of 128: 107.8,
+// 111.8 to 1024, 111.5 to 4096), nor shorter than is worth a merge.  A workgroup takes 0.0048 us a token, a
+// merge 0.13 us a split, so a single context is quickest in splits of sqrt(26 ctx): of 32768 tokens 11.0 us, 16.0 in splits of
+// 256; of 8192 9.9, 10.7 in 256, 11.4 in 1024; of 2048 8.1, 9.0 in 512.  Up to 512 tokens a second split costs more
+// than it saves: 6.3 us, 7.8 in two.
+constexpr int kTokOneSplit = 512, kTokMaxSplit = 2048, kTokSplitRate = 26;
+// Beyond so many rounds of workgroups splits grow again: any contexts balance (200 mixed contexts: equal with
+// 4, 8 and 16).
+constexpr int kTokRounds = 8;
+// Up to 16 columns go to the tokens kernel, which reads the cache once for each 8, and more of them while it reads at
+// most this: 5.4 TB/s from the L2 of an XCD, or 5.6 ns a workgroup, as many bytes as kTokLeastBytes, where contexts are
+// short.  The columns kernel reads the cache once, and takes 6 to 10 us more to begin.  28 / 4 heads of 128, us by tokens
+// and by columns: 64 rows of a context of 64 5.3 and 12.5, 256 of 256 11.2 and 18.1, 64 of 2048 (112 MiB) 17.9
+// and 22.0, 3 of each of 16 x 4096 (192 MiB) 36 and 30.7, 8 sequences of 64 rows (168) 14.4 and 13.0, 32 of 16 13.8 and 9.9.
+constexpr int64_t kTokMostBytes = 128 << 20, kTokLeastBytes = 96 << 10;
 // Columns of a workgroup of the columns kernel (Kv8Cols).
 constexpr int kColsOf64 = 128, kColsOf128 = 256;
 // Its splits fill the chip once, planned as a workgroup a CU (128) or two (64, whose registers hold three), but
-// are not shorter than pays for their partials.
+// are not shorter than pays for their partials: of 64, 200 rows at the end of each of 4 x 1024 tokens 19.4 us, 21.0
+// in splits of 256 and of 1024; of 128, 512 rows on 4096 47.7, 48.6 in 512.  No more than 32: 128 rows on 16384
+// 46.5, 69.5 with 8, 46.5 with 128.
 constexpr int kColsMinSplit64 = 512, kColsMinSplit128 = 256, kColsMaxSplits = 32;
 constexpr int64_t kMaxArrivals = 1 << 16;  // (sequence, kv head, column tile)
 constexpr int kSelPages = 4 * 16;          // pages of a workgroup's waves at once (kv8_select.hip)
@@ -107,13 +120,14 @@ Kv8Plan kv8_plan(int batch, int total_rows, int max_rows, int max_ctx, int hkv, 
   const int64_t cols = (int64_t)std::min(max_rows, total_rows) * group;
   const int64_t pairs = (int64_t)batch * hkv;
   const int64_t units = pairs * ceil_div(cols, kTokCols);
-  p.tokens = units <= kMaxArrivals && (cols <= 2 * kTokCols || (cols <= kTokMostCols && units <= kTokSlots));
+  p.tokens = units <= kMaxArrivals && (cols <= 2 * kTokCols || units * std::max((int64_t)max_ctx * 2 * head_dim, kTokLeastBytes) <= kTokMostBytes);
   if (p.tokens) {
     p.tiles = (int)ceil_div(cols, kTokCols);
     // a stage for each of 4 waves
     const int round = head_dim == 64 ? 256 : 128;
     const int64_t fill = units * max_ctx / kTokSlots;
-    int64_t st = std::min<int64_t>(std::max<int64_t>(fill, kTokMinSplit), kTokMaxSplit);
+    int64_t st = max_ctx <= kTokOneSplit ? kTokOneSplit : (int64_t)std::sqrt((double)kTokSplitRate * max_ctx);
+    st = std::min<int64_t>(std::max(fill, st), kTokMaxSplit);
     st = std::max({st, fill / kTokRounds, ceil_div(max_ctx, kTokMaxSplits)});
     p.split_tokens = (int)(ceil_div(st, round) * round);
     p.longest_first = p.tiles == 1 && batch <= 64 && units * ceil_div(max_ctx, p.split_tokens) > kTokSlots;

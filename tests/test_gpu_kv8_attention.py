@@ -60,9 +60,15 @@ def make_q(c, total, hq, dtype, seed=1, std=1.4, extra=0):
 
 
 def run(luc, c, rows, hq, dtype, seed=1, max_ctx=None, max_rows=None, packed=True, tail=0, q_std=1.4, scale=None,
-        q=None, q_extra=0, out_extra=0, ws=None, stream=None, start=None, tables=None, num_blocks=None):
-    """Rows of every sequence at the end of its context: (q, out, scale)."""
-    n, total = len(c.ctx), sum(rows) + tail
+        q=None, q_extra=0, out_extra=0, ws=None, stream=None, start=None, tables=None, num_blocks=None, columns=False):
+    """Rows of every sequence at the end of its context: (q, out, scale).  columns: sizes of a call that allows for
+    so many rows that it goes to the kernel for prompts, whatever rows there are."""
+    n = len(c.ctx)
+    if columns:
+        tail = max(tail, 12000 // (n * hq))
+        max_rows = max_rows or sum(rows) + tail
+        q = q if q is None or len(q) == sum(rows) + tail else torch.cat([q, q[:1].expand(tail, -1)])
+    total = sum(rows) + tail
     q = make_q(c, total, hq, dtype, seed, q_std, q_extra) if q is None else q
     out = torch.full((total, hq * c.d + out_extra), 7.0, dtype=DT[dtype], device="cuda")
     cu = torch.tensor(np.concatenate([[0], np.cumsum(rows)]), dtype=torch.int32, device="cuda") if packed else None
@@ -122,44 +128,58 @@ def test_rows_against_64_bit_attention(luc, hq, hkv, d, ctx, rows, dtype):
     c = Cache(ctx, hkv, d, seed=sum(rows))
     q, out, scale = run(luc, c, rows, hq, dtype, tail=3, q_extra=8, out_extra=4)
     verify(c, rows, hq, dtype, q, out, scale)
+    q, out, scale = run(luc, c, rows, hq, dtype, q_extra=8, out_extra=4, columns=True)
+    verify(c, rows, hq, dtype, q, out, scale)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("ctx,rows", [([4100], [230]), ([6000, 3500, 40], [100, 90, 1]), ([1100, 5000], [2, 200])],
+                         ids=lambda x: "_".join(map(str, x)))
+@pytest.mark.parametrize("hq,hkv,d", HEADS)
+def test_rows_over_long_contexts(luc, hq, hkv, d, ctx, rows, dtype):
+    """Prompts' rows whose contexts are split."""
+    c = Cache(ctx, hkv, d, seed=sum(rows))
+    q, out, scale = run(luc, c, rows, hq, dtype, tail=1)
+    verify(c, rows, hq, dtype, q, out, scale)
 
 
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("rows", [[1, 1], [3, 2], [90, 33]])
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
-def test_scales_and_large_scores(luc, d, rows, dtype):
+@pytest.mark.parametrize("columns", [False, True])
+def test_scales_and_large_scores(luc, d, rows, dtype, columns):
     """Scores of both signs far from 0 (the running maximum moves), a negative scale, a query of zeros, and
     pages whose sizes differ by up to 2^20."""
     c = Cache([700, 650], 2, d, seed=3, k_std=4.0)
     for scale, std in ((0.5, 4.0), (-0.25, 4.0), (1.0, 0.0), (3e-3, 200.0), (0.0, 1.0)):
-        q, out, _ = run(luc, c, rows, 6, dtype, q_std=std, scale=scale)
+        q, out, _ = run(luc, c, rows, 6, dtype, q_std=std, scale=scale, columns=columns)
         verify(c, rows, 6, dtype, q, out, scale)
     c = Cache([700, 650], 2, d, seed=4, k_std=0.02, v_std=1.0, spread=5)
-    q, out, scale = run(luc, c, rows, 6, dtype)
+    q, out, scale = run(luc, c, rows, 6, dtype, columns=columns)
     verify(c, rows, 6, dtype, q, out, scale)
     c = Cache([300, 150], 2, d, seed=5, v_std=2.0 ** -9)  # values near fp16's subnormals
-    q, out, scale = run(luc, c, rows, 6, dtype)
+    q, out, scale = run(luc, c, rows, 6, dtype, columns=columns)
     verify(c, rows, 6, dtype, q, out, scale)
 
 
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
-@pytest.mark.parametrize("ctx,n", [(40, 1), (40, 3), (200, 70)])
-def test_values_that_are_not_numbers(luc, d, ctx, n, dtype):
+@pytest.mark.parametrize("ctx,n,columns", [(40, 1, False), (40, 3, False), (200, 70, False), (40, 3, True), (200, 70, True)])
+def test_values_that_are_not_numbers(luc, d, ctx, n, dtype, columns):
     """A NaN of V reaches its dimension of the rows that see its token, and nothing else; one of K the whole
     row's head.  Rows before it are as if it were not there."""
     hq = 8
     start = ctx - n
     t = start + n // 2          # between the rows' limits (the row's own token, for one)
     c = Cache([ctx], 2, d, seed=7)
-    q, clean, scale = run(luc, c, [n], hq, dtype)
+    q, clean, scale = run(luc, c, [n], hq, dtype, columns=columns)
     page, off = int(c.tables[0, t // PAGE]), t % PAGE
     dim = 37
     c.vp[page, c.layer, 0, (off // 4 * d + dim) * 4 + off % 4] = 0xFF
     u = start + n - 1           # the last row's own
     c.kp[int(c.tables[0, u // PAGE]), c.layer, 1, (u % PAGE) * d + 5] = 0x7F
-    _, out, _ = run(luc, c, [n], hq, dtype, q=q)
-    o, w = out.view(n, hq, d), clean.view(n, hq, d)
+    _, out, _ = run(luc, c, [n], hq, dtype, q=q, columns=columns)
+    o, w = out[:n].view(n, hq, d), clean[:n].view(n, hq, d)
     rest = [x for x in range(d) if x != dim]
     assert torch.equal(o[:, :4, rest], w[:, :4, rest])
     assert torch.equal(o[:t - start, :4], w[:t - start, :4])
@@ -170,29 +190,30 @@ def test_values_that_are_not_numbers(luc, d, ctx, n, dtype):
     page = int(c.tables[0, 0])
     c.vp[page, c.layer, 1, (0 * d + 11) * 4 + 2] = 0x7F
     if n < 10:
-        _, out, _ = run(luc, c, [n], hq, dtype, q=q)
-        assert bool(out.view(n, hq, d)[:, 4:, 11].isnan().all())
+        _, out, _ = run(luc, c, [n], hq, dtype, q=q, columns=columns)
+        assert bool(out[:n].view(n, hq, d)[:, 4:, 11].isnan().all())
 
 
 @pytest.mark.parametrize("d", [64, 128])
-@pytest.mark.parametrize("rows", [[1, 1, 1, 1], [2, 3, 1, 4], [60, 70, 1, 50]])
-def test_contexts_out_of_bounds_are_nan(luc, d, rows):
+@pytest.mark.parametrize("rows,columns", [([1, 1, 1, 1], False), ([2, 3, 1, 4], False), ([60, 70, 1, 50], False),
+                                          ([2, 3, 1, 4], True), ([60, 70, 1, 50], True)])
+def test_contexts_out_of_bounds_are_nan(luc, d, rows, columns):
     """Contexts past max_ctx, negative positions, more rows than max_rows, pages outside the pool."""
     c = Cache([300, 200, 150, 400], 2, d, seed=5)
     hq = 10
-    q, clean, scale = run(luc, c, rows, hq, "bf16")
+    q, clean, scale = run(luc, c, rows, hq, "bf16", columns=columns)
     verify(c, rows, hq, "bf16", q, clean, scale)
     ends = np.cumsum(rows)
     seq = [slice(e - r, e) for e, r in zip(ends, rows)]
-    _, out, _ = run(luc, c, rows, hq, "bf16", q=q, max_ctx=350)
+    _, out, _ = run(luc, c, rows, hq, "bf16", columns=columns, q=q, max_ctx=350)
     assert bool(out[seq[3]].isnan().all()) and bool(out[:ends[2]].isfinite().all())
     start = [x - r for x, r in zip(c.ctx, rows)]
-    _, out, _ = run(luc, c, rows, hq, "bf16", q=q, start=[start[0], -1, start[2], -(1 << 31)])
+    _, out, _ = run(luc, c, rows, hq, "bf16", columns=columns, q=q, start=[start[0], -1, start[2], -(1 << 31)])
     assert bool(out[seq[1]].isnan().all()) and bool(out[seq[3]].isnan().all())
     verify(c, rows, hq, "bf16", q, out, scale, skip=(1, 3))
     if max(rows) > 1:
         most = sorted(rows)[-2]
-        _, out, _ = run(luc, c, rows, hq, "bf16", q=q, max_rows=most)
+        _, out, _ = run(luc, c, rows, hq, "bf16", columns=columns, q=q, max_rows=most)
         big = rows.index(max(rows))
         assert bool(out[seq[big]].isnan().all())
         verify(c, rows, hq, "bf16", q, out, scale, skip=(big,))
@@ -200,14 +221,14 @@ def test_contexts_out_of_bounds_are_nan(luc, d, rows):
     tables = c.dev_tables.clone()
     tables[0, 6] = -1
     tables[3, 24] = c.pages
-    _, out, _ = run(luc, c, rows, hq, "bf16", q=q, tables=tables)
+    _, out, _ = run(luc, c, rows, hq, "bf16", columns=columns, q=q, tables=tables)
     assert bool(out[seq[0]].isnan().all())
     verify(c, rows, hq, "bf16", q, out, scale, skip=(0, 3))
     first = max(0, 384 - (400 - rows[3]))
     assert bool(out[seq[3]][first:].isnan().all())
     assert torch.equal(out[seq[3]][:first], clean[seq[3]][:first])
     # a pool of fewer pages than the tables name
-    _, out, _ = run(luc, c, rows, hq, "bf16", q=q, num_blocks=int(c.tables[2, :10].max()))
+    _, out, _ = run(luc, c, rows, hq, "bf16", columns=columns, q=q, num_blocks=int(c.tables[2, :10].max()))
     assert bool(out[seq[2]].isnan().all())
 
 
@@ -228,7 +249,7 @@ def test_one_workspace_for_calls_of_other_sizes(luc):
     assert all(torch.equal(a, b) for a, b in zip(chosen, again))
 
 
-@pytest.mark.parametrize("rows", [[1, 1, 1], [50, 70, 1]])
+@pytest.mark.parametrize("rows", [[1, 1, 1], [50, 70, 1], [150, 200, 170]])
 def test_another_stream_and_a_captured_call(luc, rows):
     c = Cache([900, 1500, 200], 2, 128, seed=7)
     q, want, scale = run(luc, c, rows, 12, "bf16")
