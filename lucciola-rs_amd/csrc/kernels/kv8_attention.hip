@@ -26,6 +26,18 @@
 // Either may cut the context into splits over workgroups, whose partial (m, l, o) go to the
 // workspace; tokens: the last workgroup of a (sequence, kv head, column tile) to arrive
 // merges them; columns: a second launch does.
+//
+// What bounds them (us).  Tokens: HBM where contexts are long: 64 rows over 1024 to 16384 tokens, 4 kv heads of 128, 110 for
+// 612 MB, 5.6 TB/s; a gather of the same slabs without arithmetic takes 96, a copy's rate 120.  Loads marked as
+// streamed: 110, 120 without.  No slower with two workgroups a CU than with three; K by 1 KB a wave
+// in another slab order 108.  The first 512 workgroups read 6.7 TB/s, the tail from 75 us on is what is lost.  Few tokens: a
+// chain of round trips, lengths -> table -> scale, K -> products -> merge of the waves, and of splits by way of the
+// workspace: 5.6 for 512 tokens, 11 for 32 rows over up to 4096.
+// Columns: issue.  512 rows after 8000, 12 / 2 heads of 128 (fp16): 36.6 and 7.7 for the merge of ten splits, 31 MB each way;
+// four prompts of 1531 to 2048, 14 / 2 heads of 64 (bf16): 40.4; matrix instructions busy
+// 38% and 32% of the SIMDs' time, VALU instructions, two thirds of their cycles exponentials, 47% and 64%: the two
+// hardly run at once whatever the waves.  Both halves of a tile at a time spill (53), wave priorities changed nothing; chunks of
+// columns in serpentine order of their lengths 40.4, in plain order 42.6.
 #include "kv8.h"
 #include "kv_split.h"
 

@@ -18,6 +18,13 @@
 // the keys' range finds the part that the last chosen one lies in; the keys there, a few, are ranked by every wave for
 // itself (many: another histogram over that part).  Then every thread writes those above, and of those equal to it the
 // first, to their places, which sums over the threads before it give.
+//
+// What bounds it: round trips, not bytes.  One context of 32768 tokens, 2 kv heads of 128 (1 MB of bounds): 10.5 us, about
+// 5 until the scores are stored (lengths and table beside each other, then bounds, products), 2 for the arrival and the keys,
+// 3.5 for the pick's four passes and barriers.  64 contexts of 1024 to 16384, 4 heads: 20.3 us for 36 MB of bounds, the
+// chain of the longest contexts' steps; with four tiles of bounds on their way instead of two 22, with streaming loads
+// of them 25.6.  Scans by DPP and the early table read took 1.0 us off either; by shuffles and four compare
+// passes over the bits of the keys the pick alone took 11.
 #include "kv8.h"
 #include "kv_split.h"
 

@@ -102,8 +102,8 @@ constexpr int kColsMinSplit64 = 512, kColsMinSplit128 = 256, kColsMaxSplits = 32
 constexpr int64_t kMaxArrivals = 1 << 16;  // (sequence, kv head, column tile)
 constexpr int kSelPages = 4 * 16;          // pages of a workgroup's waves at once (kv8_select.hip)
 // Workgroups of a selection before they take more pages each, up to 16 times kSelPages.  64 contexts of 1024 to 16384
-// tokens, 8 kv heads, selection and attention over 96 pages: 45.5 us; planned for 256 49.9, 1024 47.2, 2048 49.4
-// (few end late, many start late).
+// tokens, 4 kv heads of 128, selection and attention over 96 pages: 44.4 us; planned for 1024 46.0, for 256 and
+// 2048 some 4 more (few end late, many start late).
 constexpr int kSelWorkgroups = 2 * kCUs;
 
 struct Kv8Plan {
