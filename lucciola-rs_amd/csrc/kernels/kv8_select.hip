@@ -9,7 +9,7 @@
 //   score = max over the group's heads of (((S_0 2^e_0 + S_1 2^e_1) + S_2 2^e_2) + S_3 2^e_3) * scale_K
 // rounds its few sums in f32, in that order: the choice is a function of the inputs, whatever computes it.
 //
-// A workgroup scores 128 pages of one (sequence, kv head) or more; the last of them to arrive picks.  Lane (n, g) of a wave loads
+// A workgroup scores 64 pages of one (sequence, kv head) or more; the last of them to arrive picks.  Lane (n, g) of a wave loads
 // bounds 64 i + 16 g .. + 15 of page n of 16; those belong to group 2 i + g / 2, so of the 16 columns of
 // v_mfma_f32_16x16x32_f16 the lower 8 take the heads' even groups (q is 0 in lanes of the odd ones) and the upper
 // 8 the same heads' odd groups.
@@ -19,12 +19,12 @@
 // itself (many: another histogram over that part).  Then every thread writes those above, and of those equal to it the
 // first, to their places, which sums over the threads before it give.
 //
-// What bounds it: round trips, not bytes.  One context of 32768 tokens, 2 kv heads of 128 (1 MB of bounds): 10.5 us, about
-// 5 until the scores are stored (lengths and table beside each other, then bounds, products), 2 for the arrival and the keys,
-// 3.5 for the pick's four passes and barriers.  64 contexts of 1024 to 16384, 4 heads: 20.3 us for 36 MB of bounds, the
-// chain of the longest contexts' steps; with four tiles of bounds on their way instead of two 22, with streaming loads
-// of them 25.6.  Scans by DPP and the early table read took 1.0 us off either; by shuffles and four compare
-// passes over the bits of the keys the pick alone took 11.
+// What bounds it: round trips, then bytes and instructions alike.  One context of 32768 tokens, 2 kv heads of 128 (1 MB of
+// bounds): 9.2 us, about 4 until the scores are stored (lengths and table beside each other, then bounds, products), 1.5
+// for the arrival, 3.4 for the pick's passes and barriers.  64 contexts of 1024 to 16384, 4 heads: 17.9 us for
+// 36 MB of bounds, of which 6.7 are the steps of the longest contexts; with codes rounded to units by additions and a
+// reduction over the heads page by page 20.3, with streaming loads of the bounds 5 more; four tiles of bounds on their way are no
+// better than one.  By shuffles and compare passes over the bits of the keys the pick alone took 11.
 #include "kv8.h"
 #include "kv_split.h"
 
@@ -44,26 +44,20 @@ struct Kv8SelectArgs {
   uint32_t* ws_key;           // [batch][hkv][max_pages], that a multiple of 4
   int32_t batch, total_rows, max_rows, max_ctx, layer, num_layers, hkv, group, num_blocks;
   int32_t budget, first, recent, chunks, max_pages;
-  int32_t tiles;  // of 16 pages a wave: a multiple of kSelTiles
+  int32_t tiles;  // of 16 pages a wave
 };
 
 constexpr int kSelWaves = 4;
-constexpr int kSelTiles = 2;  // of 16 pages, whose bounds a wave loads at once
 constexpr int kDppRowRor8 = 0x128;
 constexpr int kSelBatch = 4 * 64 * kSelWaves, kSelBatches = 4;  // keys that a pick reads at once
 constexpr int kSelBinBits = 10, kSelBins = 1 << kSelBinBits;
 
-// Whole numbers as packed fp16: codes rounded to units.  |x| <= 448, and from 1024 to 2048 fp16 has no fractions.
-__device__ inline uint32_t whole2(uint32_t w) {
-  const half2_t big = {(_Float16)1536.0f, (_Float16)1536.0f};
-  half2_t x = __builtin_bit_cast(half2_t, w);
-  x = x + big;
-  asm("" : "+v"(x));  // (not folded)
-  return __builtin_bit_cast(uint32_t, (half2_t)(x - big));
-}
+// Codes as whole numbers of 2^-24, eight to an operand: fp16's subnormals are those, up to 1023, so the conversion itself
+// rounds codes (448 at most) to units, ties to even.
+constexpr float kWhole = 0x1p-24f;
 __device__ inline uint4 whole8(uint32_t a, uint32_t b) {
-  return make_uint4(whole2(kv8_pair<kF16, false>(a, 1.0f)), whole2(kv8_pair<kF16, true>(a, 1.0f)),
-                    whole2(kv8_pair<kF16, false>(b, 1.0f)), whole2(kv8_pair<kF16, true>(b, 1.0f)));
+  return make_uint4(kv8_pair<kF16, false>(a, kWhole), kv8_pair<kF16, true>(a, kWhole), kv8_pair<kF16, false>(b, kWhole),
+                    kv8_pair<kF16, true>(b, kWhole));
 }
 __device__ inline f32x4_t mfma_f16(uint4 a, uint4 b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -308,7 +302,7 @@ __device__ void kv8_select_impl(const Kv8SelectArgs& A) {
   for (int i = threadIdx.x; i < kSelBins; i += 64 * kSelWaves) s.hist[i] = 0;
   if (threadIdx.x == 0) s.length = 0;
 
-  // ---- scores of 16 pages at a time, kSelTiles times 16 with their bounds one step ahead
+  // ---- scores of 16 pages at a time, their bounds one step ahead
   {
     const int n = lane & 15, g = lane >> 4;
     const int last = min(count, p0 + 16 * A.tiles);
@@ -324,27 +318,23 @@ __device__ void kv8_select_impl(const Kv8SelectArgs& A) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) raw[i][k] = on ? *(const uint4*)(src + 64 * i + 8 * k) : make_uint4(0, 0, 0, 0);
     struct Step {
-      uint4 hi[kSelTiles][H], lo[kSelTiles][H];
-      float scale[kSelTiles];
-      bool bad[kSelTiles];
+      uint4 hi[H], lo[H];
+      float scale;
+      bool bad;
     };
-    auto load = [&](Step& T, int t0) __attribute__((always_inline)) {
-      const int first = p0 + 16 * t0;
-      if (t0 && t0 % 4 == 0) pages = table[min(first + lane, last - 1)];
+    auto load = [&](Step& T, int tile) __attribute__((always_inline)) {
+      if (tile && tile % 4 == 0) pages = table[min(p0 + 16 * tile + lane, last - 1)];
+      const int page = __shfl(pages, 16 * (tile & 3) + n);
+      // a page outside the pool is never an address: page 0 is read instead, and the page comes last
+      T.bad = page < 0 || page >= A.num_blocks;
+      const int64_t at = (int64_t)(T.bad ? 0 : page) * stride + base;
+      const uint8_t* const p = A.bounds + at * (2 * D) + 16 * g;
 #pragma unroll
-      for (int t = 0; t < kSelTiles; ++t) {
-        const int page = __shfl(pages, 16 * ((t0 + t) & 3) + n);
-        // a page outside the pool is never an address: page 0 is read instead, and the page comes last
-        T.bad[t] = page < 0 || page >= A.num_blocks;
-        const int64_t at = (int64_t)(T.bad[t] ? 0 : page) * stride + base;
-        const uint8_t* const p = A.bounds + at * (2 * D) + 16 * g;
-#pragma unroll
-        for (int i = 0; i < H; ++i) {
-          T.hi[t][i] = *(const uint4*)(p + 64 * i);
-          T.lo[t][i] = *(const uint4*)(p + D + 64 * i);
-        }
-        T.scale[t] = A.scales[at].x;
+      for (int i = 0; i < H; ++i) {
+        T.hi[i] = *(const uint4*)(p + 64 * i);
+        T.lo[i] = *(const uint4*)(p + D + 64 * i);
       }
+      T.scale = A.scales[at].x;
     };
     Step T[2];
     if (p0 < last) load(T[0], 0);
@@ -372,7 +362,7 @@ __device__ void kv8_select_impl(const Kv8SelectArgs& A) {
       const uint32_t bits = __float_as_uint(top);  // the smallest e with top <= 127 * 2^e (1.984375 * 2^6)
       const int e = max((int)(bits >> 23) - 127 - 6 + ((bits & 0x7fffffu) > 0x7e0000u ? 1 : 0), kKv8LeastExp);
       const float down = pow2f(-e);
-      unit[i] = __shfl(pow2f(e), (lane & 15) | (n >> 3) << 5);  // of the column's group: lanes g = 0, 1 or 2, 3
+      unit[i] = __shfl(pow2f(e) / kWhole, (lane & 15) | (n >> 3) << 5);  // of the column's group: lanes g = 0, 1 or 2, 3
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         uint32_t wp[4], wn[4];
@@ -388,50 +378,52 @@ __device__ void kv8_select_impl(const Kv8SelectArgs& A) {
         qn[i][k] = make_uint4(wn[0], wn[1], wn[2], wn[3]);
       }
     }
-    auto score = [&](const Step& T, int t0) __attribute__((always_inline)) {
+    auto score = [&](const Step& T, int tile) __attribute__((always_inline)) {
+      f32x4_t sum[H];
 #pragma unroll
-      for (int t = 0; t < kSelTiles; ++t) {
-        f32x4_t sum[H];
+      for (int i = 0; i < H; ++i) {
+        sum[i] = (f32x4_t){0, 0, 0, 0};
+        sum[i] = mfma_f16(whole8(T.hi[i].x, T.hi[i].y), qp[i][0], sum[i]);
+        sum[i] = mfma_f16(whole8(T.hi[i].z, T.hi[i].w), qp[i][1], sum[i]);
+        sum[i] = mfma_f16(whole8(T.lo[i].x, T.lo[i].y), qn[i][0], sum[i]);
+        sum[i] = mfma_f16(whole8(T.lo[i].z, T.lo[i].w), qn[i][1], sum[i]);
+      }
+      // rows 4 g + r are pages; columns n < 8 the even groups' sums, n >= 8 the odd ones'.  Lanes n < 8 go on with pages
+      // r = 0 and 1, their partners n ^ 8 with 2 and 3
+      float all[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
 #pragma unroll
         for (int i = 0; i < H; ++i) {
-          sum[i] = (f32x4_t){0, 0, 0, 0};
-          sum[i] = mfma_f16(whole8(T.hi[t][i].x, T.hi[t][i].y), qp[i][0], sum[i]);
-          sum[i] = mfma_f16(whole8(T.hi[t][i].z, T.hi[t][i].w), qp[i][1], sum[i]);
-          sum[i] = mfma_f16(whole8(T.lo[t][i].x, T.lo[t][i].y), qn[i][0], sum[i]);
-          sum[i] = mfma_f16(whole8(T.lo[t][i].z, T.lo[t][i].w), qn[i][1], sum[i]);
+          const float own = (n < 8 ? sum[i][r] : sum[i][r + 2]) * unit[i];
+          const float other = dpp_mov<kDppRowRor8>((n < 8 ? sum[i][r + 2] : sum[i][r]) * unit[i]);
+          if (i == 0) all[r] = own + other;
+          else all[r] = (all[r] + (n < 8 ? own : other)) + (n < 8 ? other : own);
         }
-        // rows 4 g + r are pages; columns n < 8 the even groups' sums, n >= 8 the odd ones'
-        float best[4];
+      // the largest over the eight heads: of two pages over a quad, of one over both quads of the eight
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float all = 0.0f;
-#pragma unroll
-          for (int i = 0; i < H; ++i) {
-            const float own = sum[i][r] * unit[i], other = dpp_mov<kDppRowRor8>(own);
-            const float even = n < 8 ? own : other, odd = n < 8 ? other : own;
-            all = i == 0 ? even + odd : (all + even) + odd;
-          }
-          best[r] = on ? all : -INFINITY;
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) best[r] = row_max16(best[r]);
-        // lane n < 4 of a row stores page 4 g + n
-        const int r = n & 3, at = 4 * g + r, p = p0 + 16 * (t0 + t) + at;
-        const float top = r == 0 ? best[0] : r == 1 ? best[1] : r == 2 ? best[2] : best[3];
-        const float sk = __shfl(T.scale[t], at);
-        const bool none = __shfl((int)T.bad[t], at);
-        if (n < 4 && p < count) {
-          const bool always = p < A.first || p >= count - A.recent;
-          __hip_atomic_store(keys + p, always ? ~0u : none ? 0u : score_key(top * sk), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
+      for (int r = 0; r < 2; ++r) {
+        all[r] = on ? all[r] : -INFINITY;
+        all[r] = fmaxf(all[r], dpp_mov<kDppQuadXor1>(all[r]));
+        all[r] = fmaxf(all[r], dpp_mov<kDppQuadXor2>(all[r]));
+      }
+      const bool second = n & 4;
+      const float top = fmaxf(second ? all[1] : all[0], dpp_mov<kDppHalfMirror>(second ? all[0] : all[1]));
+      // the first lane of a quad stores page 4 g + n / 4
+      const int at = 4 * g + (n >> 2), p = p0 + 16 * tile + at;
+      const float sk = __shfl(T.scale, at);
+      const bool none = __shfl((int)T.bad, at);
+      if ((n & 3) == 0 && p < count) {
+        const bool always = p < A.first || p >= count - A.recent;
+        __hip_atomic_store(keys + p, always ? ~0u : none ? 0u : score_key(top * sk), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
     };
-    const int steps = (last - p0 + 16 * kSelTiles - 1) / (16 * kSelTiles);  // (none: below 1)
+    const int steps = (last - p0 + 15) / 16;  // (none: below 1)
     for (int i = 0; i < steps; i += 2) {
-      if (i + 1 < steps) load(T[1], (i + 1) * kSelTiles);
-      score(T[0], i * kSelTiles);
-      if (i + 2 < steps) load(T[0], (i + 2) * kSelTiles);
-      if (i + 1 < steps) score(T[1], (i + 1) * kSelTiles);
+      if (i + 1 < steps) load(T[1], i + 1);
+      score(T[0], i);
+      if (i + 2 < steps) load(T[0], i + 2);
+      if (i + 1 < steps) score(T[1], i + 1);
     }
   }
   // ---- the last workgroup of the (sequence, kv head) to arrive picks

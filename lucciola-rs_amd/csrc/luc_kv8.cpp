@@ -75,7 +75,11 @@ constexpr int kCUs = 256;
 constexpr int kAppendManyRows = 512;
 constexpr int kTokCols = 8;          // columns of a workgroup
 constexpr int kTokMaxSplits = 256;   // kv_split.h
-constexpr int kTokSlots = 2 * kCUs;  // workgroups that a launch is planned for: two a CU (three or four: no faster)
+// Workgroups that a launch is planned for: one a CU.  Short splits of a launch planned for two cost more by their merge than
+// they gain: of 4 kv heads of 128, 64 contexts of 1536 18.1 us and 21.2, 8 of 4096 11.2 and 13.3; of 2 of 64, 64 mixed ones up
+// to 4096 12.9 and 12.1, 128 of 2048 11.8 and 14.0; long ones alike.
+constexpr int kTokSlots = kCUs;
+constexpr int kTokAtOnce = 2 * kCUs;  // more of them go longest first (512 of one length each: 17.3 us, 20.3 so)
 // Split lengths of a tokens launch: what fills the chip once, but not longer than lets mixed contexts end together (64
 // contexts of 8192, 7 heads of 64 a group: 24.3 us, 28.1 of splits to 1024; 128 mixed up to 8192, 7 of 128: 107.8,
 // 111.8 to 1024, 111.5 to 4096), nor shorter than is worth a merge.  A workgroup takes 0.0048 us a token, a
@@ -102,8 +106,8 @@ constexpr int kColsMinSplit64 = 512, kColsMinSplit128 = 256, kColsMaxSplits = 32
 constexpr int64_t kMaxArrivals = 1 << 16;  // (sequence, kv head, column tile)
 constexpr int kSelPages = 4 * 16;          // pages of a workgroup's waves at once (kv8_select.hip)
 // Workgroups of a selection before they take more pages each, up to 16 times kSelPages.  64 contexts of 1024 to 16384
-// tokens, 4 kv heads of 128, selection and attention over 96 pages: 44.4 us; planned for 1024 46.0, for 256 and
-// 2048 some 4 more (few end late, many start late).
+// tokens, 4 kv heads of 128, selection and attention over 96 pages: 39.1 us; planned for 256 42.6, for 1024 39.0, but 8 of
+// 65536 then take 21.8 instead of 19.5 to choose from.
 constexpr int kSelWorkgroups = 2 * kCUs;
 
 struct Kv8Plan {
@@ -130,7 +134,7 @@ Kv8Plan kv8_plan(int batch, int total_rows, int max_rows, int max_ctx, int hkv, 
     st = std::min<int64_t>(std::max(fill, st), kTokMaxSplit);
     st = std::max({st, fill / kTokRounds, ceil_div(max_ctx, kTokMaxSplits)});
     p.split_tokens = (int)(ceil_div(st, round) * round);
-    p.longest_first = p.tiles == 1 && batch <= 64 && units * ceil_div(max_ctx, p.split_tokens) > kTokSlots;
+    p.longest_first = p.tiles == 1 && batch <= 64 && units * ceil_div(max_ctx, p.split_tokens) > kTokAtOnce;
   } else {
     p.tiles = (int)ceil_div(cols, head_dim == 64 ? kColsOf64 : kColsOf128);
     const int64_t wgs = pairs * p.tiles;
@@ -376,7 +380,7 @@ int luc_kv8_select(luc_ctx* ctx, void* stream, int dtype, int32_t* pages, int bu
   const size_t need = select_workspace_bytes(batch, max_ctx, budget, num_kv_heads);
   if (int rc = check_workspace(workspace, workspace_bytes, need)) return rc;
   const int max_pages = (int)ceil_div(max_ctx, 4 * LUC_BLOCK_SIZE) * 4;
-  int tiles = 2;
+  int tiles = 1;
   while (tiles < 16 && (int64_t)batch * num_kv_heads * ceil_div(max_pages, kSelPages * tiles) > kSelWorkgroups) tiles *= 2;
   const int64_t chunks = need ? ceil_div(max_pages, kSelPages * tiles) : 1;
   const int64_t grid = ceil_div(batch * chunks, 8) * 8 * num_kv_heads;
