@@ -227,7 +227,7 @@ int attend(luc_ctx* ctx, void* stream, int dtype, int head_dim, const Kv8Plan& p
   const int64_t units = (int64_t)a.batch * a.hkv * plan.tiles;
   const int64_t threads = !plan.tokens && head_dim == 128 ? 512 : 256;
   const int64_t items = (int64_t)a.total_rows * a.hkv * a.group;  // of the merge, head_dim / 4 threads each
-  if (units * plan.splits * threads > UINT32_MAX || (!plan.tokens && plan.splits > 1 && items * (head_dim / 4) > UINT32_MAX))
+  if (units > UINT32_MAX / (plan.splits * threads) || (!plan.tokens && plan.splits > 1 && items * (head_dim / 4) > UINT32_MAX))
     return fail(LUC_E_INVALID, "batch x kv heads x rows too large");
   if (int rc = check_device(ctx)) return rc;
   a.tiles = plan.tiles;

@@ -20,10 +20,12 @@ def rope(max_pos, d):
 
 
 class Book:
-    """8-bit pools on the device, the same on the host, and 16-bit pools beside them."""
+    """8-bit pools on the device, the same on the host, and 16-bit pools beside them.  lead: every call is one of many
+    rows, of which so many without a slot come before, and more behind."""
 
     def __init__(self, luc, hq, hkv, d, dtype, pages=12, layers=2, layer=1, bias=True, norm=True, seed=0, bounds=True,
-                 fill=0xFF):
+                 fill=0xFF, lead=None):
+        self.lead = lead
         self.luc, self.hq, self.hkv, self.d, self.dt, self.layers, self.layer = luc, hq, hkv, d, DT[dtype], layers, layer
         self.gen = torch.Generator().manual_seed(seed)
         rnd = lambda *s: torch.randn(*s, generator=self.gen)  # noqa: E731
@@ -49,6 +51,11 @@ class Book:
 
     def append(self, slots, pos, qkv, in_place=False, num_blocks=None):
         """One call, checked against the host."""
+        if self.lead is not None:
+            pad = self.rows(self.lead + 600, extra=qkv.shape[1] - (self.hq + 2 * self.hkv) * self.d)
+            qkv = torch.cat([pad[:self.lead], qkv, pad[self.lead:]])
+            slots = [-1] * self.lead + [int(x) for x in slots] + [-1] * 600
+            pos = [3] * self.lead + list(pos) + [-1] * 50 + [9] * 550
         n, a, b, c = len(slots), self.hq * self.d, (self.hq + self.hkv) * self.d, (self.hq + 2 * self.hkv) * self.d
         q, k, v = qkv[:, :a], qkv[:, a:b], qkv[:, b:c]
         sl = torch.tensor(slots, dtype=torch.int64, device="cuda")
@@ -61,6 +68,7 @@ class Book:
                                      num_blocks=num_blocks, **self.kw)
         print(f"  append8: rows {n} heads {self.hq}/{self.hkv}x{self.d} {self.dt} slots {slots[:6]}", flush=True)
         if in_place:
+            want_q[:, :a] = torch.where(((ps >= 0) & (ps < 400))[:, None], want_q[:, :a], q)  # (the others' q stays)
             qkv = qkv.clone()
             q, k, v = qkv[:, :a], qkv[:, a:b], qkv[:, b:c]
         self.luc.kv8_append(q, k, v, self.cos, self.sin, ps, sl, self.k, self.v, self.scales, *args,
@@ -92,10 +100,11 @@ def seq(table, start, n):
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("hq,hkv,d", HEADS)
-def test_prompts_and_steps(luc, hq, hkv, d, dtype):
+@pytest.mark.parametrize("lead", [None, 0, 13])
+def test_prompts_and_steps(luc, hq, hkv, d, dtype, lead):
     """Prompts of odd lengths, then rows one by one, several, and up to a page's end, louder and quieter than what
     the pages hold; a page that is taken by another sequence."""
-    book = Book(luc, hq, hkv, d, dtype, seed=d + hq)
+    book = Book(luc, hq, hkv, d, dtype, seed=d + hq, lead=lead)
     a, b = [7, 2, 9, 0, 4], [11, 1, 5]
     for n_a, start_a, n_b, start_b, k_scale, v_scale in (
             (33, 0, 17, 0, 1.4, 1.0), (1, 33, 1, 17, 1.4, 1.0), (1, 34, 1, 18, 9.0, 40.0), (3, 35, 13, 19, 100.0, 0.01),
@@ -108,8 +117,9 @@ def test_prompts_and_steps(luc, hq, hkv, d, dtype):
 
 @pytest.mark.parametrize("hq,hkv,d", HEADS[:2])
 @pytest.mark.parametrize("norm,bias", [(False, False), (True, False), (False, True)])
-def test_norms_and_biases(luc, hq, hkv, d, norm, bias):
-    book = Book(luc, hq, hkv, d, "bf16", norm=norm, bias=bias, bounds=norm)
+@pytest.mark.parametrize("lead", [None, 7])
+def test_norms_and_biases(luc, hq, hkv, d, norm, bias, lead):
+    book = Book(luc, hq, hkv, d, "bf16", norm=norm, bias=bias, bounds=norm, lead=lead)
     s, p = seq([3, 8, 1, 5], 5, 50)
     book.append(s, p, book.rows(50))
     for i in range(55, 60):
@@ -136,21 +146,25 @@ def test_values_at_the_edges(luc, dtype):
         book.append(*seq([4 + i // 4], i % 4, 1), qkv[7 + i:8 + i])
 
 
-def test_rows_that_have_no_place(luc):
+@pytest.mark.parametrize("lead", [None, 15])
+def test_rows_that_have_no_place(luc, lead):
     """Slots and positions of no page and no table: the rows' q, or nothing, and no cache."""
-    book = Book(luc, 14, 2, 64, "f16")
+    book = Book(luc, 14, 2, 64, "f16", lead=lead)
     slots = [-1, 37, 38, 12 * PAGE, 39, -(1 << 40), 1 << 40, 96, 97, 98]
     pos = [5, 6, 7, 8, 9, 10, 11, 399, 400, -1]
     book.append(slots, pos, book.rows(10))
+    # a page whose first row, or one in between, has no position
+    book.append([7 * PAGE, 7 * PAGE + 1, 7 * PAGE + 2, 8 * PAGE, 7 * PAGE + 3, 8 * PAGE + 1], [400, 1, -1, -7, 2, 3], book.rows(6))
     # a pool of fewer pages than the tensors hold
     s, p = seq([5, 6], 12, 9)
     book.append(s, p, book.rows(9), num_blocks=6)
 
 
 @pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (12, 2, 128)])
-def test_rows_in_any_order(luc, hq, hkv, d):
+@pytest.mark.parametrize("lead", [None, 0, 1, 11, 16, 31])
+def test_rows_in_any_order(luc, hq, hkv, d, lead):
     """Rows of a page in descending order, with others and padding between them, as far apart as they may be."""
-    book = Book(luc, hq, hkv, d, "bf16")
+    book = Book(luc, hq, hkv, d, "bf16", lead=lead)
     s, p = seq([2, 7], 0, 32)
     book.append(s[::-1], p[::-1], book.rows(32))
     # two pages row by row, and one of them again at other offsets, 31 rows behind the first
@@ -163,9 +177,10 @@ def test_rows_in_any_order(luc, hq, hkv, d):
 
 
 @pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (32, 8, 128)])
-def test_many_rows(luc, hq, hkv, d):
+@pytest.mark.parametrize("lead", [None, 5])
+def test_many_rows(luc, hq, hkv, d, lead):
     """A batch of single rows and ragged prompts beyond what one workgroup has."""
-    book = Book(luc, hq, hkv, d, "bf16", pages=90, layers=1, layer=0)
+    book = Book(luc, hq, hkv, d, "bf16", pages=90, layers=1, layer=0, lead=lead)
     perm = np.random.default_rng(1).permutation(90).tolist()
     s, p = [], []
     for i, n in enumerate((100, 1, 16, 31, 64)):

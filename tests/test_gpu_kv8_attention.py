@@ -411,6 +411,28 @@ def test_equal_scores(luc, d):
                 assert got[b, h].tolist() == want_pages(c, b, h, q[b], 8, 20, 1, 2), (i, b, h)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_codes_are_rounded_to_units(luc, d, dtype):
+    """A query of one dimension: pages whose bounds there are every code, in any order; what decides is the code's
+    nearest whole number, halves to the even one, and of equal ones the lower page."""
+    codes = np.random.default_rng(d).permutation(np.delete(np.arange(256), [127, 255]))
+    c = Cache([254 * PAGE], 2, d, seed=1)
+    ids = c.tables[0]
+    c.scales[ids, 1, :, 0] = 0.25
+    c.sp = torch.from_numpy(c.scales).cuda()
+    for dim, value in ((5, 1.0), (37, -3.0), (d - 1, 0.5), (16, -1e-3)):
+        c.bounds[:] = 0
+        c.bounds[ids, 1, :, 0 if value > 0 else 1, dim] = codes[:, None]
+        c.bp = torch.from_numpy(c.bounds).cuda()
+        q = torch.zeros(1, 6 * d, dtype=DT[dtype], device="cuda")
+        q.view(6, d)[[0, 1, 2, 4], dim] = value
+        for budget in (3, 20, 60, 100, 128, 150, 180, 220, 253):
+            pages, _ = sparse(luc, c, 6, dtype, budget, 0, 1, q=q)
+            for h in range(2):
+                assert pages[0, h].tolist() == want_pages(c, 0, h, q[0], 6, budget, 0, 1), (dim, budget, h)
+
+
 def test_many_pages(luc):
     """More pages than a workgroup keeps keys of, and scores of both signs over many powers of two."""
     hkv, d, n = 1, 64, 8300
