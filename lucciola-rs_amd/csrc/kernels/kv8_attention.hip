@@ -33,12 +33,12 @@
 // in another slab order 108.  The first 512 workgroups read 6.7 TB/s, the tail from 75 us on is what is lost.  Few tokens: a
 // chain of round trips, lengths -> table -> scale, K -> products -> merge of the waves, and of splits by way of the
 // workspace: 5.6 for 512 tokens, 11 for 32 rows over up to 4096, 21.6 for 96 chosen pages of each of 64 contexts (100 MB).
-// Columns: issue.  512 rows after 8000, 12 / 2 heads of 128 (fp16): 36.6 and 7.7 for the merge of ten splits, 31 MB each way;
-// four prompts of 1531 to 2048, 14 / 2 heads of 64 (bf16): 40.4; matrix instructions busy
-// 38% and 32% of the SIMDs' time, VALU instructions, two thirds of their cycles exponentials, 47% and 64%: the two
-// hardly run at once whatever the waves.  1024 rows at the end of 32768 tokens, 28 / 4 heads of 128: 455, 1040 TFLOP/s; with the two
-// waves of a SIMD a phase apart by barriers, one's products beside the other's softmax, 475.  Both halves of a tile at a time spill (53), wave priorities changed nothing; chunks of
-// columns in serpentine order of their lengths 40.4, in plain order 42.6.
+// Columns: issue.  512 rows after 8000, 12 / 2 heads of 128 (fp16): 36.6 and 7.7 for the merge of ten splits, 31 MB each
+// way; four prompts of 1531 to 2048, 14 / 2 heads of 64 (bf16): 40.4; matrix instructions busy 38% and 32% of the SIMDs'
+// time, VALU instructions, two thirds of their cycles exponentials, 47% and 64%: the two hardly run at once whatever the
+// waves.  1024 rows at the end of 32768 tokens, 28 / 4 heads of 128: 455, 1040 TFLOP/s; with the two waves of a SIMD a phase
+// apart by barriers, one's products beside the other's softmax, 475.  Both halves of a tile at a time spill (53 for the first
+// case), wave priorities changed nothing; chunks of columns in serpentine order of their lengths 40.4, in plain order 42.6.
 #include "kv8.h"
 #include "kv_split.h"
 
