@@ -460,9 +460,10 @@ class LucAttn:
             o_rows, o_stride = self._rows("q_out", q_out, qw, head_dim, dtype, dev)
             if o_rows != rows:
                 raise ValueError(f"q_out has {o_rows} rows, q {rows}")
-        max_pos = cos.shape[0]
-        if cos.shape[-1] * 2 != head_dim or cos.shape != sin.shape:
-            raise ValueError(f"rope tables {tuple(cos.shape)}, {tuple(sin.shape)}: want [positions, {head_dim // 2}]")
+        table = cos.shape
+        max_pos = table[0]
+        if table[-1] * 2 != head_dim or table != sin.shape:
+            raise ValueError(f"rope tables {tuple(table)}, {tuple(sin.shape)}: want [positions, {head_dim // 2}]")
         return [self.ctx, _stream(stream), dtype_code(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), stride,
                 q_bias if q_bias is None else arr("q_bias", q_bias, dtype, dev, qw),
                 k_bias if k_bias is None else arr("k_bias", k_bias, dtype, dev, kw),
@@ -567,10 +568,11 @@ class LucAttn:
     def _kv8_pools(self, k_pool, v_pool, scales, num_layers, hkv, head_dim, num_blocks, dev):
         """(k address, v address, scales address, pages) of 8-bit pools: uint8 [pages, layers, kv heads,
         16 * head_dim], scales float32 [pages, layers, kv heads, 2]."""
-        pages, u8 = len(k_pool), torch.uint8
+        shape, u8 = k_pool.shape, torch.uint8
+        pages = shape[0] if shape else 0  # (len() of a tensor takes three times as long)
         want = (pages, num_layers, hkv, 16 * head_dim)
-        if k_pool.shape != want or v_pool.shape != want:
-            raise ValueError(f"8-bit pools {tuple(k_pool.shape)}, {tuple(v_pool.shape)}: want {('pages', *want[1:])}")
+        if shape != want or v_pool.shape != want:
+            raise ValueError(f"8-bit pools {tuple(shape)}, {tuple(v_pool.shape)}: want {('pages', *want[1:])}")
         if scales.shape != (pages, num_layers, hkv, 2):
             raise ValueError(f"scales {tuple(scales.shape)}: want {(pages, num_layers, hkv, 2)}")
         # (one test for the three: a call of its own for each would cost a fifth of a launch)
@@ -676,9 +678,10 @@ class LucAttn:
 
     def _chosen(self, pages, batch, hkv, dev):
         """(address, budget) of pages int32 [batch, hkv, budget]."""
-        if pages.dim() != 3 or pages.shape[:2] != (batch, hkv):
-            raise ValueError(f"pages {tuple(pages.shape)}: want [{batch}, {hkv}, budget]")
-        return self._array("pages", pages, torch.int32, dev, 0), pages.shape[2]
+        shape = pages.shape
+        if len(shape) != 3 or shape[0] != batch or shape[1] != hkv:
+            raise ValueError(f"pages {tuple(shape)}: want [{batch}, {hkv}, budget]")
+        return self._array("pages", pages, torch.int32, dev, 0), shape[2]
 
     def kv8_select(self, pages, q, bounds, scales, tables, start_pos, batch, max_ctx, first, recent, layer,
                    num_layers, hq, hkv, head_dim, cu_seqlens=None, workspace=None, block_size=16, stream=None,
@@ -689,15 +692,17 @@ class LucAttn:
         rows, q_stride = self._rows("q", q, hq * head_dim, head_dim, q.dtype, dev)
         if cu_seqlens is None and rows < batch:
             raise ValueError(f"q has {rows} rows, fewer than the batch's {batch}")
-        if scales.dim() != 4 or scales.shape[1:] != (num_layers, hkv, 2):
-            raise ValueError(f"scales {tuple(scales.shape)}: want [pages, {num_layers}, {hkv}, 2]")
-        bp = self._bounds(bounds, scales.shape[0], num_layers, hkv, head_dim, dev)
+        shape = scales.shape
+        blocks = shape[0] if shape else 0
+        if shape != (blocks, num_layers, hkv, 2):
+            raise ValueError(f"scales {tuple(shape)}: want [pages, {num_layers}, {hkv}, 2]")
+        bp = self._bounds(bounds, blocks, num_layers, hkv, head_dim, dev)
         sp = self._array("scales", scales, torch.float32, dev, 0)
         cp, budget = self._chosen(pages, batch, hkv, dev)
         tp, stride, cu, start = self._batch_args(tables, start_pos, cu_seqlens, batch, dev)
         self._check(self.lib.luc_kv8_select(
             self.ctx, _stream(stream), dtype_code(q), cp, budget, first, recent, q.data_ptr(), q_stride, bp, sp, tp,
-            stride, self._pages_of(scales.shape[0], num_blocks), cu, start, batch,
+            stride, self._pages_of(blocks, num_blocks), cu, start, batch,
             batch if cu_seqlens is None else rows, max_ctx, layer, num_layers, hq, hkv, head_dim, block_size,
             *self._workspace_args(workspace, dev)))
 
