@@ -87,8 +87,8 @@ constexpr int kTokAtOnce = 2 * kCUs;  // more of them go longest first (512 of o
 // 256; of 8192 9.9, 10.7 in 256, 11.4 in 1024; of 2048 8.1, 9.0 in 512.  Up to 512 tokens a second split costs more
 // than it saves: 6.3 us, 7.8 in two.
 constexpr int kTokOneSplit = 512, kTokMaxSplit = 2048, kTokSplitRate = 26;
-// Beyond so many rounds of workgroups splits grow again: any contexts balance (200 mixed contexts: equal with
-// 4, 8 and 16).
+// Beyond so many rounds of workgroups splits grow again: any contexts balance (200 mixed contexts up to 8192, 8 kv heads of
+// 128: 288 us, 290 without; 4 and 16 lie between).
 constexpr int kTokRounds = 8;
 // Up to 16 columns go to the tokens kernel, which reads the cache once for each 8, and more of them while it reads at
 // most this: 5.4 TB/s from the L2 of an XCD, or 5.6 ns a workgroup, as many bytes as kTokLeastBytes, where contexts are
