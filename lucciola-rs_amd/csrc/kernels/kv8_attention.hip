@@ -613,7 +613,9 @@ template <int D> struct Kv8Tile {
 };
 template <int D> struct Kv8Cols {
   static constexpr int WAVES = D == 128 ? 8 : 4;
-  static constexpr int F = 2;  // fragments of a wave
+  // Fragments of a wave.  Four of D = 64 read LDS half as often, with 246 registers: 1024 rows on 32768 tokens (14 / 2 heads)
+  // 136 us, 171 with two, but 512 on 8512 41.5 and 37.6, 8192 on themselves 199 and 139: longer chains that end later.
+  static constexpr int F = 2;
   static constexpr int N = WAVES * F * 16;
 };
 
