@@ -133,6 +133,7 @@ Kv8Plan kv8_plan(int batch, int total_rows, int max_rows, int max_ctx, int hkv, 
     int64_t st = max_ctx <= kTokOneSplit ? kTokOneSplit : (int64_t)std::sqrt((double)kTokSplitRate * max_ctx);
     st = std::min<int64_t>(std::max(fill, st), kTokMaxSplit);
     st = std::max({st, fill / kTokRounds, ceil_div(max_ctx, kTokMaxSplits)});
+    st = std::min<int64_t>(st, max_ctx);  // (the rounds of the largest calls ask for more than 32 bits)
     p.split_tokens = (int)(ceil_div(st, round) * round);
     p.longest_first = p.tiles == 1 && batch <= 64 && units * ceil_div(max_ctx, p.split_tokens) > kTokAtOnce;
   } else {
