@@ -135,6 +135,7 @@ Kv4Plan kv4_plan(int batch, int total_rows, int max_rows, int max_ctx, int hkv, 
     const int64_t fill = units * max_ctx / kTokSlots;
     int64_t st = std::min<int64_t>(std::max<int64_t>(fill, kTokMinSplit), kTokMaxSplit);
     st = std::max({st, fill / kTokRounds, ceil_div(max_ctx, kTokMaxSplits)});
+    st = std::min<int64_t>(st, max_ctx);  // (the rounds of the largest calls ask for more than 32 bits)
     p.split_tokens = (int)(ceil_div(st, round) * round);
     p.longest_first = p.tiles == 1 && batch <= 64 && units * ceil_div(max_ctx, p.split_tokens) > kTokSlots;
   } else {

@@ -33,13 +33,13 @@ LARGEST = [(n, n, 1, 1 << 30, h, h, d) for n, h, d in (
 LARGEST += [(8192, 8192, 1, 1 << 26, 64, 8, 128), (16384, 16384, 2, 1 << 29, 8, 2, 64)]
 
 
-@pytest.mark.parametrize("fn", ["luc_kv8_workspace_size"])
+@pytest.mark.parametrize("fn", ["luc_kv8_workspace_size", "luc_kv4_workspace_size"])
 def test_the_largest_calls_have_a_plan(fn):
     """One split of every context: no workspace."""
     assert sizes(fn, *LARGEST) == [0] * len(LARGEST)
 
 
-@pytest.mark.parametrize("fn", ["luc_kv8_workspace_size"])
+@pytest.mark.parametrize("fn", ["luc_kv8_workspace_size", "luc_kv4_workspace_size"])
 def test_long_contexts_keep_their_splits(fn):
     """Of two splits or more, each has partials of 8 columns: (m, l) and o, behind 2^16 counters."""
     for size, (batch, splits, d) in zip(sizes(fn, (1, 1, 1, 1 << 30, 8, 1, 64), (2, 2, 1, 1 << 30, 8, 1, 128)),
