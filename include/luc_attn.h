@@ -501,8 +501,8 @@ int luc_kv4_attention(luc_ctx* ctx, void* stream, int dtype, void* out, int64_t 
  * page anew: its scales and bounds are those of the call's rows.  Rows at later offsets join what the page
  * holds: the scales grow where they need to (every code of the page is then rounded again), the bounds take them
  * in (a NaN counts as 0).  Tokens that a page held behind its new end (luc_block_truncate) still count in both.
- * Slots of one call are distinct (what a slot named twice holds is not defined), and the rows of one page (same slot /
- * 16) lie within 32 successive rows, as luc_block_extend gives them.  bounds may be NULL: none are kept. */
+ * Rows come in any order: those of one page (same slot / 16) are written together wherever they lie in the call.  Slots of
+ * one call are distinct (what a slot named twice holds is not defined).  bounds may be NULL: none are kept. */
 int luc_kv8_append(luc_ctx* ctx, void* stream, int dtype, const void* q, const void* k, const void* v,
                    int64_t row_stride, const void* q_bias, const void* k_bias, const void* v_bias,
                    const void* q_norm, const void* k_norm, float eps, const float* cos_table,

@@ -70,9 +70,10 @@ struct Kv8SelectArgs {
 };
 
 constexpr int kCUs = 256;
-// Rows from which a wave of an append looks through 16 rows for runs, instead of through its own.  28 + 2 x 4 heads of
-// 128, us by either: 256 rows 6.1 and 5.8, 512 6.4 and 6.3, 1024 6.9 and 8.2, 4096 15.6 and 24.8.
-constexpr int kAppendManyRows = 512;
+// Rows up to which a wave of an append has the runs of one row and the slots of all in registers, and beyond which it has those of
+// 16.  28 + 2 x 4 heads of 128, us by either: a prompt of 256 rows 6.3 and 6.4, of 512 7.0 and 6.5; 512 single rows 7.4
+// and 49, one run after the other.
+constexpr int kAppendManyRows = 512;  // kManyRows of kv8_append.hip
 constexpr int kTokCols = 8;          // columns of a workgroup
 constexpr int kTokMaxSplits = 256;   // kv_split.h
 // Workgroups that a launch is planned for: one a CU.  Short splits of a launch planned for two cost more by their merge than
@@ -284,8 +285,9 @@ int luc_kv8_append(luc_ctx* ctx, void* stream, int dtype, const void* q, const v
   const bool many = num_tokens > kAppendManyRows;
   const int64_t runs = ceil_div(ceil_div(num_tokens, many ? 16 : 1) * num_kv_heads * 2, 4);
   const int64_t grid = ceil_div((int64_t)num_tokens * num_q_heads, 4096 / head_dim) + runs;
-  // the blocks of runs evenly among q's, an odd number apart: block x runs on XCD x % 8
-  a.every = (uint32_t)std::min<int64_t>((grid / runs - 1) | 1, 1 << 30);
+  // the blocks of runs evenly among q's, an odd number apart (block x runs on XCD x % 8), and all of them in the first half:
+  // they take longest
+  a.every = (uint32_t)std::min<int64_t>((grid / runs / 2) | 1, 1 << 30);
   if (grid * 256 > UINT32_MAX) return fail(LUC_E_INVALID, "too many rows for one launch");
   if (int rc = check_device(ctx)) return rc;
   const hipFunction_t fn = kernel(ctx, many ? kAppendMany : kAppend, dtype, head_dim);

@@ -604,8 +604,7 @@ class LucAttn:
                    v_bias=None, q_out=None, block_size=16, stream=None, num_blocks=None):
         """luc_kv8_append: qk_norm_rope_append into 8-bit pools (uint8 [pages, layers, kv heads, 16 *
         head_dim]) with their scales (float32 [pages, layers, kv heads, 2]) and, if given, key bounds
-        (uint8 [pages, layers, kv heads, 2, head_dim]).  The rows of a page lie within 32 successive rows, as
-        block_extend's do."""
+        (uint8 [pages, layers, kv heads, 2, head_dim]).  Rows in any order, slots distinct."""
         args, rows, dtype, dev = self._append_args(q, k, v, cos, sin, positions, slots, hq, hkv, head_dim,
                                                    q_norm, k_norm, eps, q_bias, k_bias, v_bias, q_out, stream)
         kp, vp, sp, pages = self._kv8_pools(k_pool, v_pool, scales, num_layers, hkv, head_dim, num_blocks, dev)
