@@ -1,4 +1,5 @@
-"""luc_kv8_append of rows in any order: a page's rows anywhere in the call are one run, as the plain form has it."""
+"""luc_kv8_append of rows in any order: a page's rows anywhere in the call are one run, as the plain form has it; and its q bit for
+bit."""
 import numpy as np
 import pytest
 import torch
@@ -77,3 +78,26 @@ def test_the_ends_of_a_call(luc, rows):
             s[at] = page * PAGE + off
     append(book, s, p)
     append(book, s, p, 9.0, 0.1)
+
+
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(14, 2, 64, "bf16"), (28, 4, 128, "f16")])
+@pytest.mark.parametrize("rows", [5, 600])
+def test_bits_of_q(luc, hq, hkv, d, dtype, rows):
+    """q is that of luc_qk_norm_rope_append in every bit, zeros' signs too, and what lies behind a row stays."""
+    book = Book(luc, hq, hkv, d, dtype, pages=rows // PAGE + 4, bias=False, seed=rows)
+    a, b = hq * d, (hq + hkv) * d
+    qkv = book.rows(rows)
+    qkv[::3, :a:2] = 0.0
+    qkv[1::3, :a:3] = -0.0
+    qkv[2::5, :a] *= -0.0
+    s, p = packed(book.pages, [rows], [0], 0)
+    slots = torch.from_numpy(s).cuda()
+    pos = torch.from_numpy(np.where(np.arange(rows) % 7 == 4, -1, p % 400).astype(np.int32)).cuda()
+    kp, vp = (torch.zeros((book.pages, 2, hkv, PAGE, d), dtype=book.dt, device="cuda") for _ in range(2))
+    want, got = (torch.full((rows, a + 8), 7.0, dtype=book.dt, device="cuda") for _ in range(2))
+    args = (qkv[:, :a], qkv[:, a:b], qkv[:, b:], book.cos, book.sin, pos, slots)
+    luc.qk_norm_rope_append(*args, kp, vp, 1, 2, hq, hkv, d, q_out=want[:, :a], **book.kw)
+    luc.kv8_append(*args, book.k, book.v, book.scales, 1, 2, hq, hkv, d, bounds=book.bounds, q_out=got[:, :a], **book.kw)
+    torch.cuda.synchronize()
+    assert bool((want[:, :a].view(torch.int16) == -32768).any()) and bool((want[:, :a].view(torch.int16) == 0).any())
+    assert torch.equal(got.view(torch.int16), want.view(torch.int16))
