@@ -539,7 +539,9 @@ int luc_kv8_attention(luc_ctx* ctx, void* stream, int dtype, void* out, int64_t 
  *   (((S_0 2^e_0 + S_1 2^e_1) + S_2 2^e_2) + S_3 2^e_3) * scale_K    (head_dim / 32 terms; the additions in f32)
  *   S_j = sum over dimensions i of 32 j .. 32 j + 31 of n_i * (n_i > 0 ? largest_i : smallest_i), a whole number
  * with the page's bounds in whole code units (nearest, ties to even), n = rint(q 2^-e_j) and e_j the smallest that
- * brings those 32 elements of q to at most 127: q . k of the page's keys is at most that, but for the roundings.  A page outside
+ * brings those 32 elements of q to at most 127.  But for these roundings no q . k of the page's keys is larger; with them a
+ * dimension whose bounds are below half a unit (1/448 of the page's largest key or less) counts as 0, so where few
+ * dimensions of a head's keys are some hundred times the others, the others hardly decide.  A page outside
  * [0, num_blocks) scores lowest.  A NaN of q counts as 0, q is clamped to +-60000; a sequence without a row, or
  * whose context is more than max_ctx, gets -1.
  *

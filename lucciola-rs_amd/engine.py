@@ -403,7 +403,9 @@ class Kv8Cache(_QuantCache):
     """An 8-bit paged cache of up to `max_seqs` sequences (pools and scales of luc_kv8_append, half the
     bytes of 16 bits) and the DeviceBlocks behind it: a step as Kv4Cache has it.  With `bounds` (1/16 of the
     pools more) a step of at most one row a sequence may `attend_sparse`: to the pages of each context that
-    score highest, instead of to all of it.  One that was made without cannot."""
+    score highest, instead of to all of it.  One that was made without cannot.  Tokens that `truncate` drops still
+    count in the scale and the bounds of the page that goes on, until its next first token: the same tokens
+    again may have coarser codes there, and be chosen by wider bounds."""
 
     def __init__(self, num_layers, num_q_heads, num_kv_heads, head_dim, num_physical_blocks,
                  max_seqs, max_position_embeddings, max_rows=None, bounds=False, device="cuda", lib=None):
