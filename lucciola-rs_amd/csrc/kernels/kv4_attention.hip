@@ -556,7 +556,7 @@ __device__ void kv4_tokens_impl(const Kv4AttnArgs& A) {
   __shared__ float s_m[NW][2 * TC], s_l[NW][2 * TC];
   __shared__ int s_last;
   // the ring's memory after the last stage: the waves' o; then, in the merge of the splits, the sets' o
-  // and the splits' weights
+  // and the splits' weights (what follows the stages is kv_tokens_finish of kv8_attention.hip too, in all but NB)
   float (*const s_o)[2 * TC][OS] = (float (*)[2 * TC][OS])s_ring;
   float4* const s_x = (float4*)s_ring;
   float (*const s_w)[TC] = (float (*)[TC])((char*)s_ring + NT * 16);
@@ -1255,7 +1255,7 @@ __device__ void kv4_columns_impl(const Kv4AttnArgs& A) {
   }
   W.finish(s_nan[D / 32], s_nan);
   // A lane holds 16 dimensions of a column.  By way of the wave's share of the tiles, which no wave
-  // reads any more, D / 4 lanes write a column side by side.
+  // reads any more, D / 4 lanes write a column side by side.  (kv_columns_out of kv8_attention.hip too.)
   __syncthreads();
   const int hq = A.hkv * A.group;
   float4* const turn = (float4*)s_tile + w * (4 * D);  // [16 columns][D / 4], swizzled

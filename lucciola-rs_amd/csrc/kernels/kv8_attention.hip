@@ -277,7 +277,9 @@ template <int DT, int D> struct Kv8Row {
 // (a wave's columns col and col + kTokCols are parts of one).  mem (kTokMergeBytes of LDS, 16-byte aligned):
 // the waves' o, [wave][column][D + 4]; s_m and s_l their maxima and sums.  All of it written, and a
 // barrier behind.  The columns of a unit that has one split go out; others go to the workspace, and the last
-// workgroup of the unit to arrive merges its splits.
+// workgroup of the unit to arrive merges its splits.  (kv4_attention.hip has the same lines in its kernels, and those of
+// kv_columns_out: what is wrong in one is wrong in both.  Through a function they take its tokens kernel of 64 dimensions from 142 to
+// 189 registers, and its columns kernels of bf16 spill.)
 template <int D> constexpr int kTokMergeBytes = kTokWaves * 2 * kTokCols * (D + 4) * 4;
 
 template <int DT, int D, class Args>
