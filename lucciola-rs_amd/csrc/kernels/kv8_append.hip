@@ -16,7 +16,8 @@
 // them; the slots of the other rows are compared with the page too, and only where one is of it (token by token orders)
 // is the run put together from all rows.  That costs calls of up to 64 rows nothing, 512 single rows of 28 + 2 x 4
 // heads of 128 7.3 us instead of 6.7, a prompt of 1000 rows 7.5 for 6.9, 2000 rows of 4 a sequence 25.1 for 23.1, 8191 single rows
-// 112 for 95.
+// 112 for 95; it grows with the rows times the pages that are not whole: 64 prompts of 2047 rows 607 for 507.  With a span's
+// heads side by side, so that a workgroup seeks one span's pages for four heads, those take 535, but 8191 rows 29.8.
 //
 // What bounds it.  8191 rows of 28 + 2 x 4 heads of 128 (bf16): 28.4 us for 147 MB, as a copy of them takes; 54 with a wave
 // a row, 73 with the blocks of runs every eighth (all on one XCD), 36.9 with streamed loads of qkv.  A bound of
