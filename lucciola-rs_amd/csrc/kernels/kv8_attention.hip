@@ -10,9 +10,10 @@
 // rescaling are lane-local up to the four lanes that share it, and the scores of two pages are
 // already the operand of the second product: lane l holds four tokens of either.  Codes become 16-bit values, scale
 // included, in one conversion a pair, exactly (fp16: where the value is one; below 2^-14 it rounds to fp16's 2^-24).
-// Weights are rounded to the rows' type, which the matrix unit takes, and summed as rounded, and held times a power of two, far
-// above fp16's smallest.  That is all of the error beyond the output's own rounding (2.3e-4 of fp16's outputs for 2.1e-4 with weights in
-// f32, 1.9e-3 for 1.7e-3 of bf16's); a second part for what the rounding takes away would double V's products.  The running maximum moves only when a score passes it by some powers of two, so most tiles
+// Weights are rounded to the rows' type, which the matrix unit takes, and summed as rounded, and held times a power of two,
+// far above fp16's smallest.  That is all of the error beyond the output's own rounding (2.3e-4 of fp16's outputs for 2.1e-4
+// with weights in f32, 1.9e-3 for 1.7e-3 of bf16's); a second part for what the rounding takes away would double V's
+// products.  The running maximum moves only when a score passes it by some powers of two, so most tiles
 // rescale nothing.
 //
 // NaN.  Tokens that no column of a tile sees, and tokens that only some see, have weight 0 there, and 0 times what
